@@ -16,7 +16,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(CSRC, "libgeodiff_hip.so")
 ARCH = "gfx950"
-FLAGS = ["-O3", "-fPIC", "-std=c++17", f"--offload-arch={ARCH}", "-Wno-unused-result"]
+# no packed f32 arithmetic (v_pk_add/mul/fma_f32): some of its forms have given wrong results on gfx950
+FLAGS = ["-O3", "-fPIC", "-std=c++17", f"--offload-arch={ARCH}", "-Wno-unused-result", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 # per-file extras.  attn_fwd: -O3's SLP vectoriser packs the softmax's neighbouring f32 adds / multiplies into v_pk_*_f32, which cost
 # more issue time beside MFMAs than the single instructions they replace (MI355X_MICROARCH.md, per-instruction constants)
 EXTRA_FLAGS = {"attn_fwd.hip": ["-fno-slp-vectorize"], "attn_fwd_mp.hip": ["-fno-slp-vectorize"], "attn_bwd.hip": ["-fno-slp-vectorize"]}
