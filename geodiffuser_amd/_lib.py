@@ -67,6 +67,21 @@ class GdHeadsMerge(Structure):               # gd_heads_merge_t
                 ("src_f32", c_int32), ("B", c_int32), ("rows", c_int32), ("heads", c_int32), ("D", c_int32)]
 
 
+GD_NORM_NONE, GD_NORM_LAYER, GD_NORM_RMS = 0, 1, 2
+
+
+class GdBlockNorm(Structure):                # gd_block_norm_t
+    _fields_ = [("x", c_void_p), ("res", c_void_p), ("gate", c_void_p), ("post_gamma", c_void_p), ("post_beta", c_void_p), ("pre_gamma", c_void_p),
+                ("pre_beta", c_void_p), ("s", c_void_p), ("y", c_void_p), ("stats", c_void_p),
+                ("rows", c_int64), ("rows_per_gate", c_int64), ("gate_ld", c_int64),
+                ("C", c_int32), ("post_kind", c_int32), ("pre_kind", c_int32), ("post_eps", c_float), ("pre_eps", c_float), ("res_scale", c_float)]
+
+
+class GdBlockNormBwd(Structure):             # gd_block_norm_bwd_t
+    _fields_ = [("f", GdBlockNorm), ("gy", c_void_p), ("gs", c_void_p), ("dx", c_void_p), ("dres", c_void_p), ("dgate", c_void_p),
+                ("dpost_gamma", c_void_p), ("dpost_beta", c_void_p), ("dpre_gamma", c_void_p), ("dpre_beta", c_void_p)]
+
+
 class GeodiffError(RuntimeError):
     pass
 
@@ -141,6 +156,15 @@ SIGNATURES = {
     "gd_ddim_step_v": (c_int, [c_void_p, c_void_p, c_void_p, c_float, c_float, c_float, c_void_p, c_int64, c_int, c_void_p]),
     "gd_masked_latent_update": (c_int, [c_void_p, c_void_p, c_void_p, c_float, c_int, c_int, c_void_p, c_void_p]),
     "gd_sumsq": (c_int, [c_void_p, c_int64, c_void_p, c_void_p]),
+    "gd_embed": (c_int, [c_void_p, c_int, c_int64, c_void_p, c_int64, c_void_p, c_int, c_int, c_float, c_void_p, c_int, c_void_p]),
+    "gd_embed_bwd_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int]),
+    "gd_embed_bwd": (c_int, [c_void_p, c_int, c_int64, c_void_p, c_int64, c_int, c_int64, c_float, c_void_p, c_void_p, c_size_t, c_int, c_void_p]),
+    "gd_embed_pos_bwd": (c_int, [c_void_p, c_int64, c_int, c_int, c_int, c_void_p, c_int, c_void_p]),
+    "gd_block_norm": (c_int, [POINTER(GdBlockNorm), c_int, c_void_p]),
+    "gd_block_norm_bwd_workspace_bytes": (c_size_t, [c_int64, c_int, c_int64]),
+    "gd_block_norm_bwd": (c_int, [POINTER(GdBlockNormBwd), c_void_p, c_size_t, c_int, c_void_p]),
+    "gd_grad_norm_workspace_bytes": (c_size_t, []),
+    "gd_grad_norm": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_float, c_void_p, c_size_t, c_void_p, c_void_p]),
     "gd_norm_rescale": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p]),
 }
 

@@ -1,0 +1,489 @@
+// The norms before and after a transformer block, fused with the block's gate and the scaled residual:
+//
+//   h = post(x)                      norm on the block's output (or x itself)
+//   s = alpha * res + gate * h       the residual stream behind the block; gate [C], [groups, C] (one row per sample) or 1
+//   y = pre(s)                       norm in front of the next block
+//
+// with   layer: xh = (v - mean v) / sqrt(var v + eps)     rms: xh = v / sqrt(mean v^2 + eps)     norm(v) = xh * gamma + beta.
+//
+// Backward, for gy = dL/dy and gs = dL/ds (what reaches the stream behind y):
+//   ds   = N'(gy * gamma_pre, xh_s) + gs,     N'(g, xh) = r (g - mean g [layer only] - xh mean(g xh)),  r = 1 / deviation of the row
+//   dres = alpha ds;   dgate = sum ds h;   dh = gate ds;   dx = N'(dh * gamma_post, xh_x) or dh
+//   dgamma = sum g_out xh, dbeta = sum g_out over all rows, for each of the two norms.
+//
+// Bound by HBM: the forward reads x, res and writes s, y once, the backward reads x, res, gy, gs and writes dx, dres once.  A row stays in
+// registers from its load to its last use (64 / 256 / 1024 threads a row, 8 or 16 channels a thread), so that the two-pass variance and
+// both norms cost no second read.  Everything between the loads and the one rounding of each result is binary32; y comes from the sum s
+// BEFORE its rounding, and the backward recomputes that sum from x and res instead of reading the rounded s: the gradients are those of
+// the function that the forward computed, at the same traffic.
+#include "train_common.hpp"
+
+// How a thread's N channels lie in a row.  VEC: words of 16 bytes (8 or 4 channels), neighbouring threads on neighbouring words - needs
+// C * sizeof(T) and every pointer to be multiples of 16; otherwise element by element, neighbouring threads on neighbouring elements.
+template <typename T, int TPR, int N, bool VEC>
+struct bn_cols {
+    static constexpr int W = VEC ? (int)(16 / sizeof(T)) : 1;
+    static __device__ __forceinline__ int col(int t, int i) { return ((i / W) * TPR + t) * W + i % W; }
+    static __device__ __forceinline__ void load(const T* __restrict__ p, int t, int C, float* v) {
+#pragma unroll
+        for (int i = 0; i < N; i += W) {
+            const int c = col(t, i);
+            if (c < C) {
+                if constexpr (VEC) {
+                    const word16<T> a = *(const word16<T>*)(p + c);
+#pragma unroll
+                    for (int j = 0; j < W; ++j) v[i + j] = (float)a.v[j];
+                } else {
+                    v[i] = (float)p[c];
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < W; ++j) v[i + j] = 0.f;
+            }
+        }
+    }
+    static __device__ __forceinline__ void store(T* __restrict__ p, int t, int C, const float* v) {
+#pragma unroll
+        for (int i = 0; i < N; i += W) {
+            const int c = col(t, i);
+            if (c < C) {
+                if constexpr (VEC) {
+                    word16<T> a;
+#pragma unroll
+                    for (int j = 0; j < W; ++j) a.v[j] = to_storage<T>(v[i + j]);
+                    *(word16<T>*)(p + c) = a;
+                } else {
+                    p[c] = to_storage<T>(v[i]);
+                }
+            }
+        }
+    }
+};
+
+// sums of K values over the row's threads, in every one of them.  TPR > 64: `lds` holds 16 * K floats; the caller's row loop is uniform
+// over the workgroup, so the barriers are too.
+template <int TPR, int K>
+__device__ __forceinline__ void bn_row_sum(float* v, float* lds) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) v[k] = wave_sum(v[k]);
+    if constexpr (TPR > 64) {
+        constexpr int WAVES = TPR / 64;
+        __syncthreads();                                     // the previous sum has been read
+        if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+            for (int k = 0; k < K; ++k) lds[k * WAVES + (threadIdx.x >> 6)] = v[k];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            float s = 0.f;
+#pragma unroll
+            for (int w = 0; w < WAVES; ++w) s += lds[k * WAVES + w];
+            v[k] = s;
+        }
+    }
+}
+
+// v -> (mean, 1 / deviation); mean is 0 for the rms norm
+template <typename COLS, int TPR, int N>
+__device__ __forceinline__ void bn_stats(const float* v, int t, int C, int kind, float eps, float* lds, float& mean, float& r) {
+    mean = 0.f;
+    if (kind == GD_NORM_LAYER) {
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < N; ++i) s += v[i];
+        bn_row_sum<TPR, 1>(&s, lds);
+        mean = s / (float)C;
+    }
+    float q = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const float d = COLS::col(t, i) < C ? v[i] - mean : 0.f;
+        q = __builtin_fmaf(d, d, q);
+    }
+    bn_row_sum<TPR, 1>(&q, lds);
+    r = rsqrtf(q / (float)C + eps);
+}
+
+template <typename T, int TPR, int N, bool VEC>
+__global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) k_block_norm(const gd_block_norm_t a) {
+    using COLS = bn_cols<T, TPR, N, VEC>;
+    constexpr int RPB = TPR < 256 ? 256 / TPR : 1;           // rows a workgroup
+    __shared__ float lds[16];
+    const int t = threadIdx.x % TPR, C = a.C;
+    const long long row = (long long)blockIdx.x * RPB + threadIdx.x / TPR;
+    if (row >= a.rows) return;                               // TPR >= 256: the whole workgroup has one row
+    float h[N], v[N], w[N];
+    COLS::load((const T*)a.x + row * C, t, C, h);
+    if (a.post_kind) {
+        float mean, r;
+        bn_stats<COLS, TPR, N>(h, t, C, a.post_kind, a.post_eps, lds, mean, r);
+        if (a.stats && t == 0) { a.stats[row * 4] = mean; a.stats[row * 4 + 1] = r; }
+#pragma unroll
+        for (int i = 0; i < N; ++i) h[i] = COLS::col(t, i) < C ? (h[i] - mean) * r : 0.f;
+        if (a.post_gamma) {
+            COLS::load((const T*)a.post_gamma, t, C, w);
+#pragma unroll
+            for (int i = 0; i < N; ++i) h[i] *= w[i];
+        }
+        if (a.post_beta) {
+            COLS::load((const T*)a.post_beta, t, C, w);
+#pragma unroll
+            for (int i = 0; i < N; ++i) h[i] += w[i];
+        }
+    }
+    if (a.gate) {
+        COLS::load((const T*)a.gate + (row / a.rows_per_gate) * a.gate_ld, t, C, w);
+#pragma unroll
+        for (int i = 0; i < N; ++i) h[i] *= w[i];
+    }
+    if (a.res) {
+        COLS::load((const T*)a.res + row * C, t, C, v);
+#pragma unroll
+        for (int i = 0; i < N; ++i) h[i] = __builtin_fmaf(a.res_scale, v[i], h[i]);
+    }
+    if (a.s) COLS::store((T*)a.s + row * C, t, C, h);
+    if (!a.pre_kind) return;
+    float mean, r;
+    bn_stats<COLS, TPR, N>(h, t, C, a.pre_kind, a.pre_eps, lds, mean, r);
+    if (a.stats && t == 0) { a.stats[row * 4 + 2] = mean; a.stats[row * 4 + 3] = r; }
+#pragma unroll
+    for (int i = 0; i < N; ++i) h[i] = (h[i] - mean) * r;
+    if (a.pre_gamma) {
+        COLS::load((const T*)a.pre_gamma, t, C, w);
+#pragma unroll
+        for (int i = 0; i < N; ++i) h[i] *= w[i];
+    }
+    if (a.pre_beta) {
+        COLS::load((const T*)a.pre_beta, t, C, w);
+#pragma unroll
+        for (int i = 0; i < N; ++i) h[i] += w[i];
+    }
+    COLS::store((T*)a.y + row * C, t, C, h);
+}
+
+// ---- backward -------------------------------------------------------------------------------------------------------------------------
+// Workgroup w takes the rows [w * R, (w + 1) * R) in order; its threads keep the column sums of their channels in registers and leave
+// them in the workspace, one row of C floats for each sum: four sums over all rows (slot w) and the gate's, which ends wherever the rows
+// of one gate end.  Going through (w, gate row) in order, each step raises w or the gate row by one, so that slot w + gate row is
+// a workgroup's own.  k_block_norm_cols then adds the slots of each column in their order: no float atomics, the same bits every time.
+enum { BN_PRE_G, BN_PRE_B, BN_POST_G, BN_POST_B, BN_SUMS };
+
+struct bn_bwd_args {
+    gd_block_norm_bwd_t a;
+    float* sums[BN_SUMS];       // [workgroups, C] or null
+    float* gate_sums;           // [workgroups + gate rows - 1, C] or null
+    long long rows_per_wg;
+};
+
+// column sums of the workgroup's rows-in-parallel, then to the workspace (threads of the first row)
+template <typename COLS, int TPR, int N>
+__device__ __forceinline__ void bn_flush(float* acc, float* __restrict__ out, int C, float* lds) {
+    const int t = threadIdx.x % TPR;
+    if constexpr (TPR < 256) {                               // one wave a row: the four waves' sums meet in LDS
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < N; ++i) lds[(threadIdx.x >> 6) * (64 * N) + i * 64 + t] = acc[i];
+        __syncthreads();
+        if (threadIdx.x < 64) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int c = COLS::col(t, i);
+                if (c < C) out[c] = (lds[i * 64 + t] + lds[64 * N + i * 64 + t]) + (lds[2 * 64 * N + i * 64 + t] + lds[3 * 64 * N + i * 64 + t]);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int c = COLS::col(t, i);
+            if (c < C) out[c] = acc[i];
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) acc[i] = 0.f;
+}
+
+template <typename T, int TPR, int N, bool VEC>
+__global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) k_block_norm_bwd(const bn_bwd_args b) {
+    using COLS = bn_cols<T, TPR, N, VEC>;
+    constexpr int RPB = TPR < 256 ? 256 / TPR : 1;
+    __shared__ float lds[TPR < 256 ? 4 * 64 * N : 32];
+    const gd_block_norm_bwd_t& a = b.a;
+    const int t = threadIdx.x % TPR, C = a.f.C;
+    const long long r0 = (long long)blockIdx.x * b.rows_per_wg, r1 = r0 + b.rows_per_wg < a.f.rows ? r0 + b.rows_per_wg : a.f.rows;
+    float acc[BN_SUMS][N] = {}, acc_gate[N] = {};
+    const long long per = a.f.gate ? a.f.rows_per_gate : a.f.rows;
+    for (long long g0 = r0; g0 < r1;) {
+        const long long gate_row = g0 / per;
+        const long long g1 = (gate_row + 1) * per < r1 ? (gate_row + 1) * per : r1;
+        for (long long base = g0; base < g1; base += RPB) {
+            const long long row = base + threadIdx.x / TPR;
+            if (row < g1) {                                  // (TPR >= 256: the same for the whole workgroup)
+                float h[N], xh[N], sv[N], w[N], d[N];
+                // forward again: xh = normalised x, h = post(x), sv = the sum
+                COLS::load((const T*)a.f.x + row * C, t, C, xh);
+                float post_r = 1.f;
+                if (a.f.post_kind) {
+                    const float mean = a.f.stats[row * 4];
+                    post_r = a.f.stats[row * 4 + 1];
+#pragma unroll
+                    for (int i = 0; i < N; ++i) h[i] = xh[i] = COLS::col(t, i) < C ? (xh[i] - mean) * post_r : 0.f;
+                    if (a.f.post_gamma) {
+                        COLS::load((const T*)a.f.post_gamma, t, C, w);
+#pragma unroll
+                        for (int i = 0; i < N; ++i) h[i] *= w[i];
+                    }
+                    if (a.f.post_beta) {
+                        COLS::load((const T*)a.f.post_beta, t, C, w);
+#pragma unroll
+                        for (int i = 0; i < N; ++i) h[i] += w[i];
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < N; ++i) h[i] = xh[i];
+                }
+                float gate[N];
+                if (a.f.gate) {
+                    COLS::load((const T*)a.f.gate + gate_row * a.f.gate_ld, t, C, gate);
+#pragma unroll
+                    for (int i = 0; i < N; ++i) sv[i] = gate[i] * h[i];
+                } else {
+#pragma unroll
+                    for (int i = 0; i < N; ++i) sv[i] = h[i];
+                }
+                if (a.f.res) {
+                    COLS::load((const T*)a.f.res + row * C, t, C, w);
+#pragma unroll
+                    for (int i = 0; i < N; ++i) sv[i] = __builtin_fmaf(a.f.res_scale, w[i], sv[i]);
+                }
+                // ds
+                if (a.gy) {
+                    const float mean = a.f.stats[row * 4 + 2], r = a.f.stats[row * 4 + 3];
+                    COLS::load((const T*)a.gy + row * C, t, C, d);
+                    float m[2] = {0.f, 0.f};
+                    if (a.f.pre_gamma) {
+                        COLS::load((const T*)a.f.pre_gamma, t, C, w);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < N; ++i) w[i] = 1.f;
+                    }
+#pragma unroll
+                    for (int i = 0; i < N; ++i) {
+                        sv[i] = COLS::col(t, i) < C ? (sv[i] - mean) * r : 0.f;
+                        acc[BN_PRE_G][i] = __builtin_fmaf(d[i], sv[i], acc[BN_PRE_G][i]);
+                        acc[BN_PRE_B][i] += d[i];
+                        d[i] *= w[i];
+                        m[0] += d[i];
+                        m[1] = __builtin_fmaf(d[i], sv[i], m[1]);
+                    }
+                    bn_row_sum<TPR, 2>(m, lds);
+                    const float m0 = a.f.pre_kind == GD_NORM_LAYER ? m[0] / (float)C : 0.f, m1 = m[1] / (float)C;
+#pragma unroll
+                    for (int i = 0; i < N; ++i) d[i] = r * (d[i] - m0 - sv[i] * m1);
+                    if (a.gs) {
+                        COLS::load((const T*)a.gs + row * C, t, C, w);
+#pragma unroll
+                        for (int i = 0; i < N; ++i) d[i] += w[i];
+                    }
+                } else {
+                    COLS::load((const T*)a.gs + row * C, t, C, d);
+                }
+                if (a.dres) {
+#pragma unroll
+                    for (int i = 0; i < N; ++i) w[i] = a.f.res_scale * d[i];
+                    COLS::store((T*)a.dres + row * C, t, C, w);
+                }
+                if (a.f.gate) {
+#pragma unroll
+                    for (int i = 0; i < N; ++i) {
+                        if (COLS::col(t, i) < C) acc_gate[i] = __builtin_fmaf(d[i], h[i], acc_gate[i]);
+                        d[i] *= gate[i];
+                    }
+                }
+                if (a.f.post_kind) {
+                    float m[2] = {0.f, 0.f};
+                    if (a.f.post_gamma) {
+                        COLS::load((const T*)a.f.post_gamma, t, C, w);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < N; ++i) w[i] = 1.f;
+                    }
+#pragma unroll
+                    for (int i = 0; i < N; ++i) {
+                        if (COLS::col(t, i) >= C) d[i] = 0.f;
+                        acc[BN_POST_G][i] = __builtin_fmaf(d[i], xh[i], acc[BN_POST_G][i]);
+                        acc[BN_POST_B][i] += d[i];
+                        d[i] *= w[i];
+                        m[0] += d[i];
+                        m[1] = __builtin_fmaf(d[i], xh[i], m[1]);
+                    }
+                    bn_row_sum<TPR, 2>(m, lds);
+                    const float m0 = a.f.post_kind == GD_NORM_LAYER ? m[0] / (float)C : 0.f, m1 = m[1] / (float)C;
+#pragma unroll
+                    for (int i = 0; i < N; ++i) d[i] = post_r * (d[i] - m0 - xh[i] * m1);
+                }
+                if (a.dx) COLS::store((T*)a.dx + row * C, t, C, d);
+            }
+        }
+        if (b.gate_sums) bn_flush<COLS, TPR, N>(acc_gate, b.gate_sums + ((long long)blockIdx.x + gate_row) * C, C, lds);
+        g0 = g1;
+    }
+#pragma unroll
+    for (int k = 0; k < BN_SUMS; ++k)
+        if (b.sums[k]) bn_flush<COLS, TPR, N>(acc[k], b.sums[k] + (long long)blockIdx.x * C, C, lds);
+}
+
+// out[c] = sum over the slots of one sum.  blockIdx.y < BN_SUMS: a sum over all workgroups; above: the gate row blockIdx.y - BN_SUMS, which
+// workgroups floor(g per / R) .. floor((g per + per - 1) / R) have.  64 channels a workgroup, 16 slots side by side.
+template <typename T>
+__global__ void __launch_bounds__(1024) k_block_norm_cols(const bn_bwd_args b, int workgroups) {
+    __shared__ float lds[16][65];
+    const gd_block_norm_bwd_t& a = b.a;
+    const int C = a.f.C, c = blockIdx.x * 64 + (threadIdx.x & 63), lane = threadIdx.x >> 6;
+    const float* src;
+    T* out;
+    long long lo = 0, hi = workgroups;
+    if (blockIdx.y < BN_SUMS) {
+        void* const dst[BN_SUMS] = {a.dpre_gamma, a.dpre_beta, a.dpost_gamma, a.dpost_beta};
+        src = b.sums[blockIdx.y];
+        out = (T*)dst[blockIdx.y];
+        if (!src) return;
+    } else {
+        const long long g = blockIdx.y - BN_SUMS, per = a.f.rows_per_gate;
+        lo = g * per / b.rows_per_wg;
+        hi = ((g + 1) * per - 1) / b.rows_per_wg + 1;
+        src = b.gate_sums + g * C;
+        out = (T*)a.dgate + g * C;
+    }
+    float s = 0.f;
+    if (c < C)
+        for (long long i = lo + lane; i < hi; i += 16) s += src[i * C + c];
+    lds[lane][threadIdx.x & 63] = s;
+    __syncthreads();
+    if (lane == 0 && c < C) {
+        s = lds[0][threadIdx.x];
+#pragma unroll
+        for (int w = 1; w < 16; ++w) s += lds[w][threadIdx.x];
+        out[c] = to_storage<T>(s);
+    }
+}
+
+static bool bn_aligned(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+static bool bn_vec(const gd_block_norm_t& f, int elem) {
+    return f.C * elem % 16 == 0 && bn_aligned(f.x) && bn_aligned(f.res) && bn_aligned(f.gate) && (!f.gate || f.gate_ld * elem % 16 == 0) &&
+           bn_aligned(f.post_gamma) && bn_aligned(f.post_beta) && bn_aligned(f.pre_gamma) && bn_aligned(f.pre_beta) && bn_aligned(f.s) && bn_aligned(f.y);
+}
+
+#define BN_MAX_C 16384
+
+// threads a row: a wave up to 1024 channels (no barrier), then 256 up to 4096, then 1024; 8 channels a thread where they suffice
+#define BN_SHAPE(C, X)                                                                                        \
+    do {                                                                                                      \
+        if ((C) <= 512) X(64, 8);                                                                             \
+        else if ((C) <= 1024) X(64, 16);                                                                      \
+        else if ((C) <= 2048) X(256, 8);                                                                      \
+        else if ((C) <= 4096) X(256, 16);                                                                     \
+        else if ((C) <= 8192) X(1024, 8);                                                                     \
+        else X(1024, 16);                                                                                     \
+    } while (0)
+
+static int bn_check(const gd_block_norm_t* f, int dtype, const char* who) {
+    GD_REQUIRE(f && f->x, GD_EINVAL, "%s: null pointer", who);
+    GD_REQUIRE(f->rows > 0 && f->C > 0, GD_EINVAL, "%s: rows and C must be positive", who);
+    GD_REQUIRE(f->C <= BN_MAX_C, GD_EUNSUPPORTED, "%s: at most %d channels (C=%d)", who, BN_MAX_C, f->C);
+    GD_REQUIRE(f->rows < (1ll << 31), GD_EUNSUPPORTED, "%s: too many rows", who);
+    GD_REQUIRE(f->post_kind >= 0 && f->post_kind <= GD_NORM_RMS && f->pre_kind >= 0 && f->pre_kind <= GD_NORM_RMS, GD_EINVAL, "%s: bad norm kind", who);
+    GD_REQUIRE(!f->gate || (f->rows_per_gate > 0 && f->rows % f->rows_per_gate == 0 && f->gate_ld >= f->C), GD_EINVAL,
+               "%s: gate rows must divide the rows and be at least C apart", who);
+    GD_REQUIRE(!f->gate || f->rows / f->rows_per_gate <= 65535 - BN_SUMS, GD_EUNSUPPORTED, "%s: at most %d gate rows", who, 65535 - BN_SUMS);
+    GD_REQUIRE(dtype == GD_F16 || dtype == GD_BF16 || dtype == GD_F32, GD_EINVAL, "%s: dtype must be f16/bf16/f32", who);
+    return GD_OK;
+}
+
+template <typename T>
+static void bn_launch(const gd_block_norm_t& a, hipStream_t st) {
+    const bool vec = bn_vec(a, sizeof(T));
+#define BN_GO(TPR, N)                                                                                         \
+    do {                                                                                                      \
+        constexpr int rpb = TPR < 256 ? 256 / TPR : 1;                                                        \
+        const unsigned grid = (unsigned)((a.rows + rpb - 1) / rpb);                                           \
+        if (vec) k_block_norm<T, TPR, N, true><<<grid, rpb * TPR, 0, st>>>(a);                                \
+        else k_block_norm<T, TPR, N, false><<<grid, rpb * TPR, 0, st>>>(a);                                   \
+    } while (0)
+    BN_SHAPE(a.C, BN_GO);
+#undef BN_GO
+}
+
+extern "C" int gd_block_norm(const gd_block_norm_t* f, int dtype, void* stream) {
+    const int rc = bn_check(f, dtype, "gd_block_norm");
+    if (rc != GD_OK) return rc;
+    GD_REQUIRE(f->s || f->y, GD_EINVAL, "gd_block_norm: no output");
+    GD_REQUIRE(!f->pre_kind == !f->y, GD_EINVAL, "gd_block_norm: y goes with the norm in front of the next block");
+    hipStream_t st = as_stream(stream);
+    if (dtype == GD_F32) bn_launch<float>(*f, st);
+    else if (dtype == GD_F16) bn_launch<f16_t>(*f, st);
+    else bn_launch<bf16_t>(*f, st);
+    GD_CHECK_LAUNCH("gd_block_norm");
+    return GD_OK;
+}
+
+// Two workgroups of four waves a CU cover the row's latencies; every further one costs BN_SUMS more rows of partial sums to write and
+// add.  At least 4 rows each.
+static long long bn_workgroups(long long rows) {
+    const long long n = (rows + 3) / 4;
+    return n < 512 ? n : 512;
+}
+
+extern "C" size_t gd_block_norm_bwd_workspace_bytes(int64_t rows, int C, int64_t gate_rows) {
+    const long long wg = bn_workgroups(rows);
+    return sizeof(float) * (size_t)C * (size_t)(BN_SUMS * wg + (gate_rows > 0 ? wg + gate_rows - 1 : 0));
+}
+
+template <typename T>
+static void bn_launch_bwd(const gd_block_norm_bwd_t& a, float* ws, hipStream_t st) {
+    bn_bwd_args b;
+    b.a = a;
+    const long long wg0 = bn_workgroups(a.f.rows);
+    b.rows_per_wg = (a.f.rows + wg0 - 1) / wg0;
+    const int wg = (int)((a.f.rows + b.rows_per_wg - 1) / b.rows_per_wg);
+    void* const dst[BN_SUMS] = {a.dpre_gamma, a.dpre_beta, a.dpost_gamma, a.dpost_beta};
+    int any = 0;
+    for (int k = 0; k < BN_SUMS; ++k) {
+        b.sums[k] = dst[k] ? ws + (size_t)k * wg0 * a.f.C : nullptr;
+        any |= dst[k] != nullptr;
+    }
+    b.gate_sums = a.dgate ? ws + (size_t)BN_SUMS * wg0 * a.f.C : nullptr;
+    const bool vec = bn_vec(a.f, sizeof(T)) && bn_aligned(a.gy) && bn_aligned(a.gs) && bn_aligned(a.dx) && bn_aligned(a.dres);
+#define BN_GO(TPR, N)                                                                                         \
+    do {                                                                                                      \
+        if (vec) k_block_norm_bwd<T, TPR, N, true><<<wg, TPR < 256 ? 256 : TPR, 0, st>>>(b);                  \
+        else k_block_norm_bwd<T, TPR, N, false><<<wg, TPR < 256 ? 256 : TPR, 0, st>>>(b);                     \
+    } while (0)
+    BN_SHAPE(a.f.C, BN_GO);
+#undef BN_GO
+    const int gates = a.dgate ? (int)(a.f.rows / a.f.rows_per_gate) : 0;
+    if (any || gates) k_block_norm_cols<T><<<dim3((a.f.C + 63) / 64, BN_SUMS + gates), 1024, 0, st>>>(b, wg);
+}
+
+extern "C" int gd_block_norm_bwd(const gd_block_norm_bwd_t* a, void* workspace, size_t workspace_bytes, int dtype, void* stream) {
+    GD_REQUIRE(a, GD_EINVAL, "gd_block_norm_bwd: null pointer");
+    const int rc = bn_check(&a->f, dtype, "gd_block_norm_bwd");
+    if (rc != GD_OK) return rc;
+    GD_REQUIRE(a->gy || a->gs, GD_EINVAL, "gd_block_norm_bwd: no incoming gradient");
+    GD_REQUIRE(!a->gy || a->f.pre_kind, GD_EINVAL, "gd_block_norm_bwd: gy goes with the norm in front of the next block");
+    GD_REQUIRE(a->f.stats || (!a->gy && !a->f.post_kind), GD_EINVAL, "gd_block_norm_bwd: the forward's stats are needed");
+    GD_REQUIRE(a->gy || (!a->dpre_gamma && !a->dpre_beta), GD_EINVAL, "gd_block_norm_bwd: dpre_gamma / dpre_beta need gy");
+    GD_REQUIRE(a->f.post_kind || (!a->dpost_gamma && !a->dpost_beta), GD_EINVAL, "gd_block_norm_bwd: dpost_gamma / dpost_beta need the norm on x");
+    GD_REQUIRE(a->f.gate || !a->dgate, GD_EINVAL, "gd_block_norm_bwd: dgate needs the gate");
+    GD_REQUIRE(a->f.res || !a->dres, GD_EINVAL, "gd_block_norm_bwd: dres needs the residual");
+    const bool sums = a->dpre_gamma || a->dpre_beta || a->dpost_gamma || a->dpost_beta || a->dgate;
+    const size_t need = sums ? gd_block_norm_bwd_workspace_bytes(a->f.rows, a->f.C, a->dgate ? a->f.rows / a->f.rows_per_gate : 0) : 0;
+    GD_REQUIRE(!need || (workspace && workspace_bytes >= need), GD_EWORKSPACE, "gd_block_norm_bwd: workspace of %zu bytes needed", need);
+    hipStream_t st = as_stream(stream);
+    if (dtype == GD_F32) bn_launch_bwd<float>(*a, (float*)workspace, st);
+    else if (dtype == GD_F16) bn_launch_bwd<f16_t>(*a, (float*)workspace, st);
+    else bn_launch_bwd<bf16_t>(*a, (float*)workspace, st);
+    GD_CHECK_LAUNCH("gd_block_norm_bwd");
+    return GD_OK;
+}

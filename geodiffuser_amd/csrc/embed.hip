@@ -1,0 +1,566 @@
+// Token embedding with scaling, and its gradients.
+//
+//   y[i] = scale * W[id[i]] + P[i mod L]                      (rows of C channels; P optional)
+//   dW[v] = scale * sum over {i: id[i] = v} of dy[i]          dP[l] = sum over the sequences of dy[b, l]
+//
+// Every row of dW is written: the rows of no token with zeros.  A row's terms are added in binary32 in the order of their positions (dealt
+// out to a fixed number of partial sums), without float atomics: the same inputs give the same bits.
+// Bound by HBM (dy once, the table's gradient once); for a few prompts by the launch.
+#include "train_common.hpp"
+
+// A lane's N channels of a slice of 64 * N: one word of 16 bytes (VEC: C * sizeof(T) and all pointers are multiples of 16), or N single
+// elements, neighbouring lanes on neighbouring elements.
+template <typename T, bool VEC>
+struct em_cols {
+    static constexpr int N = VEC ? (int)(16 / sizeof(T)) : 8, SLICE = 64 * N;
+    static __device__ __forceinline__ int col(int slice, int lane, int i) { return slice * SLICE + (VEC ? lane * N + i : i * 64 + lane); }
+    static __device__ __forceinline__ void load(const T* __restrict__ p, int slice, int lane, int C, float* v) {
+        if constexpr (VEC) {
+            const int c = col(slice, lane, 0);
+            word16<T> a = {};
+            if (c < C) a = *(const word16<T>*)(p + c);
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[i] = (float)a.v[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int c = col(slice, lane, i);
+                v[i] = c < C ? (float)p[c] : 0.f;
+            }
+        }
+    }
+    static __device__ __forceinline__ void store(T* __restrict__ p, int slice, int lane, int C, const float* v) {
+        if constexpr (VEC) {
+            const int c = col(slice, lane, 0);
+            word16<T> a;
+#pragma unroll
+            for (int i = 0; i < N; ++i) a.v[i] = to_storage<T>(v[i]);
+            if (c < C) *(word16<T>*)(p + c) = a;
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int c = col(slice, lane, i);
+                if (c < C) p[c] = to_storage<T>(v[i]);
+            }
+        }
+    }
+};
+
+struct em_ids {
+    const void* p;
+    int wide;                   // 64-bit ids
+    __device__ __forceinline__ long long operator[](long long i) const { return wide ? ((const long long*)p)[i] : (long long)((const int*)p)[i]; }
+};
+
+// one wave a row; an id outside the table gives a row of NaN (there is no such row, and no way to raise from here)
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256) k_embed(const em_ids ids, long long n, const T* __restrict__ table, const T* __restrict__ pos, int L, int V, int C,
+                                               float scale, T* __restrict__ y) {
+    using COLS = em_cols<T, VEC>;
+    const int lane = threadIdx.x & 63;
+    const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (row >= n) return;
+    const long long id = ids[row];
+    const bool in = id >= 0 && id < V;
+    const T* src = table + (in ? id : 0) * C;
+    const T* ps = pos ? pos + (row % L) * C : nullptr;
+    for (int sl = 0; sl * COLS::SLICE < C; ++sl) {
+        float v[COLS::N], q[COLS::N] = {};
+        COLS::load(src, sl, lane, C, v);
+        if (ps) COLS::load(ps, sl, lane, C, q);
+#pragma unroll
+        for (int i = 0; i < COLS::N; ++i) {
+            v[i] = in ? __builtin_fmaf(scale, v[i], q[i]) : __builtin_nanf("");
+        }
+        COLS::store(y + row * C, sl, lane, C, v);
+    }
+}
+
+// sum of the four waves' values, in wave 0
+template <int N>
+__device__ __forceinline__ void em_fold(float* v, float (*lds)[64 * N], int wave, int lane) {
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; ++i) lds[wave][i * 64 + lane] = v[i];
+    __syncthreads();
+    if (wave == 0) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = (lds[0][i * 64 + lane] + lds[1][i * 64 + lane]) + (lds[2][i * 64 + lane] + lds[3][i * 64 + lane]);
+    }
+}
+
+// rows of the table that a workgroup looks after for zeros
+#define EM_ZERO_ROWS 16
+
+// The first workgroups: (position, slice).  The one at a token's first position adds up all of that token's rows; the others end at once.
+// The workgroups behind them: EM_ZERO_ROWS rows of the table each, zeros where no position has the row's token.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256) k_embed_bwd_scan(const em_ids ids, int n, const T* __restrict__ dy, int V, int C, long long padding, float scale,
+                                                        T* __restrict__ dtable) {
+    using COLS = em_cols<T, VEC>;
+    constexpr int N = COLS::N;
+    __shared__ float lds[4][64 * N];
+    __shared__ int list[256], count[4];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int slices = (C + COLS::SLICE - 1) / COLS::SLICE;
+    const long long owners = (long long)n * slices;
+    if (blockIdx.x < owners) {
+        const int first = (int)(blockIdx.x / slices), sl = (int)(blockIdx.x % slices);
+        const long long id = ids[first];
+        if (id < 0 || id >= V || id == padding) return;
+        bool before = false;
+        for (int j = tid; j < first; j += 256) before |= ids[j] == id;
+        if (__syncthreads_or(before)) return;
+        float acc[N] = {};
+        for (int base = first; base < n; base += 256) {
+            const int j = base + tid;
+            const bool mine = j < n && ids[j] == id;
+            const unsigned long long mask = __ballot(mine);
+            if (lane == 0) count[wave] = __popcll(mask);
+            __syncthreads();
+            int at = 0, total = 0;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                if (w < wave) at += count[w];
+                total += count[w];
+            }
+            if (mine) list[at + __popcll(mask & ((1ull << lane) - 1))] = j;
+            __syncthreads();
+#pragma unroll 4
+            for (int m = wave; m < total; m += 4) {
+                float v[N];
+                COLS::load(dy + (long long)list[m] * C, sl, lane, C, v);
+#pragma unroll
+                for (int i = 0; i < N; ++i) acc[i] += v[i];
+            }
+            __syncthreads();
+        }
+        em_fold<N>(acc, lds, wave, lane);
+        if (wave == 0) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) acc[i] *= scale;
+            COLS::store(dtable + id * C, sl, lane, C, acc);
+        }
+        return;
+    }
+    const long long v0 = ((long long)blockIdx.x - owners) * EM_ZERO_ROWS;
+    int* there = list;
+    if (tid < EM_ZERO_ROWS) there[tid] = 0;
+    __syncthreads();
+    for (int j = tid; j < n; j += 256) {
+        const long long id = ids[j];
+        if (id >= v0 && id < v0 + EM_ZERO_ROWS && id != padding) there[id - v0] = 1;
+    }
+    __syncthreads();
+    const float zero[N] = {};
+    for (int r = wave; r < EM_ZERO_ROWS; r += 4)
+        if (v0 + r < V && !there[r])
+            for (int sl = 0; sl < slices; ++sl) COLS::store(dtable + (v0 + r) * C, sl, lane, C, zero);
+}
+
+// ---- many positions: the positions sorted by token ---------------------------------------------------------------------------------------
+// A stable least-significant-digit radix sort of (token, position), 8 bits a pass, two launches each.  Ids that add nothing get the key
+// `vocab` and end up last.  A workgroup counts / moves EM_SORT_KEYS consecutive entries or more, each of its four waves a run of them; the
+// rank among equal digits of a round of 64 is a match of the digit's bits over the wave, so that the order of equal tokens is that of their
+// positions.  The scatter's workgroups each add up the whole table of counts themselves (at most EM_SORT_BLOCKS rows of 256): a launch
+// less than a scan would need.
+#define EM_SORT_KEYS 2048
+#define EM_SORT_BLOCKS 512
+
+struct em_sort {
+    long long n;
+    int per_block;              // a multiple of 256
+    int blocks;
+};
+
+static em_sort em_sort_of(long long n) {
+    long long blocks = (n + EM_SORT_KEYS - 1) / EM_SORT_KEYS;
+    if (blocks > EM_SORT_BLOCKS) blocks = EM_SORT_BLOCKS;
+    const long long per = ((n + blocks - 1) / blocks + 255) / 256 * 256;
+    return em_sort{n, (int)per, (int)((n + per - 1) / per)};
+}
+
+struct em_keys {                // a pass's input: the ids themselves, or the last pass's output
+    em_ids ids;
+    const uint32_t *key, *pos;
+    unsigned vocab;
+    long long padding;
+    __device__ __forceinline__ uint32_t operator()(long long i) const {
+        if (key) return key[i];
+        const long long id = ids[i];
+        return id >= 0 && id < (long long)vocab && id != padding ? (uint32_t)id : vocab;
+    }
+};
+
+// lanes of the wave whose digit is this lane's (0 for lanes without a key)
+__device__ __forceinline__ unsigned long long em_match(int digit, bool live) {
+    unsigned long long m = __ballot(live);
+#pragma unroll
+    for (int b = 0; b < 8; ++b) {
+        const unsigned long long s = __ballot((digit >> b) & 1);
+        m &= (digit >> b) & 1 ? s : ~s;
+    }
+    return live ? m : 0;
+}
+
+// counts[digit] += occurrences in the wave's entries [lo, hi)
+__device__ __forceinline__ void em_count(const em_keys& k, long long lo, long long hi, int shift, volatile int* counts) {
+    const int lane = threadIdx.x & 63;
+    for (long long base = lo; base < hi; base += 64) {
+        const long long i = base + lane;
+        const bool live = i < hi;
+        const int d = live ? (int)(k(i) >> shift) & 255 : 0;
+        const unsigned long long m = em_match(d, live);
+        if (live && (m & ((1ull << lane) - 1)) == 0) counts[d] += __popcll(m);
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
+__global__ void __launch_bounds__(256) k_embed_sort_count(const em_keys k, const em_sort s, int shift, int* __restrict__ table, uint32_t* __restrict__ there, int there_words) {
+    __shared__ int counts[4][256];
+    const int wave = threadIdx.x >> 6;
+    for (int i = threadIdx.x; i < 4 * 256; i += 256) counts[0][i] = 0;
+    // the first pass also clears the marks of the tokens that occur, for the last one
+    for (int i = blockIdx.x * 256 + threadIdx.x; i < there_words; i += gridDim.x * 256) there[i] = 0;
+    __syncthreads();
+    const long long run = s.per_block / 4, lo = (long long)blockIdx.x * s.per_block + wave * run, hi = lo + run < s.n ? lo + run : s.n;
+    em_count(k, lo, hi, shift, counts[wave]);
+    __syncthreads();
+    table[blockIdx.x * 256 + threadIdx.x] = counts[0][threadIdx.x] + counts[1][threadIdx.x] + counts[2][threadIdx.x] + counts[3][threadIdx.x];
+}
+
+__global__ void __launch_bounds__(256) k_embed_sort_move(const em_keys k, const em_sort s, int shift, const int* __restrict__ table, uint32_t* __restrict__ key_out,
+                                                         uint32_t* __restrict__ pos_out, unsigned char* __restrict__ there) {
+    __shared__ int counts[4][256], scan[256];
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+    for (int i = tid; i < 4 * 256; i += 256) counts[0][i] = 0;
+    // thread = digit: how many entries of it lie in earlier workgroups, and in all
+    int before = 0, all = 0;
+#pragma unroll 8
+    for (int b = 0; b < s.blocks; ++b) {
+        const int c = table[b * 256 + tid];
+        before += b < (int)blockIdx.x ? c : 0;
+        all += c;
+    }
+    scan[tid] = all;
+    __syncthreads();
+    const long long run = s.per_block / 4, lo = (long long)blockIdx.x * s.per_block + wave * run, hi = lo + run < s.n ? lo + run : s.n;
+    em_count(k, lo, hi, shift, counts[wave]);
+#pragma unroll
+    for (int o = 1; o < 256; o <<= 1) {                      // inclusive scan over the digits
+        const int v = tid >= o ? scan[tid - o] : 0;
+        __syncthreads();
+        scan[tid] += v;
+        __syncthreads();
+    }
+    int at = scan[tid] - all + before;                       // first place of this digit's entries of this workgroup
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        const int c = counts[w][tid];
+        counts[w][tid] = at;
+        at += c;
+    }
+    __syncthreads();
+    volatile int* place = counts[wave];
+    for (long long base = lo; base < hi; base += 64) {
+        const long long i = base + lane;
+        const bool live = i < hi;
+        const uint32_t key = live ? k(i) : 0;
+        const int d = (int)(key >> shift) & 255;
+        const unsigned long long m = em_match(d, live);
+        const int rank = __popcll(m & ((1ull << lane) - 1));
+        const int first = live ? place[d] : 0;
+        __builtin_amdgcn_wave_barrier();
+        if (live && rank == 0) place[d] = first + __popcll(m);
+        __builtin_amdgcn_wave_barrier();
+        if (live) {
+            key_out[first + rank] = key;
+            pos_out[first + rank] = k.key ? k.pos[i] : (uint32_t)i;
+            if (there && key < k.vocab) there[key] = 1;
+        }
+    }
+}
+
+// Sums over the sorted entries: a wave takes `tile` of them (at most 64) and one slice of channels, and writes each token whose entries all
+// lie in its tile.  A token that goes on beyond a border of the tile leaves a partial sum: `head` if its first entry lies before the
+// tile, `tail` if it begins in it.  The workgroups behind those write the zero rows.
+struct em_sum {
+    const uint32_t *key, *pos;
+    const unsigned char* there;
+    float *head, *tail;         // [tiles, C]
+    long long n;
+    int tile, tiles, slices, C;
+    unsigned vocab;
+    float scale;
+};
+
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256) k_embed_bwd_sum(const em_sum a, const T* __restrict__ dy, T* __restrict__ dtable) {
+    using COLS = em_cols<T, VEC>;
+    constexpr int N = COLS::N, AHEAD = 8;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, C = a.C;
+    const long long items = (long long)a.tiles * a.slices;
+    const long long item_blocks = (items + 3) / 4;
+    if (blockIdx.x < item_blocks) {
+        const long long item = (long long)blockIdx.x * 4 + wave;
+        if (item >= items) return;
+        const int t = (int)(item / a.slices), sl = (int)(item % a.slices);
+        const long long e0 = (long long)t * a.tile;
+        // lane = entry: its key, its position, whether it is its token's last one
+        const bool mine = lane < a.tile && e0 + lane < a.n;
+        const uint32_t key = mine ? a.key[e0 + lane] : a.vocab, pos = mine ? a.pos[e0 + lane] : 0;
+        const uint32_t next = mine && e0 + lane + 1 < a.n ? a.key[e0 + lane + 1] : 0xffffffffu;
+        const uint32_t prev = e0 > 0 ? a.key[e0 - 1] : 0xffffffffu;
+        const unsigned long long ends = __ballot(key != next);
+        const int live = __popcll(__ballot(key < a.vocab));  // sorted: the entries without a row of the table are the last ones
+        bool from_before = prev == (uint32_t)__builtin_amdgcn_readfirstlane((int)key);
+        float acc[N] = {};
+        for (int e = 0; e < live; e += AHEAD) {
+            float v[AHEAD][N];
+#pragma unroll
+            for (int j = 0; j < AHEAD; ++j) {                // (the last entry again instead of a branch between the loads)
+                const int at = e + j < live ? e + j : live - 1;
+                COLS::load(dy + (long long)(uint32_t)__builtin_amdgcn_readlane((int)pos, at) * C, sl, lane, C, v[j]);
+            }
+#pragma unroll
+            for (int j = 0; j < AHEAD; ++j) {
+                if (e + j >= live) break;
+#pragma unroll
+                for (int i = 0; i < N; ++i) acc[i] += v[j][i];
+                if ((ends >> (e + j)) & 1) {
+                    if (from_before) {
+#pragma unroll
+                        for (int i = 0; i < N; ++i) if (COLS::col(sl, lane, i) < C) a.head[(long long)t * C + COLS::col(sl, lane, i)] = acc[i];
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < N; ++i) acc[i] *= a.scale;
+                        COLS::store(dtable + (long long)(uint32_t)__builtin_amdgcn_readlane((int)key, e + j) * C, sl, lane, C, acc);
+                    }
+#pragma unroll
+                    for (int i = 0; i < N; ++i) acc[i] = 0.f;
+                    from_before = false;
+                }
+            }
+        }
+        if (live > 0 && !((ends >> (live - 1)) & 1)) {
+            float* part = from_before ? a.head : a.tail;
+#pragma unroll
+            for (int i = 0; i < N; ++i) if (COLS::col(sl, lane, i) < C) part[(long long)t * C + COLS::col(sl, lane, i)] = acc[i];
+        }
+        return;
+    }
+    const float zero[N] = {};
+    const long long v0 = ((long long)blockIdx.x - item_blocks) * EM_ZERO_ROWS;
+    for (int r = wave; r < EM_ZERO_ROWS; r += 4)
+        if (v0 + r < a.vocab && !a.there[v0 + r])
+            for (int sl = 0; sl < a.slices; ++sl) COLS::store(dtable + (v0 + r) * C, sl, lane, C, zero);
+}
+
+// The tokens whose entries go over a tile's border: the tail of the tile where they begin + the heads of the tiles that they go on into.
+// Most go over one border: the first workgroups each look at one tile's end and take up to EM_LONG - 1 heads, 1024 channels wide.
+// A token with more (padding has half of all tiles) is the work of the workgroups behind them, 16 channels and 64 tiles side by side: among
+// EM_LONG tiles in a row one has a multiple of EM_LONG as its number, and the first such tile's workgroups do it.
+#define EM_LONG 64
+
+// tile u begins with an entry of `key` and so ends tile u - 1
+__device__ __forceinline__ bool em_goes_on(const em_sum& a, long long u, uint32_t key) {
+    return u > 0 && u < a.tiles && a.key[u * a.tile] == key && a.key[u * a.tile - 1] == key;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(1024) k_embed_bwd_join(const em_sum a, int wide, T* __restrict__ dtable) {
+    __shared__ float lds[64][17];
+    const int tid = threadIdx.x, lane = tid & 63, C = a.C;
+    if ((int)blockIdx.x < a.tiles * wide) {
+        const int t = blockIdx.x / wide, c = (blockIdx.x % wide) * 1024 + tid;
+        if (t + 1 >= a.tiles) return;
+        const uint32_t key = a.key[(long long)(t + 1) * a.tile];
+        if (key >= a.vocab || !em_goes_on(a, t + 1, key) || (a.key[(long long)t * a.tile] == key && em_goes_on(a, t, key))) return;
+        const unsigned long long on = __ballot(em_goes_on(a, (long long)t + 1 + lane, key));
+        if (~on == 0) return;
+        const int more = __builtin_ctzll(~on);
+        if (c >= C) return;
+        float s = a.tail[(long long)t * C + c];
+#pragma unroll 8
+        for (int u = 1; u <= more; ++u) s += a.head[(long long)(t + u) * C + c];
+        dtable[(long long)key * C + c] = to_storage<T>(s * a.scale);
+        return;
+    }
+    const int groups = (C + 15) / 16, b = blockIdx.x - a.tiles * wide;
+    const long long q = (long long)(b / groups + 1) * EM_LONG;
+    if (q >= a.tiles) return;
+    const uint32_t key = a.key[q * a.tile];
+    if (key >= a.vocab) return;
+    const unsigned long long back = __ballot(em_goes_on(a, q - lane, key));      // every wave of the workgroup finds the same
+    if (!(back & 1)) return;
+    const int c0 = ~back ? __builtin_ctzll(~back) : EM_LONG;
+    if (c0 == EM_LONG && em_goes_on(a, q - EM_LONG, key)) return;               // an earlier multiple of EM_LONG has it
+    const long long t = q - c0;
+    long long more = 0;
+    for (long long u = t + 1;; u += 1024) {
+        const int n = __syncthreads_count(em_goes_on(a, u + tid, key));
+        more += n;
+        if (n < 1024) break;
+    }
+    if (more < EM_LONG) return;
+    const int part = tid >> 4, c = (b % groups) * 16 + (tid & 15);
+    float s = 0.f;
+    if (c < C) {
+#pragma unroll 8
+        for (long long u = part; u < more; u += 64) s += a.head[(t + 1 + u) * C + c];
+    }
+    lds[part][tid & 15] = s;
+    __syncthreads();
+    if (part == 0 && c < C) {
+        s = a.tail[t * C + c];
+#pragma unroll 8
+        for (int w = 0; w < 64; ++w) s += lds[w][tid];
+        dtable[(long long)key * C + c] = to_storage<T>(s * a.scale);
+    }
+}
+
+// dP: one workgroup a (position row, slice); the four waves share the sequences
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256) k_embed_pos_bwd(const T* __restrict__ dy, long long B, int L, int C, T* __restrict__ dpos) {
+    using COLS = em_cols<T, VEC>;
+    constexpr int N = COLS::N;
+    __shared__ float lds[4][64 * N];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = blockIdx.x, sl = blockIdx.y;
+    float acc[N] = {};
+    if (l < L) {
+#pragma unroll 4
+        for (long long b = wave; b < B; b += 4) {
+            float v[N];
+            COLS::load(dy + (b * L + l) * C, sl, lane, C, v);
+#pragma unroll
+            for (int i = 0; i < N; ++i) acc[i] += v[i];
+        }
+    }
+    em_fold<N>(acc, lds, wave, lane);
+    if (wave == 0) COLS::store(dpos + (long long)l * C, sl, lane, C, acc);
+}
+
+static bool em_vec(int C, int elem, const void* a, const void* b, const void* c = nullptr) {
+    return C * elem % 16 == 0 && (((uintptr_t)a | (uintptr_t)b | (uintptr_t)c) & 15) == 0;
+}
+
+// picks T and VEC for a launch expression
+#define EM_LAUNCH(dtype, vec, CALL)                                                                           \
+    do {                                                                                                      \
+        if ((dtype) == GD_F32) { using T = float; if (vec) { constexpr bool VEC = true; CALL; } else { constexpr bool VEC = false; CALL; } }   \
+        else if ((dtype) == GD_F16) { using T = f16_t; if (vec) { constexpr bool VEC = true; CALL; } else { constexpr bool VEC = false; CALL; } } \
+        else { using T = bf16_t; if (vec) { constexpr bool VEC = true; CALL; } else { constexpr bool VEC = false; CALL; } }                     \
+    } while (0)
+
+#define EM_ELEM(dtype) ((dtype) == GD_F32 ? 4 : 2)
+
+static int em_check(int64_t n, int64_t vocab, int C, int dtype, const char* who) {
+    GD_REQUIRE(n >= 0 && n < (1ll << 30), GD_EUNSUPPORTED, "%s: %lld positions (at most 2^30)", who, (long long)n);
+    GD_REQUIRE(vocab > 0 && vocab < (1ll << 31) - 1, GD_EUNSUPPORTED, "%s: a table of %lld rows", who, (long long)vocab);
+    GD_REQUIRE(C > 0 && C <= (1 << 20), GD_EUNSUPPORTED, "%s: C=%d", who, C);
+    GD_REQUIRE(dtype == GD_F16 || dtype == GD_BF16 || dtype == GD_F32, GD_EINVAL, "%s: dtype must be f16/bf16/f32", who);
+    return GD_OK;
+}
+
+extern "C" int gd_embed(const void* ids, int ids64, int64_t n, const void* table, int64_t vocab, const void* pos, int L, int C, float scale, void* y, int dtype,
+                        void* stream) {
+    const int rc = em_check(n, vocab, C, dtype, "gd_embed");
+    if (rc != GD_OK) return rc;
+    GD_REQUIRE(n > 0 && ids && table && y, GD_EINVAL, "gd_embed: null pointer or no positions");
+    GD_REQUIRE(!pos || L > 0, GD_EINVAL, "gd_embed: position rows need the sequence length");
+    const bool vec = em_vec(C, EM_ELEM(dtype), table, y, pos);
+    hipStream_t st = as_stream(stream);
+    EM_LAUNCH(dtype, vec, (k_embed<T, VEC><<<(unsigned)((n + 3) / 4), 256, 0, st>>>(em_ids{ids, ids64}, n, (const T*)table, (const T*)pos, L, (int)vocab, C, scale, (T*)y)));
+    GD_CHECK_LAUNCH("gd_embed");
+    return GD_OK;
+}
+
+// Up to here every workgroup may look through all ids by itself (one launch); above, they are sorted first.
+#define EM_SCAN_MAX 1024
+
+struct em_plan {
+    em_sort sort;
+    int passes, tile, tiles;
+    size_t key[2], pos[2], table, there, head, tail, bytes;
+};
+
+static em_plan em_plan_of(long long n, long long vocab, int C) {
+    em_plan p = {};
+    if (n <= EM_SCAN_MAX) return p;
+    p.sort = em_sort_of(n);
+    p.passes = 1;
+    while (p.passes < 4 && ((unsigned long long)vocab >> (8 * p.passes))) ++p.passes;
+    // 64 entries a tile; fewer where the tiles would not fill the chip's waves
+    p.tile = 64;
+    while (p.tile > 8 && n / p.tile < 4096) p.tile /= 2;
+    p.tiles = (int)((n + p.tile - 1) / p.tile);
+    size_t at = 0;
+    const auto take = [&](size_t bytes) { const size_t here = at; at += (bytes + 255) / 256 * 256; return here; };
+    for (int k = 0; k < 2; ++k) { p.key[k] = take(4 * (size_t)n); p.pos[k] = take(4 * (size_t)n); }
+    p.table = take(4 * 256 * (size_t)p.sort.blocks);
+    p.there = take((size_t)vocab);
+    p.head = take(4 * (size_t)p.tiles * C);
+    p.tail = take(4 * (size_t)p.tiles * C);
+    p.bytes = at;
+    return p;
+}
+
+extern "C" size_t gd_embed_bwd_workspace_bytes(int64_t n, int64_t vocab, int C) {
+    return n < 0 || vocab <= 0 || C <= 0 ? 0 : em_plan_of(n, vocab, C).bytes;
+}
+
+extern "C" int gd_embed_bwd(const void* ids, int ids64, int64_t n, const void* dy, int64_t vocab, int C, int64_t padding, float scale, void* dtable,
+                            void* workspace, size_t workspace_bytes, int dtype, void* stream) {
+    const int rc = em_check(n, vocab, C, dtype, "gd_embed_bwd");
+    if (rc != GD_OK) return rc;
+    GD_REQUIRE(dtable && (n == 0 || (ids && dy)), GD_EINVAL, "gd_embed_bwd: null pointer");
+    const bool vec = em_vec(C, EM_ELEM(dtype), dy, dtable);
+    const int slice = vec ? 64 * (16 / EM_ELEM(dtype)) : 512, slices = (C + slice - 1) / slice;
+    const long long zeros = (vocab + EM_ZERO_ROWS - 1) / EM_ZERO_ROWS;
+    const em_plan p = em_plan_of(n, vocab, C);
+    GD_REQUIRE(!p.bytes || (workspace && workspace_bytes >= p.bytes && ((uintptr_t)workspace & 15) == 0), GD_EWORKSPACE, "gd_embed_bwd: workspace of %zu bytes needed", p.bytes);
+    hipStream_t st = as_stream(stream);
+    const em_ids in = {ids, ids64};
+    if (!p.bytes) {
+        const long long grid = n * slices + zeros;
+        GD_REQUIRE(grid < (1ll << 31), GD_EUNSUPPORTED, "gd_embed_bwd: table too large");
+        EM_LAUNCH(dtype, vec, (k_embed_bwd_scan<T, VEC><<<(unsigned)grid, 256, 0, st>>>(in, (int)n, (const T*)dy, (int)vocab, C, padding, scale, (T*)dtable)));
+    } else {
+        const long long grid = ((long long)p.tiles * slices + 3) / 4 + zeros;
+        GD_REQUIRE(grid < (1ll << 31) && (long long)p.tiles * ((C + 1023) / 1024 + 1) + (long long)(p.tiles / EM_LONG) * ((C + 15) / 16) < (1ll << 31), GD_EUNSUPPORTED,
+                   "gd_embed_bwd: too many positions for this width");
+        char* const ws = (char*)workspace;
+        em_keys k = {in, nullptr, nullptr, (unsigned)vocab, padding};
+        for (int i = 0; i < p.passes; ++i) {
+            const bool last = i + 1 == p.passes;
+            uint32_t *const key = (uint32_t*)(ws + p.key[i & 1]), *const pos = (uint32_t*)(ws + p.pos[i & 1]);
+            k_embed_sort_count<<<p.sort.blocks, 256, 0, st>>>(k, p.sort, 8 * i, (int*)(ws + p.table), (uint32_t*)(ws + p.there), i == 0 ? (int)((vocab + 3) / 4) : 0);
+            k_embed_sort_move<<<p.sort.blocks, 256, 0, st>>>(k, p.sort, 8 * i, (const int*)(ws + p.table), key, pos, last ? (unsigned char*)(ws + p.there) : nullptr);
+            k.key = key;
+            k.pos = pos;
+        }
+        const em_sum a = {k.key, k.pos, (const unsigned char*)(ws + p.there), (float*)(ws + p.head), (float*)(ws + p.tail), n, p.tile, p.tiles, slices, C, (unsigned)vocab, scale};
+        EM_LAUNCH(dtype, vec, (k_embed_bwd_sum<T, VEC><<<(unsigned)grid, 256, 0, st>>>(a, (const T*)dy, (T*)dtable)));
+        const int wide = (C + 1023) / 1024;
+        const unsigned joins = (unsigned)((long long)p.tiles * wide + (long long)((p.tiles - 1) / EM_LONG) * ((C + 15) / 16));
+        if (p.tiles > 1) {
+            if (dtype == GD_F32) k_embed_bwd_join<float><<<joins, 1024, 0, st>>>(a, wide, (float*)dtable);
+            else if (dtype == GD_F16) k_embed_bwd_join<f16_t><<<joins, 1024, 0, st>>>(a, wide, (f16_t*)dtable);
+            else k_embed_bwd_join<bf16_t><<<joins, 1024, 0, st>>>(a, wide, (bf16_t*)dtable);
+        }
+    }
+    GD_CHECK_LAUNCH("gd_embed_bwd");
+    return GD_OK;
+}
+
+extern "C" int gd_embed_pos_bwd(const void* dy, int64_t B, int L, int C, int pos_rows, void* dpos, int dtype, void* stream) {
+    const int rc = em_check(B * (L > 0 ? L : 0), 1, C, dtype, "gd_embed_pos_bwd");
+    if (rc != GD_OK) return rc;
+    GD_REQUIRE(dpos && B >= 0 && L >= 0 && pos_rows >= L && pos_rows > 0 && (B * L == 0 || dy), GD_EINVAL, "gd_embed_pos_bwd: bad argument");
+    const bool vec = em_vec(C, EM_ELEM(dtype), dy, dpos);
+    const int slice = vec ? 64 * (16 / EM_ELEM(dtype)) : 512;
+    hipStream_t st = as_stream(stream);
+    EM_LAUNCH(dtype, vec, (k_embed_pos_bwd<T, VEC><<<dim3((unsigned)pos_rows, (C + slice - 1) / slice), 256, 0, st>>>((const T*)dy, B, L, C, (T*)dpos)));
+    GD_CHECK_LAUNCH("gd_embed_pos_bwd");
+    return GD_OK;
+}

@@ -6,7 +6,7 @@ from __future__ import annotations
 import numpy as np
 import torch
 
-from . import diffusion, graphs
+from . import diffusion, graphs, training
 from .attention_processors import VanillaAttentionProcessor
 from .scheduler import DDIMInverseScheduler, DDIMScheduler
 
@@ -182,6 +182,8 @@ class NullInversion:
                     loss = torch.nn.functional.mse_loss(latents_prev_rec, latent_prev)
                     optimizer.zero_grad()
                     loss.backward()
+                    if self.max_grad_norm is not None:
+                        training.clip_grad_norm_(uncond_embeddings, self.max_grad_norm)
                     optimizer.step()
                     if loss.item() < epsilon + i * 2e-5:
                         break
@@ -202,8 +204,11 @@ class NullInversion:
             uncond_embeddings = None
         return (image_gt, image_rec), ddim_latents[-1], uncond_embeddings, ddim_latents, ddim_noise
 
-    def __init__(self, model, num_ddim_steps=50, uncond_text="", device="cuda:0", progress_bar=None, guidance_scale=3.0):
+    def __init__(self, model, num_ddim_steps=50, uncond_text="", device="cuda:0", progress_bar=None, guidance_scale=3.0, max_grad_norm=None):
+        """``max_grad_norm``: null-text optimisation clips its embedding's gradient to this norm before each Adam step (None, as the
+        reference: no clipping)."""
         self.guidance_scale = guidance_scale
+        self.max_grad_norm = max_grad_norm
         self.progress_bar = progress_bar
         self.device = device
         self.num_ddim_steps = num_ddim_steps

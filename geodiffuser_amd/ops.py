@@ -7,7 +7,7 @@ from __future__ import annotations
 import ctypes
 import threading
 import os
-from typing import List, Optional, Sequence, Tuple
+from typing import List, NamedTuple, Optional, Sequence, Tuple
 
 import torch
 
@@ -1085,3 +1085,276 @@ def conv3x3(x, w, bias=None, stride: int = 1, upsample: bool = False, res=None):
     check(lib.gd_conv3x3(x.data_ptr(), w.data_ptr(), _p(bias), _p(res), out.data_ptr(), n, H, W, C, K, stride, int(bool(upsample)),
                          ctypes.byref(cfg), _p(ws), nb, _DT[x.dtype], _stream()), "gd_conv3x3")
     return out
+
+
+# ---------------------------------------------------------------------------------------------------
+# Training side: token embedding, block norms, gradient clipping (embed.hip, block_norm.hip, grad_clip.hip).  f16 / bf16 / f32.  The
+# autograd forms are in training.py.  A call runs on its tensors' device (whichever device is current) and that device's current stream.
+# At a prompt's sizes a call is bound by this file, not by its kernel: hence plain integers for pointers, the raw stream handle, and one
+# buffer behind several small outputs.
+# ---------------------------------------------------------------------------------------------------
+def _launch(fn, what: str, dev: int, *args) -> None:
+    """fn(*args, current stream of GPU ``dev``), with that GPU current."""
+    if torch._C._cuda_getDevice() == dev:
+        code = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    else:
+        with torch.cuda.device(dev):
+            code = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    if code:
+        check(code, what)
+
+
+def _dt(t: torch.Tensor, name: str) -> int:
+    dt = _DT.get(t.dtype)
+    if dt is None:
+        raise _lib.GeodiffError(f"{name}: expected float16/bfloat16/float32, got {t.dtype}")
+    return dt
+
+
+def _like(t: Optional[torch.Tensor], name: str, ref: torch.Tensor, shape) -> int:
+    """Address of t (0: None), which has to be contiguous, on ref's device, of its dtype and of ``shape``."""
+    if t is None:
+        return 0
+    _need(t, name, ref.dtype)
+    if t.shape != shape or t.device != ref.device:
+        raise _lib.GeodiffError(f"{name}: expected shape {tuple(shape)} on {ref.device}, got {tuple(t.shape)} on {t.device}")
+    return t.data_ptr()
+
+
+def _token_ids(ids: torch.Tensor, ref: torch.Tensor) -> int:
+    _need(ids, "ids")
+    if ids.dtype not in (torch.int64, torch.int32) or ids.device != ref.device or ids.dim() < 1:
+        raise _lib.GeodiffError(f"ids: expected an int64 / int32 tensor on {ref.device}, got {ids.dtype} on {ids.device}")
+    return int(ids.dtype == torch.int64)
+
+
+def embed_tokens(ids, table, pos=None, scale: float = 1.0):
+    """y = scale * table[ids] + pos[:L]: ids int64 / int32 [..., L], table [V, C], pos [>= L, C] or None -> [..., L, C].  One rounding.  An id
+    outside the table gives a row of NaN (nothing is read there, and the device is not synchronised to raise)."""
+    lib = _lib.load()
+    _need(table, "table")
+    dt = _dt(table, "table")
+    wide = _token_ids(ids, table)
+    shape = ids.shape
+    L = shape[-1]
+    if table.dim() != 2 or (pos is not None and (pos.dim() != 2 or pos.shape[0] < L)):
+        raise _lib.GeodiffError("embed_tokens: table is [V, C], pos is [>= L, C]")
+    V, C = table.shape
+    pp = 0 if pos is None else _like(pos, "pos", table, (pos.shape[0], C))
+    y = torch.empty(*shape, C, dtype=table.dtype, device=table.device)
+    n = ids.numel()
+    if n and C:
+        _launch(lib.gd_embed, "gd_embed", table.get_device(), ids.data_ptr(), wide, n, table.data_ptr(), V, pp, L, C, scale, y.data_ptr(), dt)
+    return y
+
+
+def embed_tokens_bwd(ids, dy, vocab: int, scale: float = 1.0, padding_idx: Optional[int] = None):
+    """Gradient of ``embed_tokens`` w.r.t. its table for dy [..., L, C] -> [vocab, C], every row written: scale * the sum of dy over the
+    positions of each token, zeros where there are none and in row ``padding_idx``.  Ids outside the table add nothing.  The order of a
+    row's sum is fixed by the positions: the same inputs give the same bits."""
+    lib = _lib.load()
+    _need(dy, "dy")
+    dt = _dt(dy, "dy")
+    wide = _token_ids(ids, dy)
+    if dy.shape[:-1] != ids.shape:
+        raise _lib.GeodiffError("embed_tokens_bwd: dy is [*ids.shape, C]")
+    if padding_idx is not None and not 0 <= padding_idx < vocab:
+        raise _lib.GeodiffError("embed_tokens_bwd: padding_idx must be a row of the table")
+    C, n = dy.shape[-1], ids.numel()
+    d = torch.empty(vocab, C, dtype=dy.dtype, device=dy.device)
+    if vocab and C:
+        nbytes = lib.gd_embed_bwd_workspace_bytes(n, vocab, C)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dy.device) if nbytes else None
+        _launch(lib.gd_embed_bwd, "gd_embed_bwd", dy.get_device(), ids.data_ptr(), wide, n, dy.data_ptr(), vocab, C, -1 if padding_idx is None else padding_idx,
+                scale, d.data_ptr(), _ip(ws), nbytes, dt)
+    return d
+
+
+def embed_positions_bwd(dy, pos_rows: int):
+    """Gradient of ``embed_tokens`` w.r.t. its position rows: dy [..., L, C] -> [pos_rows, C], the sum over the leading axes; rows L and up
+    are zeros."""
+    lib = _lib.load()
+    _need(dy, "dy")
+    dt = _dt(dy, "dy")
+    if dy.dim() < 2 or pos_rows < dy.shape[-2]:
+        raise _lib.GeodiffError("embed_positions_bwd: dy is [..., L, C] with L <= pos_rows")
+    L, C = dy.shape[-2:]
+    d = torch.empty(pos_rows, C, dtype=dy.dtype, device=dy.device)
+    if pos_rows and C:
+        _launch(lib.gd_embed_pos_bwd, "gd_embed_pos_bwd", dy.get_device(), dy.data_ptr(), dy.numel() // (L * C) if L else 0, L, C, pos_rows, d.data_ptr(), dt)
+    return d
+
+
+class Norm(NamedTuple):
+    """One norm of ``block_norm``: kind "layer" or "rms", gamma / beta [C] of the activations' dtype (None: 1 / 0), eps."""
+    kind: str
+    gamma: Optional[torch.Tensor] = None
+    beta: Optional[torch.Tensor] = None
+    eps: float = 1e-5
+
+
+_NORM_KINDS = {"layer": _lib.GD_NORM_LAYER, "rms": _lib.GD_NORM_RMS}
+
+
+def _norm_args(norm: Optional[Norm], name: str, x: torch.Tensor, C: int):
+    """-> kind, address of gamma, address of beta, eps"""
+    if norm is None:
+        return 0, 0, 0, 0.0
+    kind = _NORM_KINDS.get(norm.kind)
+    if kind is None:
+        raise _lib.GeodiffError(f"block_norm: {name} norm must be 'layer' or 'rms', got {norm.kind!r}")
+    return kind, _like(norm.gamma, name + " gamma", x, (C,)), _like(norm.beta, name + " beta", x, (C,)), norm.eps
+
+
+def _block_norm_args(x, res, pre, post, gate, res_scale, s: int, y: int, stats: int):
+    """-> (gd_block_norm_t, rows, C, rows of the gate); s, y, stats: addresses."""
+    shape = x.shape
+    C = shape[-1]
+    rows = x.numel() // C
+    pre_kind, pre_g, pre_b, pre_eps = _norm_args(pre, "pre", x, C)
+    post_kind, post_g, post_b, post_eps = _norm_args(post, "post", x, C)
+    gp, per, ld, gate_rows = 0, rows, C, 1
+    if gate is not None:
+        per_sample = gate.dim() == 2 and x.dim() >= 2
+        if (gate.device != x.device or gate.dtype != x.dtype or gate.shape != ((shape[0], C) if per_sample else (C,)) or gate.stride(-1) != 1
+                or (per_sample and gate.shape[0] > 1 and gate.stride(0) < C)):
+            raise _lib.GeodiffError("block_norm: gate is [C] or [x.shape[0], C] of x's dtype and device, its rows contiguous")
+        gp = gate.data_ptr()
+        if per_sample and shape[0]:
+            gate_rows, per = shape[0], rows // shape[0]
+            ld = gate.stride(0) if gate_rows > 1 else C
+    return _lib.GdBlockNorm(x.data_ptr(), _like(res, "res", x, shape), gp, post_g, post_b, pre_g, pre_b, s, y, stats, rows, per, ld, C, post_kind, pre_kind, post_eps, pre_eps,
+                            res_scale), gate_rows
+
+
+def _block_norm_x(x):
+    _need(x, "x")
+    if x.dim() < 1 or x.shape[-1] == 0:
+        raise _lib.GeodiffError("block_norm: x is [..., C]")
+    return _dt(x, "x")
+
+
+def block_norm(x, res, pre: Optional[Norm], post: Optional[Norm] = None, gate=None, res_scale: float = 1.0):
+    """The residual stream behind a transformer block and the norm in front of the next one, in one launch:
+
+        s = res_scale * res + gate * post(x),   y = pre(s)            -> (s, y, stats)
+
+    x, res [..., C] (res None: nothing is added; with neither gate nor post, s is then x itself), C <= 16384; gate [C], or [x.shape[0], C]
+    with a row for each sample (its rows may be strided); pre / post: ``Norm`` or None (pre None: y is None).  y is computed from the
+    unrounded sum; stats [rows, 4] f32 is what ``block_norm_bwd`` needs."""
+    lib = _lib.load()
+    dt = _block_norm_x(x)
+    plain = res is None and gate is None and post is None
+    if plain and pre is None:
+        raise _lib.GeodiffError("block_norm: nothing to compute")
+    s = x if plain else torch.empty_like(x)
+    y = torch.empty_like(x) if pre is not None else None
+    stats = torch.empty(x.numel() // x.shape[-1], 4, dtype=torch.float32, device=x.device)
+    a, _ = _block_norm_args(x, res, pre, post, gate, res_scale, 0 if plain else s.data_ptr(), _ip(y), stats.data_ptr())
+    if a.rows:
+        _launch(lib.gd_block_norm, "gd_block_norm", x.get_device(), ctypes.byref(a), dt)
+    return s, y, stats
+
+
+_BLOCK_NORM_GRADS = ("dx", "dres", "dgate", "dpost_gamma", "dpost_beta", "dpre_gamma", "dpre_beta")
+
+
+def block_norm_bwd(x, res, gy, gs, stats, pre: Optional[Norm], post: Optional[Norm] = None, gate=None, res_scale: float = 1.0,
+                   need: Optional[Sequence[str]] = None):
+    """Gradients of ``block_norm``: gy = dL/dy, gs = dL/ds (one of them may be None), stats from the forward call, the other arguments as
+    there.  -> {"dx", "dres", "dgate", "dpost_gamma", "dpost_beta", "dpre_gamma", "dpre_beta"}: None where the call has no such input,
+    or where ``need`` (names of the ones that are wanted; default: all) leaves it out."""
+    lib = _lib.load()
+    dt = _block_norm_x(x)
+    if gy is None and gs is None:
+        raise _lib.GeodiffError("block_norm_bwd: gy or gs is needed")
+    if gy is not None and pre is None:
+        raise _lib.GeodiffError("block_norm_bwd: gy without the norm that made y")
+    if need is not None and not set(need) <= set(_BLOCK_NORM_GRADS):
+        raise _lib.GeodiffError(f"block_norm_bwd: need names {_BLOCK_NORM_GRADS}")
+    _need(stats, "stats", torch.float32)
+    shape = x.shape
+    C = shape[-1]
+    rows = x.numel() // C
+    if stats.shape != (rows, 4) or stats.device != x.device:
+        raise _lib.GeodiffError("block_norm_bwd: stats are not those of this call's forward")
+    f, gate_rows = _block_norm_args(x, res, pre, post, gate, res_scale, 0, 0, stats.data_ptr())
+    pgy, pgs = _like(gy, "gy", x, shape), _like(gs, "gs", x, shape)
+    out = dict.fromkeys(_BLOCK_NORM_GRADS)
+    want = [k for k, t in zip(_BLOCK_NORM_GRADS, (x, res, gate, post and post.gamma, post and post.beta, pre and pre.gamma, pre and pre.beta))
+            if t is not None and (need is None or k in need)]
+    rows_of = [gate_rows if k == "dgate" else 1 for k in want if k not in ("dx", "dres")]
+    for k in want[:2]:
+        if k in ("dx", "dres"):
+            out[k] = torch.empty_like(x)
+    if rows_of:
+        # the sums over rows: rows of one buffer
+        small = iter((torch.zeros if rows == 0 else torch.empty)(sum(rows_of), C, dtype=x.dtype, device=x.device).split(rows_of))
+        for k in want:
+            if k == "dgate":
+                out[k] = next(small).view(gate.shape)
+            elif k not in ("dx", "dres"):
+                out[k] = next(small)[0]
+    if rows == 0 or not want:
+        return out
+    if gy is None:
+        # nothing reaches y's norm: its parameters' gradients are zeros, and the kernel is not asked for them
+        for k in ("dpre_gamma", "dpre_beta"):
+            if out[k] is not None:
+                out[k].zero_()
+    ptr = [_ip(out[k]) if gy is not None or not k.startswith("dpre") else 0 for k in _BLOCK_NORM_GRADS]
+    nbytes = lib.gd_block_norm_bwd_workspace_bytes(rows, C, gate_rows if ptr[2] else 0) if any(ptr[2:]) else 0
+    if not any(ptr):
+        return out
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
+    _launch(lib.gd_block_norm_bwd, "gd_block_norm_bwd", x.get_device(), ctypes.byref(_lib.GdBlockNormBwd(f, pgy, pgs, *ptr)), _ip(ws), nbytes, dt)
+    return out
+
+
+def _grad_norm(grads, norm_type, max_norm, out):
+    lib = _lib.load()
+    grads = list(grads)
+    norm_type = float(norm_type)
+    if norm_type not in (2.0, float("inf")):
+        raise _lib.GeodiffError(f"grad_norm: norm_type must be 2 or inf, got {norm_type}")
+    if not grads:
+        raise _lib.GeodiffError("grad_norm: no tensors")
+    dev = grads[0].get_device()
+    for t in grads:
+        if not t.is_cuda or t.get_device() != dev:
+            raise _lib.GeodiffError(f"grad_norm: expected GPU tensors of one device (the HIP path has no CPU fallback), got {t.device}")
+        if not t.is_contiguous() and not (t.dim() == 4 and t.is_contiguous(memory_format=torch.channels_last)):
+            raise _lib.GeodiffError("grad_norm: tensors must be contiguous (or channels_last)")
+    n = len(grads)
+    src = (ctypes.c_void_p * n)(*[t.data_ptr() for t in grads])
+    numel = (ctypes.c_int64 * n)(*[t.numel() for t in grads])
+    dts = (ctypes.c_int32 * n)(*[_DT.get(t.dtype, -1) for t in grads])
+    dst = None
+    if max_norm is not None:
+        max_norm = float(max_norm)
+        if not max_norm >= 0:
+            raise _lib.GeodiffError(f"clip_grad_norm: max_norm must not be negative or NaN, got {max_norm}")
+        dst = src
+        if out is not None:
+            out = list(out)
+            if len(out) != n or any(o.shape != t.shape or o.dtype != t.dtype or o.get_device() != dev or o.stride() != t.stride() for o, t in zip(out, grads)):
+                raise _lib.GeodiffError("clip_grad_norm: out needs a tensor of the same shape, strides, dtype and device for each gradient")
+            dst = (ctypes.c_void_p * n)(*[t.data_ptr() for t in out])
+    nbytes = lib.gd_grad_norm_workspace_bytes()
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=grads[0].device)
+    norm = torch.empty((), dtype=torch.float32, device=grads[0].device)
+    _launch(lib.gd_grad_norm, "gd_grad_norm", dev, src, dst, numel, dts, n, int(norm_type != 2.0), max_norm or 0.0, ws.data_ptr(), nbytes, norm.data_ptr())
+    return norm
+
+
+def grad_norm(grads, norm_type: float = 2.0):
+    """Norm over all elements of a list of f16 / bf16 / f32 tensors (mixed types are fine): sqrt(sum g^2), or max |g| for norm_type inf.
+    -> 0-d f32 tensor on their device (no synchronisation); NaN if an element is."""
+    return _grad_norm(grads, norm_type, None, None)
+
+
+def clip_grad_norm(grads, max_norm: float, norm_type: float = 2.0, out=None):
+    """Scales the tensors by min(1, max_norm / (norm + 1e-6)), norm as ``grad_norm`` -> norm (before clipping).  In place, or into the tensors
+    ``out`` (one for each, same shape and strides).  The tensors must not overlap.  An infinite or NaN norm scales like any other number:
+    by 0 or NaN."""
+    return _grad_norm(grads, norm_type, max_norm, out)

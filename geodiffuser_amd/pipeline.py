@@ -17,6 +17,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from . import training
 from .scheduler import DDIMScheduler
 from .unet_sd21 import GroupNormAct, UNet2DConditionModel, sd14_unet, sdxl_unet, tiny_unet
 
@@ -63,8 +64,17 @@ class TextEncoder(nn.Module):
         self.layers = nn.ModuleList([_TextLayer(width, heads) for _ in range(layers)])
         self.ln_f = nn.LayerNorm(width)
 
+    def _embed(self, input_ids):
+        """Token + position embedding: one launch on the GPU (gd_embed, the same rounding), with its gradient where table or positions learn."""
+        w, pos = self.tok.weight, self.pos.to(self.tok.weight.dtype)
+        stock = type(self.tok) is nn.Embedding and self.tok.padding_idx is None and self.tok.max_norm is None and not (
+            self.tok._forward_hooks or self.tok._forward_pre_hooks or self.tok._backward_hooks)
+        if stock and w.is_cuda and input_ids.device == pos.device == w.device and w.dtype in (torch.float16, torch.bfloat16, torch.float32) and w.is_contiguous():
+            return training.embed_tokens(input_ids.contiguous(), w, pos.contiguous())
+        return self.tok(input_ids) + pos[: input_ids.shape[1]]
+
     def forward(self, input_ids):
-        x = self.tok(input_ids) + self.pos[: input_ids.shape[1]].to(self.tok.weight.dtype)
+        x = self._embed(input_ids)
         L = x.shape[1]
         mask = torch.full((L, L), float("-inf"), device=x.device, dtype=x.dtype).triu(1)
         for l in self.layers:

@@ -535,6 +535,58 @@ int gd_softsplat_bwd(const float* in, const float* flow, const float* outgrad, i
 typedef struct gd_copy_rows { const void* src; void* dst; int64_t bytes; } gd_copy_rows_t;
 int gd_copy_rows(const gd_copy_rows_t* entries, int n, int row, int64_t max_bytes, void* stream);
 
+/* ------------------------------------------------------------------------------------------------
+ * Training side of the text tower and of the transformer blocks (what the reference leaves to torch's autograd: it learns text
+ * embeddings only, U/inversion.py:213-259, U/optimization.py:165-253).  f16 / bf16 / f32 storage, binary32 arithmetic (binary64
+ * for the gradient norm), one rounding of each result, fixed summation orders (no float atomics).
+ * ---------------------------------------------------------------------------------------------- */
+
+/* y[i] = scale * table[ids[i]] + pos[i mod L] for n positions: table [vocab, C], pos [>= L, C] or NULL, y [n, C], ids int64 (ids64 = 1) or
+ * int32.  An id outside [0, vocab) gives a row of NaN. */
+int gd_embed(const void* ids, int ids64, int64_t n, const void* table, int64_t vocab, const void* pos, int L, int C, float scale, void* y, int dtype,
+             void* stream);
+/* dtable[v] = scale * sum of dy[i] over the positions with ids[i] = v, for EVERY row v of the table (zeros where there is none, and in
+ * row `padding`; -1: no such row); ids outside the table add nothing. */
+size_t gd_embed_bwd_workspace_bytes(int64_t n, int64_t vocab, int C);
+int gd_embed_bwd(const void* ids, int ids64, int64_t n, const void* dy, int64_t vocab, int C, int64_t padding, float scale, void* dtable,
+                 void* workspace, size_t workspace_bytes, int dtype, void* stream);
+/* dpos[l] = sum over b of dy[b, l], dy [B, L, C]; rows L .. pos_rows - 1 become zeros. */
+int gd_embed_pos_bwd(const void* dy, int64_t B, int L, int C, int pos_rows, void* dpos, int dtype, void* stream);
+
+/* h = post(x);  s = res_scale * res + gate * h;  y = pre(s) for rows of C <= 16384 channels.
+ *   kinds: GD_NORM_NONE, GD_NORM_LAYER (xh = (v - mean) / sqrt(var + eps)), GD_NORM_RMS (xh = v / sqrt(mean v^2 + eps)), then
+ *   xh * gamma + beta; gamma, beta [C] or NULL (1, 0).  gate: one row of C for every rows_per_gate rows, gate_ld elements apart, or
+ *   NULL (1).  res NULL: s = gate * h.  s may be NULL; y goes with pre_kind.  stats [rows, 4] f32 (mean, 1 / deviation of x, then of
+ *   s; NULL: not kept) is what the backward needs.  y is computed from the unrounded s. */
+enum { GD_NORM_NONE = 0, GD_NORM_LAYER = 1, GD_NORM_RMS = 2 };
+typedef struct gd_block_norm {
+    const void *x, *res, *gate, *post_gamma, *post_beta, *pre_gamma, *pre_beta;
+    void *s, *y;
+    float* stats;
+    int64_t rows, rows_per_gate, gate_ld;
+    int32_t C, post_kind, pre_kind;
+    float post_eps, pre_eps, res_scale;
+} gd_block_norm_t;
+int gd_block_norm(const gd_block_norm_t* f, int dtype, void* stream);
+/* Its gradients: f as in the forward call (s, y are not read), gy = dL/dy, gs = dL/ds (either may be NULL); dx, dres [rows, C], dgate [rows /
+ * rows_per_gate, C], the four parameter gradients [C]; each of them may be NULL. */
+typedef struct gd_block_norm_bwd {
+    gd_block_norm_t f;
+    const void *gy, *gs;
+    void *dx, *dres, *dgate, *dpost_gamma, *dpost_beta, *dpre_gamma, *dpre_beta;
+} gd_block_norm_bwd_t;
+/* gate_rows: rows of dgate, 0 without it */
+size_t gd_block_norm_bwd_workspace_bytes(int64_t rows, int C, int64_t gate_rows);
+int gd_block_norm_bwd(const gd_block_norm_bwd_t* a, void* workspace, size_t workspace_bytes, int dtype, void* stream);
+
+/* Norm over all elements of `count` tensors: norm[0] = sqrt(sum g^2) (inf_norm = 0) or max |g| (1), NaN if an element is.  dst not NULL:
+ * also dst[i] = src[i] * min(1, max_norm / (norm + 1e-6)), in place where dst[i] == src[i]; no destination may overlap another
+ * tensor of the call.  src, dst, n (elements; 0 is fine), dtype (GD_F16 / GD_BF16 / GD_F32) are HOST arrays, read before the call
+ * returns. */
+size_t gd_grad_norm_workspace_bytes(void);
+int gd_grad_norm(const void* const* src, void* const* dst, const int64_t* n, const int32_t* dtype, int count, int inf_norm, float max_norm,
+                 void* workspace, size_t workspace_bytes, float* norm, void* stream);
+
 /* Host helper: *id = 1 + the runtime's id of the capture sequence `stream` is recording, 0 when it is not capturing (callers that hand
  * out pre-zeroed scratch must not share a chunk between two hipGraph captures). */
 int gd_stream_capture_id(void* stream, unsigned long long* id);

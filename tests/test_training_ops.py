@@ -1,0 +1,853 @@
+"""The training-side operators (geodiffuser_amd.ops / .training: token embedding, block norms, gradient clipping) against plain
+implementations in 64 bits, at the sizes, layouts and values where they can go wrong, and their refusals.
+
+Tolerances, derived before any run.  Storage of type T rounds a result r by at most u |r| with u = finfo(T).eps / 2, or half its smallest
+subnormal (``_close``).  The arithmetic before that rounding is binary32 (2^-24 relative a step); a result that is a sum of terms t_i
+built by at most k roundings on any path is then off by at most k 2^-24 sum |t_i|.  Each check states its k and its sum of magnitudes."""
+import ctypes
+import math
+
+import pytest
+import torch
+
+from geodiffuser_amd import GeodiffError
+
+gpu = pytest.mark.gpu
+DEV = "cuda"
+DTYPES = [torch.float16, torch.bfloat16, torch.float32]
+U32 = 2.0 ** -24
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from geodiffuser_amd import _lib, ops as _ops
+    _lib.load()
+    return _ops
+
+
+def _gen(seed):
+    return torch.Generator(device="cpu").manual_seed(seed)
+
+
+def _randn(g, *shape, dtype=torch.float32, std=1.0, mean=0.0, dev=DEV):
+    return (torch.randn(*shape, generator=g) * std + mean).to(dev).to(dtype)
+
+
+def _close(got, ref, k, mag, what=""):
+    """|got - ref| <= u |ref| + half a subnormal + k 2^-24 mag, NaN and infinities where ref has them."""
+    fi = torch.finfo(got.dtype)
+    u = 0.0 if got.dtype == torch.float32 else fi.eps / 2
+    got, ref = got.double(), ref.double()
+    assert got.shape == ref.shape, (what, got.shape, ref.shape)
+    fine = ref.isfinite()
+    assert torch.equal(got.isnan(), ref.isnan()) and torch.equal(got[~fine & ~ref.isnan()], ref[~fine & ~ref.isnan()]), what
+    err = (got - ref).abs()
+    tol = (u * (1 + u) + U32) * ref.abs() + fi.smallest_normal * fi.eps / 2 + k * U32 * mag.double()
+    bad = (err > tol) & fine
+    if bool(bad.any()):
+        i = int((err - tol).masked_fill(~bad, -1).argmax())
+        raise AssertionError(f"{what}: {int(bad.sum())} of {bad.numel()} off, worst at {i}: {float(got.flatten()[i])} for {float(ref.flatten()[i])}, "
+                             f"tolerance {float(tol.expand_as(err).flatten()[i])}")
+
+
+def _misaligned(t):
+    """The same values at an address that is a multiple of the element only."""
+    return torch.cat([t.new_zeros(1), t.flatten()])[1:].view(t.shape)
+
+
+# ------------------------------------------------------------------------------------------------ token embedding
+def _embed_ref(ids, table, pos, scale):
+    V = table.shape[0]
+    ok = (ids >= 0) & (ids < V)
+    y = table.double()[ids.long().clamp(0, V - 1)] * scale
+    if pos is not None:
+        y = y + pos.double()[:ids.shape[-1]]
+    return torch.where(ok[..., None], y, torch.nan)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape,V,C,pos,scale", [
+    ((1, 1), 5, 8, True, 1.0), ((1,), 3, 1, False, 2.0), ((2, 77), 49408, 1024, True, 1.0), ((3, 5), 100, 333, True, 333 ** 0.5), ((2, 3, 7), 9, 1280, False, 0.5),
+    ((1, 77), 1000, 2056, True, 1.0), ((513, 9), 4000, 40, True, -3.0), ((4, 2), 1, 65, True, 1.0)])
+def test_embedding_lookup(ops, dtype, shape, V, C, pos, scale):
+    g = _gen(C)
+    ids = torch.randint(0, V, shape, generator=g)
+    ids.view(-1)[-1] = V - 1
+    table, P = _randn(g, V, C, dtype=dtype), _randn(g, shape[-1] + 2, C, dtype=dtype) if pos else None
+    ref = _embed_ref(ids.to(DEV), table, P, scale)
+    mag = (table.double()[ids.to(DEV)] * scale).abs() + (0 if P is None else P.double()[:shape[-1]].abs())
+    for idx in (ids.to(DEV), ids.to(DEV).int()):
+        # k = 2: scale itself to 32 bits, the fused multiply-add
+        _close(ops.embed_tokens(idx, table, P, scale=scale), ref, 2, mag)
+    _close(ops.embed_tokens(ids.to(DEV), _misaligned(table), P, scale=scale), ref, 2, mag)
+
+
+@gpu
+def test_embedding_lookup_outside_the_table_is_nan(ops):
+    table = torch.ones(4, 24, device=DEV)
+    ids = torch.tensor([[0, -1, 4, 3, -2 ** 40, 2 ** 40]], device=DEV)
+    y = ops.embed_tokens(ids, table, torch.ones(6, 24, device=DEV))
+    assert torch.equal(y.isnan().all(-1), torch.tensor([[False, True, True, False, True, True]], device=DEV)) and torch.equal(y[0, 0], torch.full((24,), 2.0, device=DEV))
+    assert ops.embed_tokens(ids[:, :0], table).shape == (1, 0, 24)
+
+
+def _check_embed_bwd(ops, ids, dy, V, scale=1.0, padding_idx=None):
+    d = ops.embed_tokens_bwd(ids, dy, V, scale=scale, padding_idx=padding_idx)
+    flat, rows = ids.reshape(-1).long(), dy.reshape(-1, dy.shape[-1]).double() * scale
+    ok = (flat >= 0) & (flat < V)
+    if padding_idx is not None:
+        ok &= flat != padding_idx
+    ref = torch.zeros(V, dy.shape[-1], dtype=torch.float64, device=DEV).index_add_(0, flat[ok], rows[ok])
+    mag = torch.zeros_like(ref).index_add_(0, flat[ok], rows[ok].abs())
+    # k: the additions of the longest row and the scaling
+    k = int(torch.bincount(flat[ok]).max()) + 2 if bool(ok.any()) else 0
+    _close(d, ref, k, mag, f"n={flat.numel()} V={V} C={dy.shape[-1]}")
+    assert not bool(d[torch.bincount(flat[ok], minlength=V) == 0].any())              # rows of no token: exact zeros
+    assert torch.equal(d, ops.embed_tokens_bwd(ids, dy, V, scale=scale, padding_idx=padding_idx))      # and the same bits again
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,V,C,kind", [
+    (0, 7, 16, "any"), (1, 1, 1, "any"), (1, 50, 9, "any"), (5, 33, 64, "same"), (77, 1000, 768, "prompt"), (255, 17, 24, "any"), (256, 300, 512, "any"),
+    (257, 300, 520, "distinct"), (308, 49408, 1024, "prompt"), (1000, 40, 333, "any"), (1500, 2000, 1280, "distinct"), (3000, 5, 128, "any"),
+    (4096, 100, 40, "same"), (4097, 49408, 96, "prompt"), (20011, 1003, 136, "prompt"), (20000, 3, 64, "any"), (9999, 70000, 72, "distinct"), (70001, 500, 33, "any")])
+def test_embedding_gradient(ops, dtype, n, V, C, kind):
+    g = _gen(n + C)
+    if kind == "same":
+        ids = torch.full((n,), V // 2)
+    elif kind == "distinct":
+        ids = torch.randperm(max(n, V), generator=g)[:n] % V
+    elif kind == "prompt":
+        ids = (V * torch.rand(n, generator=g) ** 5).long()
+        ids[torch.rand(n, generator=g) < 0.6] = 0
+    else:
+        ids = torch.randint(0, V, (n,), generator=g)
+    dy = _randn(g, n, C, dtype=dtype)
+    _check_embed_bwd(ops, ids.to(DEV), dy, V)
+    _check_embed_bwd(ops, ids.to(DEV).int(), _misaligned(dy) if n else dy, V, scale=0.125)
+
+
+@gpu
+@pytest.mark.parametrize("n", [6, 300, 9000])
+def test_embedding_gradient_skips_padding_and_foreign_ids(ops, n):
+    g = _gen(n)
+    ids = torch.randint(-2, 8, (3, n // 3), generator=g).to(DEV)                      # -2, -1, 6, 7 lie outside a table of 6 rows
+    dy = _randn(g, *ids.shape, 40)
+    for pad in (None, 0, 5):
+        _check_embed_bwd(ops, ids, dy, 6, padding_idx=pad)
+    ids[ids == 3] = 2 ** 40                                                            # beyond 32 bits
+    _check_embed_bwd(ops, ids, dy, 6)
+    _check_embed_bwd(ops, torch.full_like(ids, -1), dy, 6)                             # nothing inside: all zeros
+
+
+@gpu
+def test_embedding_gradient_keeps_nan_and_inf_in_their_rows(ops):
+    for n in (40, 8000):
+        ids = (torch.arange(n) % 8).to(DEV)
+        dy = torch.ones(n, 16, device=DEV)
+        dy[1, 2], dy[2, 3] = math.nan, math.inf
+        d = ops.embed_tokens_bwd(ids, dy, 9)
+        want = torch.full((9, 16), n / 8, device=DEV)
+        want[8] = 0
+        want[1, 2], want[2, 3] = math.nan, math.inf
+        assert torch.equal(d.nan_to_num(nan=-1, posinf=-2), want.nan_to_num(nan=-1, posinf=-2))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("lead,L,P,C", [((1,), 1, 1, 8), ((4,), 77, 77, 1024), ((2, 3), 5, 9, 33), ((0,), 3, 4, 16), ((1000,), 7, 77, 40), ((3001,), 2, 3, 520)])
+def test_position_gradient(ops, dtype, lead, L, P, C):
+    dy = _randn(_gen(L), *lead, L, C, dtype=dtype)
+    d = ops.embed_positions_bwd(dy, P)
+    rows = dy.double().reshape(-1, L, C)
+    pad = torch.zeros(P - L, C, dtype=torch.float64, device=DEV)
+    _close(d, torch.cat([rows.sum(0), pad]), rows.shape[0], torch.cat([rows.abs().sum(0), pad]))        # k: one addition a sequence
+    assert not bool(d[L:].any()) and torch.equal(d, ops.embed_positions_bwd(dy, P))
+    if dy.numel():
+        assert rel_same(ops.embed_positions_bwd(_misaligned(dy), P), d, rows.shape[0], rows.abs().sum(0).max())
+
+
+def rel_same(a, b, k, mag):
+    """Two results of the same sums in possibly different orders."""
+    u = 0.0 if a.dtype == torch.float32 else torch.finfo(a.dtype).eps
+    return bool(((a.double() - b.double()).abs() <= u * b.double().abs() + 2 * k * U32 * mag + torch.finfo(a.dtype).smallest_normal).all())
+
+
+@gpu
+def test_embedding_offsets_beyond_32_bits(ops):
+    """A table and a gradient of more than 2^31 elements: the rows behind that border are the ones asked for."""
+    V, C = (1 << 21) + 5, 1024
+    table = torch.zeros(V, C, dtype=torch.bfloat16, device=DEV)
+    table[-1], table[-3] = 3.0, 5.0
+    ids = torch.tensor([[V - 1, V - 3, 0]], device=DEV)
+    assert ops.embed_tokens(ids, table)[0, :, 7].tolist() == [3.0, 5.0, 0.0]
+    d = ops.embed_tokens_bwd(ids, torch.ones(1, 3, C, dtype=torch.bfloat16, device=DEV), V)
+    assert d[[V - 1, V - 3, 0, V - 2], C - 1].tolist() == [1.0, 1.0, 1.0, 0.0] and float(d.sum(dtype=torch.float32)) == 3.0 * C
+    del d
+    ids = torch.zeros(V, dtype=torch.int32, device=DEV)                               # the same buffer as the gradient of as many positions
+    ids[-1], ids[-3] = 2, 1
+    d = ops.embed_tokens_bwd(ids, table, 4)
+    assert d[:, 5].tolist() == [0.0, 5.0, 3.0, 0.0]
+    assert ops.embed_positions_bwd(table.view(1, V, C), V)[-1, 0].item() == 3.0
+
+
+def test_embedding_refusals():
+    from geodiffuser_amd import ops
+    t, ids = torch.zeros(4, 8), torch.zeros(2, 3, dtype=torch.long)
+    for call in (lambda: ops.embed_tokens(ids, t), lambda: ops.embed_tokens_bwd(ids, torch.zeros(2, 3, 8), 4), lambda: ops.embed_positions_bwd(torch.zeros(2, 3, 8), 3)):
+        with pytest.raises(GeodiffError, match="GPU tensor"):
+            call()
+
+
+@gpu
+def test_embedding_refusals_on_the_device(ops):
+    t, ids, dy = torch.zeros(4, 8, device=DEV), torch.zeros(2, 3, dtype=torch.long, device=DEV), torch.zeros(2, 3, 8, device=DEV)
+    bad = [lambda: ops.embed_tokens(ids.cpu(), t), lambda: ops.embed_tokens(ids.float(), t), lambda: ops.embed_tokens(ids.short(), t), lambda: ops.embed_tokens(ids, t.double()),
+           lambda: ops.embed_tokens(ids, t.t()), lambda: ops.embed_tokens(ids.t(), t), lambda: ops.embed_tokens(ids, t, t[:2]), lambda: ops.embed_tokens(ids, t, t.half()),
+           lambda: ops.embed_tokens(ids, t, torch.zeros(4, 9, device=DEV)), lambda: ops.embed_tokens(ids, t, t.cpu()), lambda: ops.embed_tokens(ids[0, 0], t),
+           lambda: ops.embed_tokens_bwd(ids, dy[:1], 4), lambda: ops.embed_tokens_bwd(ids, dy, 4, padding_idx=4), lambda: ops.embed_tokens_bwd(ids, dy, 4, padding_idx=-1),
+           lambda: ops.embed_tokens_bwd(ids, dy.double(), 4), lambda: ops.embed_positions_bwd(dy, 2), lambda: ops.embed_tokens(ids, torch.zeros(0, 8, device=DEV))]
+    for i, call in enumerate(bad):
+        with pytest.raises(GeodiffError):
+            call()
+            pytest.fail(str(i))
+
+
+# ------------------------------------------------------------------------------------------------ block norms
+EPS = 1e-5
+
+
+def _norm64(v, kind, gamma, beta, eps):
+    """-> (output, xh, r, magnitudes of what a value of xh is made of)."""
+    mean = v.mean(-1, keepdim=True) if kind == "layer" else torch.zeros_like(v[..., :1])
+    r = ((v - mean).pow(2).mean(-1, keepdim=True) + eps).rsqrt()
+    xh = (v - mean) * r
+    y = xh if gamma is None else xh * gamma
+    return (y if beta is None else y + beta), xh, r
+
+
+def _block_ref(x, res, pre, post, gate, res_scale, gy=None, gs=None):
+    """Values and magnitudes (sums of the absolute values of all terms) of the forward and of the gradients, in 64 bits."""
+    d = lambda t: None if t is None else t.double()
+    X, R, G = d(x), d(res), d(gate)
+    if G is not None and G.dim() == 2 and x.dim() > 2:
+        G = G.view(G.shape[0], *([1] * (x.dim() - 2)), G.shape[1])
+    one = lambda t, like: torch.ones_like(like) if t is None else d(t).expand_as(like)
+    v, m = {}, {}
+    if post is not None:
+        h, xh, xr = _norm64(X, post.kind, d(post.gamma), d(post.beta), post.eps)
+        # an error of the mean or the values reaches xh as (|v| + mean |v|) r, one of r as |xh|
+        mxh = (X.abs() + X.abs().mean(-1, keepdim=True)) * xr + xh.abs()
+        mh = mxh * one(post.gamma, X).abs() + (0 if post.beta is None else d(post.beta).abs())
+    else:
+        h, mh = X, X.abs()
+    s = h if G is None else G * h
+    ms = mh if G is None else G.abs() * mh
+    if R is not None:
+        s, ms = s + res_scale * R, ms + abs(res_scale) * R.abs()
+    v["s"], m["s"] = s, ms
+    if pre is not None:
+        y, sh, sr = _norm64(s, pre.kind, d(pre.gamma), d(pre.beta), pre.eps)
+        # the sum's own error (its magnitude) enters the mean and the deviation too
+        msh = (ms + ms.mean(-1, keepdim=True)) * sr + sh.abs() * (1 + (ms * sh.abs()).mean(-1, keepdim=True) * sr)
+        v["y"], m["y"] = y, msh * one(pre.gamma, X).abs() + (0 if pre.beta is None else d(pre.beta).abs())
+    if gy is None and gs is None:
+        return v, m
+    lead = tuple(range(x.dim() - 1))
+    over = lambda t, dims: t.sum(dims) if dims else t                # (torch sums over everything for no dimensions)
+    ds, mds = torch.zeros_like(s), torch.zeros_like(s)
+    if gy is not None:
+        g = d(gy) * one(pre.gamma, X)
+        gm = g.mean(-1, keepdim=True) if pre.kind == "layer" else 0.0
+        ds = sr * (g - gm - sh * (g * sh).mean(-1, keepdim=True))
+        ga = g.abs()
+        mds = sr * (ga + ga.mean(-1, keepdim=True) + msh * (ga * sh.abs()).mean(-1, keepdim=True) + sh.abs() * (ga * msh).mean(-1, keepdim=True))
+        mds = mds + ds.abs() * (1 + (ms * sh.abs()).mean(-1, keepdim=True) * sr)
+        v["dpre_gamma"], m["dpre_gamma"] = over(d(gy) * sh, lead), over(d(gy).abs() * msh, lead)
+        v["dpre_beta"], m["dpre_beta"] = over(d(gy), lead), over(d(gy).abs(), lead)
+    if gs is not None:
+        ds, mds = ds + d(gs), mds + d(gs).abs()
+    v["dres"], m["dres"] = res_scale * ds, abs(res_scale) * mds
+    dh, mdh = ds, mds
+    if G is not None:
+        dims = lead if gate.dim() == 1 else tuple(range(1, x.dim() - 1))
+        v["dgate"], m["dgate"] = over(ds * h, dims), over(mds * h.abs() + ds.abs() * mh, dims)
+        dh, mdh = G * ds, G.abs() * mds
+    if post is not None:
+        v["dpost_gamma"], m["dpost_gamma"] = over(dh * xh, lead), over(mdh * xh.abs() + dh.abs() * mxh, lead)
+        v["dpost_beta"], m["dpost_beta"] = over(dh, lead), over(mdh, lead)
+        gam = one(post.gamma, X)
+        g, mg = dh * gam, mdh * gam.abs()
+        gm = g.mean(-1, keepdim=True) if post.kind == "layer" else 0.0
+        dh = xr * (g - gm - xh * (g * xh).mean(-1, keepdim=True))
+        mdh = xr * (mg + mg.mean(-1, keepdim=True) + mxh * (g * xh).abs().mean(-1, keepdim=True) + xh.abs() * (mg * xh.abs() + g.abs() * mxh).mean(-1, keepdim=True))
+        mdh = mdh + dh.abs() * (1 + (X.abs() * xh.abs()).mean(-1, keepdim=True) * xr)
+    v["dx"], m["dx"] = dh, mdh
+    return v, m
+
+
+# roundings on any path of one row's arithmetic: 16 channels a thread, 6 + 16 additions across threads, and fewer than 30 in the formulas
+K_ROW = 64
+
+
+def _check_block(ops, x, res, pre, post, gate, res_scale, gy, gs):
+    s, y, stats = ops.block_norm(x, res, pre, post=post, gate=gate, res_scale=res_scale)
+    v, m = _block_ref(x, res, pre, post, gate, res_scale, gy, gs)
+    _close(s, v["s"], K_ROW, m["s"], "s")
+    if pre is None:
+        assert y is None
+    else:
+        _close(y, v["y"], K_ROW, m["y"], "y")
+    if gy is None and gs is None:
+        return
+    d = ops.block_norm_bwd(x, res, gy, gs, stats, pre, post=post, gate=gate, res_scale=res_scale)
+    rows = x.numel() // x.shape[-1]
+    there = dict(dx=x, dres=res, dgate=gate, dpost_gamma=post and post.gamma, dpost_beta=post and post.beta, dpre_gamma=pre and pre.gamma, dpre_beta=pre and pre.beta)
+    for k, t in there.items():
+        if t is None:
+            assert d[k] is None, k
+            continue
+        assert d[k].dtype == t.dtype and d[k].shape == t.shape, k
+        if gy is None and k.startswith("dpre"):
+            assert not bool(d[k].any())
+            continue
+        # the rows' own arithmetic twice (forward again, backward); sums over rows: one more addition a row at most
+        _close(d[k], v[k], 2 * K_ROW + (0 if k in ("dx", "dres") else rows), m[k], k)
+    again = ops.block_norm_bwd(x, res, gy, gs, stats, pre, post=post, gate=gate, res_scale=res_scale)
+    assert all(t is None or torch.equal(t, again[k]) for k, t in d.items())
+
+
+def _block_case(ops, shape, dtype, kind, gate, post, res, seed, affine=True, beta=True, strided=False, off=False):
+    g = _gen(seed)
+    C = shape[-1]
+    mis = _misaligned if off else lambda t: t
+    norm = lambda kd: ops.Norm(kd, mis(_randn(g, C, dtype=dtype, std=0.2, mean=1.0)) if affine else None,
+                               _randn(g, C, dtype=dtype, std=0.2) if affine and beta else None, EPS)
+    x = mis(_randn(g, *shape, dtype=dtype, std=0.8, mean=0.3))
+    r = _randn(g, *shape, dtype=dtype, std=1.5, mean=-0.2) if res else None
+    gt = None
+    if gate == "channel":
+        gt = _randn(g, C, dtype=dtype, std=0.4, mean=0.7)
+    elif gate == "sample":
+        gt = _randn(g, shape[0], 3 * C if strided else C, dtype=dtype, std=0.4, mean=0.7)
+        gt = gt[:, C:2 * C] if strided else gt
+    return x, r, norm(kind), norm("rms" if kind == "layer" and seed % 2 else kind) if post else None, gt, _randn(g, *shape, dtype=dtype), _randn(g, *shape, dtype=dtype, std=0.6)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("kind,gate,post,res,scale", [
+    ("layer", None, False, True, 1.0), ("rms", "sample", True, True, 0.5), ("layer", "channel", True, True, 1.0), ("rms", None, True, False, 1.0),
+    ("layer", "sample", False, False, 1.0), ("rms", "channel", False, True, -2.0), ("layer", None, False, False, 1.0)])
+@pytest.mark.parametrize("shape", [(1, 1, 8), (1, 77, 1024), (3, 5, 333), (2, 130, 320), (5, 1, 513), (2, 37, 2048)])
+def test_block_norm(ops, dtype, kind, gate, post, res, scale, shape):
+    x, r, pre, po, gt, gy, gs = _block_case(ops, shape, dtype, kind, gate, post, res, sum(shape))
+    _check_block(ops, x, r, pre, po, gt, scale, gy, gs)
+
+
+@gpu
+@pytest.mark.parametrize("C", [1, 2, 7, 64, 65, 512, 520, 1000, 1024, 1025, 1032, 1500, 2056, 4096, 4097, 4104, 8192, 8200, 16383, 16384])
+def test_block_norm_widths(ops, C):
+    for dtype in (torch.float32, torch.bfloat16):
+        x, r, pre, po, gt, gy, gs = _block_case(ops, (2, 6, C), dtype, "layer", "sample", True, True, C)
+        _check_block(ops, x, r, pre, po, gt, 1.0, gy, gs)
+
+
+@gpu
+@pytest.mark.parametrize("shape", [(1, 1, 40), (40,), (3, 40), (1, 3, 40), (2, 2, 40), (2, 1023, 40), (700, 3, 40), (2, 3, 4, 5, 40), (1, 5000, 40), (300, 7, 24)])
+def test_block_norm_row_counts_and_gate_rows(ops, shape):
+    """Rows of one gate that end inside, at and across a workgroup's rows; a 2-d gate beside 2-d activations is a gate for each row."""
+    for gate in ("channel", "sample") if len(shape) > 1 else ("channel",):
+        x, r, pre, po, gt, gy, gs = _block_case(ops, shape, torch.float32, "rms", gate, True, True, 3)
+        _check_block(ops, x, r, pre, po, gt, 1.0, gy, gs)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_block_norm_layouts_and_missing_parts(ops, dtype):
+    for C in (96, 333):
+        x, r, pre, po, gt, gy, gs = _block_case(ops, (3, 9, C), dtype, "layer", "sample", True, True, 8, strided=True)
+        assert not gt.is_contiguous()
+        _check_block(ops, x, r, pre, po, gt, 0.7, gy, gs)
+        x, r, pre, po, gt, gy, gs = _block_case(ops, (3, 9, C), dtype, "rms", "channel", True, True, 9, off=True)
+        _check_block(ops, x, r, pre, po, gt, 0.7, gy, gs)
+        x, r, pre, po, gt, gy, gs = _block_case(ops, (3, 9, C), dtype, "layer", "channel", True, True, 10, affine=False)
+        _check_block(ops, x, r, pre, po, gt, 1.0, gy, gs)
+        x, r, pre, po, gt, gy, gs = _block_case(ops, (3, 9, C), dtype, "layer", None, True, True, 11, beta=False)
+        _check_block(ops, x, r, pre, po, gt, 1.0, gy, None)
+        _check_block(ops, x, r, pre, po, gt, 1.0, None, gs)
+        _check_block(ops, x, r, None, po, gt, 1.0, None, gs)                         # no norm in front of the next block
+        _check_block(ops, x, r, None, None, gt, 1.0, None, gs)
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["layer", "rms"])
+@pytest.mark.parametrize("C", [40, 1024, 3000])
+def test_block_norm_hard_values(ops, kind, C):
+    """Equal values in a row (variance 0), a zero row, a large mean, large and tiny magnitudes; a NaN and an infinity stay in their rows."""
+    g = _gen(C)
+    x = _randn(g, 8, C)
+    x[0], x[1] = 3.25, 0.0
+    x[2] += 1000.0
+    x[3] *= 1e15
+    x[4] *= 1e-15
+    gy, gs = _randn(g, 8, C), _randn(g, 8, C)
+    _check_block(ops, x, None, ops.Norm(kind, _randn(g, C), None, 1e-6), None, None, 1.0, gy, gs)
+    x[5, 3], x[6, C - 1] = math.nan, math.inf
+    n = ops.Norm(kind, None, None, 1e-6)
+    s, y, stats = ops.block_norm(x, torch.zeros_like(x), n)
+    assert y[[0, 1, 2, 3, 4, 7]].isfinite().all() and y[5].isnan().all() and y[6, C - 1].isnan()
+    d = ops.block_norm_bwd(x, torch.zeros_like(x), gy, gs, stats, n)["dx"]
+    assert d[[0, 1, 2, 3, 4, 7]].isfinite().all() and d[5].isnan().all()
+
+
+@gpu
+def test_block_norm_need_and_empty(ops):
+    x, r, pre, po, gt, gy, gs = _block_case(ops, (2, 33, 64), torch.float32, "layer", "sample", True, True, 5)
+    _, _, stats = ops.block_norm(x, r, pre, po, gt)
+    full = ops.block_norm_bwd(x, r, gy, gs, stats, pre, po, gt)
+    for need in (["dx"], ["dgate"], ["dpre_beta", "dres"], ["dpost_gamma"], []):
+        part = ops.block_norm_bwd(x, r, gy, gs, stats, pre, po, gt, need=need)
+        for k, t in part.items():
+            assert (t is None) == (k not in need) and (t is None or torch.equal(t, full[k])), (k, need)
+    e = x[:, :0]
+    s, y, stats = ops.block_norm(e, r[:, :0], pre, po, gt)
+    assert s.shape == y.shape == e.shape
+    d = ops.block_norm_bwd(e, r[:, :0], e, e, stats, pre, po, gt)
+    assert d["dx"].shape == e.shape and not bool(d["dgate"].any()) and not bool(d["dpre_gamma"].any())
+    s, y, _ = ops.block_norm(x, None, pre)
+    assert s is x
+
+
+@gpu
+def test_block_norm_against_differences(ops):
+    """<gradient, direction> of the kernel against central differences, of the 64-bit formula and of the kernel's own forward at the same step."""
+    g = _gen(77)
+    x, r, pre, po, gt, gy, gs = _block_case(ops, (2, 3, 48), torch.float32, "layer", "sample", True, True, 4)
+    leaves = dict(dx=x, dres=r, dgate=gt, dpre_gamma=pre.gamma, dpre_beta=pre.beta, dpost_gamma=po.gamma, dpost_beta=po.beta)
+    dirs = {k: _randn(g, *t.shape) for k, t in leaves.items()}
+
+    def loss(h, f64):
+        c = lambda k, t: (t.double() + h * dirs[k].double()) if f64 else (t + h * dirs[k])
+        n, p = ops.Norm(pre.kind, c("dpre_gamma", pre.gamma), c("dpre_beta", pre.beta), EPS), ops.Norm(po.kind, c("dpost_gamma", po.gamma), c("dpost_beta", po.beta), EPS)
+        if f64:
+            v, _ = _block_ref(c("dx", x), c("dres", r), n, p, c("dgate", gt), 0.5)
+            s, y = v["s"], v["y"]
+        else:
+            s, y, _ = ops.block_norm(c("dx", x), c("dres", r), n, post=p, gate=c("dgate", gt), res_scale=0.5)
+        return float((gs.double() * s.double()).sum() + (gy.double() * y.double()).sum())
+
+    _, _, stats = ops.block_norm(x, r, pre, po, gt, 0.5)
+    d = ops.block_norm_bwd(x, r, gy, gs, stats, pre, po, gt, 0.5)
+    slope = sum(float((d[k].double() * dirs[k].double()).sum()) for k in leaves)
+    v, m = _block_ref(x, r, pre, po, gt, 0.5, gy, gs)
+    mag = sum(float((m[k] * dirs[k].double().abs()).sum()) for k in leaves)
+    h = 2.0 ** -17                                        # truncation ~ h^2 times third derivatives of order 1e3 (rows of deviation ~ 1): below 1e-7 of mag
+    assert abs((loss(h, True) - loss(-h, True)) / (2 * h) - slope) <= (2 * K_ROW + 8) * U32 * mag + 1e-6 * mag
+    h = 2.0 ** -5                                         # the kernel against the formula at the same points: the outputs' rounding over 2 h
+    _, mf = _block_ref(x, r, pre, po, gt, 0.5)
+    noise = float((gs.double().abs() * mf["s"]).sum() + (gy.double().abs() * mf["y"]).sum())
+    # (x + h d rounds too, by one step: 2 K_ROW covers it; 4: the magnitudes at the moved points)
+    assert abs((loss(h, False) - loss(-h, False)) - (loss(h, True) - loss(-h, True))) <= 2 * 4 * 2 * K_ROW * U32 * noise
+
+
+def test_block_norm_refuses_cpu_tensors():
+    from geodiffuser_amd import ops
+    with pytest.raises(GeodiffError, match="GPU tensor"):
+        ops.block_norm(torch.zeros(2, 8), None, ops.Norm("layer"))
+
+
+@gpu
+def test_block_norm_refusals(ops):
+    x, n = torch.zeros(2, 3, 8, device=DEV), ops.Norm("layer")
+    c = torch.ones(8, device=DEV)
+    st = torch.zeros(6, 4, device=DEV)
+    big = torch.zeros(1, 16385, device=DEV)
+    bad = [lambda: ops.block_norm(x.double(), None, n), lambda: ops.block_norm(x.transpose(0, 1), None, n), lambda: ops.block_norm(x, x[:1], n), lambda: ops.block_norm(x, x.half(), n),
+           lambda: ops.block_norm(x, None, None), lambda: ops.block_norm(x, None, ops.Norm("batch")), lambda: ops.block_norm(x, None, ops.Norm("layer", c[:4])),
+           lambda: ops.block_norm(x, None, ops.Norm("layer", c.half())), lambda: ops.block_norm(x, None, n, gate=torch.ones(3, 8, device=DEV)),
+           lambda: ops.block_norm(x, None, n, gate=torch.ones(8, 2, device=DEV).t()), lambda: ops.block_norm(x, None, n, gate=c.cpu()), lambda: ops.block_norm(big, None, n),
+           lambda: ops.block_norm(x, None, n, gate=torch.ones(1, 1, 8, device=DEV)), lambda: ops.block_norm(x, None, n, gate=c[None].expand(2, 8)),
+           lambda: ops.block_norm_bwd(x, None, None, None, st, n), lambda: ops.block_norm_bwd(x, x, x, None, st[:5], n), lambda: ops.block_norm_bwd(x, x, x, None, st, None),
+           lambda: ops.block_norm_bwd(x, x, x, None, st, n, need=["dy"]), lambda: ops.block_norm_bwd(x, x, x[:1], None, st, n),
+           lambda: ops.block_norm(torch.zeros(70000, 8, device=DEV), None, n, gate=torch.ones(70000, 8, device=DEV)), lambda: ops.block_norm(x[..., :0], None, n)]
+    for i, call in enumerate(bad):
+        with pytest.raises(GeodiffError):
+            call()
+            pytest.fail(str(i))
+
+
+# ------------------------------------------------------------------------------------------------ gradient norm and clipping
+def _norm_ref(ts, kind=2.0):
+    flat = torch.cat([t.double().flatten() for t in ts])
+    if kind == 2.0:
+        return flat.square().sum().sqrt()
+    return flat.abs().max() if flat.numel() else flat.sum()
+
+
+def _check_clip(ops, ts, max_norm, kind=2.0):
+    keep = [t.clone() for t in ts]
+    ref = _norm_ref(ts, kind)
+    n = ops.grad_norm(ts, kind)
+    assert n.shape == () and n.dtype == torch.float32
+    # binary64 inside: the conversion to f32 and nothing else that 2^-24 could see
+    _close(n, ref, 1, ref)
+    assert all(torch.equal(a, b) for a, b in zip(ts, keep))
+    f = min(1.0, max_norm / (float(ref) + 1e-6))
+    out = [torch.full_like(t, 7.0) for t in ts]
+    assert torch.equal(ops.clip_grad_norm(ts, max_norm, kind, out=out), n) and all(torch.equal(a, b) for a, b in zip(ts, keep))
+    for t, o in zip(ts, out):
+        _close(o, t.double() * f, 2, (t.double() * f).abs())              # the factor to f32, the product
+    assert torch.equal(ops.clip_grad_norm(ts, max_norm, kind), n) and all(torch.equal(a, b) for a, b in zip(ts, out))
+    return f
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("sizes", [(1,), (0, 3, 0), (78848,), (8191, 8192, 8193, 16384, 5), (7, 8, 9, 64, 1000003), (3,) * 127, (11,) * 128, (5,) * 129, tuple(range(300)), (70001,) * 260])
+def test_gradient_norm_and_clipping(ops, dtype, sizes):
+    for max_norm in (1e-3, 1e6):
+        g = torch.Generator(device=DEV).manual_seed(len(sizes))
+        ts = [torch.randn(n, generator=g, device=DEV).to(dtype) for n in sizes]
+        f = _check_clip(ops, ts, max_norm)
+        assert (f < 1) == (max_norm < 1)
+
+
+@gpu
+def test_clipping_mixed_types_and_layouts(ops):
+    """Tensors of all three types packed without gaps in a buffer (starts at any multiple of the element), channels_last and 0-d ones."""
+    for k in range(3):
+        g = _gen(k)
+        ts = []
+        for dtype in DTYPES:
+            sizes = [int(n) for n in torch.randint(1, 40000, (12,), generator=g)]
+            flat = _randn(g, sum(sizes), dtype=dtype)
+            ts += list(flat.split(sizes))
+        ts += [_randn(g, 8, 6, 3, 3, dtype=torch.bfloat16).to(memory_format=torch.channels_last), _randn(g, 1)[0], _randn(g, 5, 0, 3)]
+        for kind in (2.0, math.inf):
+            _check_clip(ops, [t.clone() if i > 35 else t for i, t in enumerate(ts)], 0.05, kind)
+
+
+@gpu
+def test_clipping_into_buffers_of_another_alignment(ops):
+    g = _gen(5)
+    for dtype in DTYPES:
+        src = [_randn(g, n, dtype=dtype) for n in (1, 100, 8195, 30000)]
+        dst = [_misaligned(torch.zeros_like(t)) for t in src]
+        n = ops.clip_grad_norm(src, 0.5, out=dst)
+        want = [torch.empty_like(t) for t in src]
+        ops.clip_grad_norm(src, 0.5, out=want)
+        assert all(torch.equal(a, b) for a, b in zip(dst, want)) and float(n) > 0.5
+        flat = torch.full((40,), 9.0, device=DEV, dtype=dtype)                    # nothing outside a destination is written
+        ops.clip_grad_norm([src[1][:10]], 1e9, out=[flat[15:25]])
+        assert torch.equal(flat[15:25], src[1][:10]) and bool((flat[:15] == 9).all()) and bool((flat[25:] == 9).all())
+
+
+@gpu
+def test_gradient_norm_of_extreme_values(ops):
+    one = lambda v, dt=torch.float32: torch.full((300,), v, device=DEV, dtype=dt)
+    for v in (1e30, 1e-30, 1e-42):                                                # squares beyond the range of f32 on either side
+        _close(ops.grad_norm([one(v)]), torch.tensor(float(one(v)[0]) * 300 ** 0.5, dtype=torch.float64, device=DEV), 1, torch.tensor(v, device=DEV))
+    _close(ops.grad_norm([one(3e38, torch.bfloat16)]), torch.tensor(math.inf, device=DEV), 0, torch.zeros((), device=DEV))
+    t = [one(3e38)]                                                               # a norm above f32's range still clips to max_norm
+    assert float(ops.clip_grad_norm(t, 1.0)) == math.inf
+    assert abs(float(_norm_ref(t)) - 1.0) < 1e-5
+    z = [torch.zeros(10, device=DEV)]
+    assert float(ops.clip_grad_norm(z, 1.0)) == 0.0 and not bool(z[0].any())
+    assert float(ops.clip_grad_norm([one(2.0)], 0.0)) > 0
+
+
+@gpu
+@pytest.mark.parametrize("kind", [2.0, math.inf])
+@pytest.mark.parametrize("where", [0, 8191, 19999])
+def test_gradient_norm_of_nan_and_inf(ops, kind, where):
+    for count in (1, 200):
+        ts = [torch.ones(20000, device=DEV) for _ in range(count)]
+        ts[-1][where] = -math.inf
+        assert float(ops.grad_norm(ts, kind)) == math.inf
+        c = [t.clone() for t in ts]
+        assert float(ops.clip_grad_norm(c, 1.0, kind)) == math.inf                 # factor 0, as max / inf is
+        assert bool(c[-1][where].isnan()) and float(c[-1].nan_to_num().abs().sum()) == 0
+        ts[-1][where] = math.nan
+        assert math.isnan(float(ops.grad_norm(ts, kind)))
+        ops.clip_grad_norm(ts, 1.0, kind)
+        assert all(bool(t.isnan().all()) for t in ts)
+
+
+@gpu
+def test_clipping_beyond_32_bits(ops):
+    t = torch.zeros((1 << 31) + 4097, dtype=torch.bfloat16, device=DEV)
+    t[-1], t[1 << 31], t[0] = 3.0, 4.0, 12.0
+    assert float(ops.clip_grad_norm([t, t.new_full((5,), 0.0)], 6.5)) == 13.0
+    assert [float(t[i]) for i in (-1, 1 << 31, 0, 1)] == [1.5, 2.0, 6.0, 0.0]
+
+
+def test_gradient_norm_refusals_on_the_host():
+    """The library's own checks, with addresses that are never followed."""
+    from geodiffuser_amd import _lib, ops
+    lib = _lib.load()
+    with pytest.raises(GeodiffError, match="GPU tensors"):
+        ops.grad_norm([torch.zeros(4)])
+    with pytest.raises(GeodiffError, match="no tensors"):
+        ops.clip_grad_norm([], 1.0)
+    with pytest.raises(GeodiffError, match="norm_type"):
+        ops.grad_norm([torch.zeros(4)], 1.0)
+
+    def call(src, dst, n, dt, max_norm=1.0, nbytes=1 << 20):
+        k = len(src)
+        arr = lambda t, v: (t * k)(*v)
+        return lib.gd_grad_norm(arr(ctypes.c_void_p, src), None if dst is None else arr(ctypes.c_void_p, dst), arr(ctypes.c_int64, n), arr(ctypes.c_int32, dt), k, 0, max_norm,
+                                ctypes.c_void_p(4096), nbytes, ctypes.c_void_p(64), None)
+
+    A, B = 1 << 20, 1 << 24
+    F32, F16 = _lib.GD_F32, _lib.GD_F16
+    assert call([A], None, [-1], [F32]) == -1 and call([A], None, [4], [7]) == -1 and call([A + 2], None, [4], [F32]) == -1 and call([0], None, [4], [F32]) == -1
+    assert call([A], [0], [4], [F32]) == -1 and call([A], [A], [4], [F32], max_norm=-1.0) == -1 and call([A], [A], [4], [F32], max_norm=math.nan) == -1
+    assert call([A], None, [4], [F32], nbytes=8) == -2
+    for src, dst, n, dt in (([A, A], [A, A], [4, 4], [F32, F32]),                              # the same tensor twice
+                            ([A, A + 8], [A, A + 8], [4, 4], [F32, F32]),                      # two that share elements
+                            ([A], [A + 4], [4], [F32]),                                        # into itself, moved
+                            ([A, B], [B, A], [4, 4], [F32, F32]),                              # into each other
+                            ([A, B], [A, B], [1 << 23, 4], [F16, F16])):                       # the second inside the first
+        assert call(src, dst, n, dt) == -1 and b"overlaps" in lib.gd_last_error(), (src, dst)
+
+
+@gpu
+def test_clipping_refusals(ops):
+    t = torch.ones(4, 6, device=DEV)
+    bad = [lambda: ops.grad_norm([t, t.cpu()]), lambda: ops.grad_norm([t.t()]), lambda: ops.grad_norm([t[:, :3]]), lambda: ops.grad_norm([t.double()]), lambda: ops.grad_norm([t.int()]),
+           lambda: ops.clip_grad_norm([t], -1.0), lambda: ops.clip_grad_norm([t], math.nan), lambda: ops.clip_grad_norm([t, t], 1.0), lambda: ops.clip_grad_norm([t, t[1:]], 1.0),
+           lambda: ops.clip_grad_norm([t], 1.0, out=[]), lambda: ops.clip_grad_norm([t], 1.0, out=[t.half()]), lambda: ops.clip_grad_norm([t], 1.0, out=[t.reshape(6, 4)]),
+           lambda: ops.clip_grad_norm([t[:2], t[2:]], 1.0, out=[t[1:3], torch.empty_like(t[:2])]), lambda: ops.grad_norm([t], 3)]
+    for i, call in enumerate(bad):
+        with pytest.raises(GeodiffError):
+            call()
+            pytest.fail(str(i))
+    assert float(t.sum()) == 24
+
+
+# ------------------------------------------------------------------------------------------------ streams, graphs
+@gpu
+def test_training_ops_on_another_stream_and_replayed_in_graphs(ops):
+    """Every operator on a side stream, and captured: two graphs replayed in turn on new inputs, with eager work between, against the eager results."""
+    g = _gen(1)
+    V, C = 900, 136
+    ids = torch.randint(0, V, (40, 77), generator=g).to(DEV)
+    table, pos = _randn(g, V, C), _randn(g, 77, C)
+    x, r, pre, po, gt, gy, gs = _block_case(ops, (4, 50, C), torch.float32, "layer", "sample", True, True, 2)
+    dy = _randn(g, 40, 77, C)
+    grads = [_randn(g, n) for n in (5, 9000, 70000)]
+    bufs = [torch.empty_like(t) for t in grads]
+
+    def all_ops():
+        s, y, stats = ops.block_norm(x, r, pre, po, gt)
+        d = ops.block_norm_bwd(x, r, gy, gs, stats, pre, po, gt)
+        n = ops.clip_grad_norm(grads, 1.0, out=bufs)
+        return [ops.embed_tokens(ids, table, pos), ops.embed_tokens_bwd(ids, dy, V), ops.embed_tokens_bwd(ids[:2], dy[:2], V), ops.embed_positions_bwd(dy, 80), s, y,
+                *d.values(), n, *[b.clone() for b in bufs], ops.grad_norm(grads, math.inf)]
+
+    want = all_ops()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = all_ops()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = all_ops()
+        graphs.append((graph, out))
+    inputs = (x, r, gy, gs, dy, table, *grads)
+    for k in range(3):
+        for t in inputs:
+            t.copy_(_randn(g, *t.shape))
+        ids.copy_(torch.randint(0, V, ids.shape, generator=g))
+        want = all_ops()
+        for graph, out in graphs if k % 2 else graphs[::-1]:
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(out, want)), k
+            want = all_ops()
+
+
+# ------------------------------------------------------------------------------------------------ as the framework uses them
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_text_tower_embedding_keeps_its_values_and_learns(ops, dtype):
+    """The tower's first layer through the operator: the bits of the unfused lookup and addition, and the gradients of table and positions."""
+    from geodiffuser_amd.pipeline import TextEncoder
+    torch.manual_seed(0)
+    te = TextEncoder(width=64, layers=2, heads=2, vocab=500).to(DEV, dtype).eval()
+    ids = torch.randint(0, 500, (3, 77), generator=_gen(2)).to(DEV)
+    ids[:, 20:] = 0
+    seen = []
+    h = te.layers[0].register_forward_pre_hook(lambda m, a: seen.append(a[0]))
+    with torch.no_grad():
+        te(ids)
+    te(ids)
+    h.remove()
+    want = te.tok(ids) + te.pos[:77]
+    assert torch.equal(seen[0], want) and torch.equal(seen[1], want) and "EmbedFn" in type(seen[1].grad_fn).__name__
+    gy = _randn(_gen(3), 3, 77, 64, dtype=dtype)
+    dt, dp = torch.autograd.grad(seen[1], [te.tok.weight, te.pos], gy)
+    ref = torch.zeros(500, 64, dtype=torch.float64, device=DEV).index_add_(0, ids.flatten(), gy.double().reshape(-1, 64))
+    mag = torch.zeros_like(ref).index_add_(0, ids.flatten(), gy.double().abs().reshape(-1, 64))
+    _close(dt, ref, 3 * 77, mag)
+    _close(dp, gy.double().sum(0), 3, gy.double().abs().sum(0))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_transformer_block_with_trainable_norms(ops, dtype):
+    """A block whose norms learn runs them on block_norm; against the same block on stock modules in 64 bits, each gradient in relative 2-norm.
+    Both round every intermediate tensor to T: about 40 such roundings lie between the loss and the first norm's gradient, each relative u in
+    2-norm; 40 u bounds their sum with nothing cancelling."""
+    from geodiffuser_amd import unet_sd21 as U
+
+    class Plain:
+        def __call__(self, attn, hidden_states, encoder_hidden_states=None, **kw):
+            c = hidden_states if encoder_hidden_states is None else encoder_hidden_states
+            return attn.to_out[0](attn.to_q(hidden_states) * torch.tanh(attn.to_k(c).mean(1, keepdim=True) + attn.to_v(c).mean(1, keepdim=True)))
+
+    torch.manual_seed(3)
+    blk = U.BasicTransformerBlock(128, 2, 64, 96).to(DEV, dtype).eval()
+    for n, p in blk.named_parameters():
+        p.requires_grad_("norm" in n)
+        if "norm" in n:
+            p.data.add_(_randn(_gen(len(n)), *p.shape, std=0.2).to(dtype))
+    for a in (blk.attn1, blk.attn2):
+        a.processor = Plain()
+    x, ctx, w = (_randn(_gen(i), *s, dtype=dtype) for i, s in enumerate(((2, 65, 128), (2, 7, 96), (2, 65, 128))))
+    calls = []
+    saved = ops.block_norm
+    ops.block_norm = lambda *a, **k: calls.append(1) or saved(*a, **k)
+    try:
+        y = blk(x, ctx)
+        (y.float() * w.float()).sum().backward()
+    finally:
+        ops.block_norm = saved
+    assert len(calls) == 3
+    import copy
+    ref = copy.deepcopy(blk).cpu().double()
+    ref.zero_grad()
+    for a in (ref.attn1, ref.attn2):
+        a.processor = Plain()
+    yr = ref(x.cpu().double(), ctx.cpu().double())
+    (yr * w.cpu().double()).sum().backward()
+    u = 40 * torch.finfo(dtype).eps / 2
+    rel = lambda a, b: float((a.detach().cpu().double() - b.detach()).norm() / b.detach().norm())
+    assert rel(y, yr) < u
+    for (n, p), q in zip(blk.named_parameters(), ref.parameters()):
+        if "norm" in n:
+            assert rel(p.grad, q.grad) < u, (n, rel(p.grad, q.grad), u)
+        else:
+            assert p.grad is None
+
+
+@gpu
+def test_a_training_step_of_the_text_tower(ops):
+    """Embedding, gated block norms and clipping as one step: every gradient against the same step on plain torch operations in 64 bits, the
+    clipped norm, and a second identical step from the same state."""
+    from geodiffuser_amd import training as T
+    g = _gen(12)
+    V, C, B, L = 300, 96, 5, 31
+    ids = torch.randint(0, V, (B, L), generator=g)
+    ids[:, 12:] = 0
+    init = dict(table=_randn(g, V, C, std=0.5), pos=_randn(g, 77, C, std=0.2), w=_randn(g, C, C, std=C ** -0.5), gate=_randn(g, B, C), g1=_randn(g, C, mean=1.0, std=0.1),
+                b1=_randn(g, C, std=0.1), g2=_randn(g, C, mean=1.0, std=0.1), g3=_randn(g, C, mean=1.0, std=0.1))
+    tgt = _randn(g, B, L, C)
+
+    def step():
+        p = {k: v.clone().requires_grad_() for k, v in init.items()}
+        x = T.embed_tokens(ids.to(DEV), p["table"], p["pos"], scale=C ** 0.5, padding_idx=0)
+        x, h = T.block_norm(x, None, T.Norm("layer", p["g1"], p["b1"]))
+        s, y = T.block_norm(h @ p["w"], x, T.Norm("rms", p["g3"]), post=T.Norm("rms", p["g2"]), gate=p["gate"], res_scale=0.5)
+        loss = ((y - tgt) ** 2).mean() + 0.1 * s.square().mean()
+        loss.backward()
+        raw = {k: v.grad.clone() for k, v in p.items()}
+        n = T.clip_grad_norm_(p.values(), 0.01)
+        return loss.detach(), n, raw, {k: v.grad for k, v in p.items()}
+
+    loss, n, raw, clipped = step()
+    q = {k: v.cpu().double().requires_grad_() for k, v in init.items()}
+    rms = lambda v, w: v / (v.pow(2).mean(-1, keepdim=True) + 1e-5).sqrt() * w
+    x = torch.nn.functional.embedding(ids, q["table"], padding_idx=0) * C ** 0.5 + q["pos"][:L]
+    h = torch.nn.functional.layer_norm(x, (C,), q["g1"], q["b1"], 1e-5)
+    s = 0.5 * x + q["gate"][:, None] * rms(h @ q["w"], q["g2"])
+    y = rms(s, q["g3"])
+    lr = ((y - tgt.cpu().double()) ** 2).mean() + 0.1 * s.square().mean()
+    lr.backward()
+    # f32 throughout: 300 roundings of 2^-24 relative in 2-norm lie between any input and any gradient (sums over C and B L included)
+    assert abs(float(loss) - float(lr)) <= 300 * U32 * float(lr)
+    for k in q:
+        assert float((raw[k].cpu().double() - q[k].grad).norm()) <= 300 * U32 * float(q[k].grad.norm()), k
+    total = math.sqrt(sum(float(v.grad.square().sum()) for v in q.values()))
+    assert abs(float(n) - total) <= 300 * U32 * total and total > 0.01
+    f = 0.01 / (total + 1e-6)
+    for k in q:
+        assert float((clipped[k].cpu().double() - f * q[k].grad).norm()) <= 600 * U32 * f * float(q[k].grad.norm()), k
+    again = step()
+    assert torch.equal(again[1], n) and all(torch.equal(again[3][k], clipped[k]) for k in ("table", "pos", "gate", "g2", "g3"))
+
+
+@gpu
+def test_block_norm_autograd_without_some_gradients(ops):
+    from geodiffuser_amd import training as T
+    x, r, pre, po, gt, gy, gs = _block_case(ops, (2, 9, 40), torch.float32, "layer", "channel", True, True, 6)
+    x.requires_grad_(), gt.requires_grad_()
+    s, y = T.block_norm(x, r, pre, po, gt, 0.5)
+    (dx, dg) = torch.autograd.grad(y, [x, gt], gy, retain_graph=True)               # s is not used
+    v, m = _block_ref(x.detach(), r, pre, po, gt.detach(), 0.5, gy, None)
+    _close(dx, v["dx"], 2 * K_ROW, m["dx"])
+    _close(dg, v["dgate"], 2 * K_ROW + 18, m["dgate"])
+    (dx,) = torch.autograd.grad(s, [x], gs.transpose(0, 1).contiguous().transpose(0, 1))      # y is not used; a strided incoming gradient
+    v, m = _block_ref(x.detach(), r, None, po, gt.detach(), 0.5, None, gs)
+    _close(dx, v["dx"], 2 * K_ROW, m["dx"])
+    s, y = T.block_norm(x, None, pre)                                                # s is x: both of its uses reach it
+    (dx,) = torch.autograd.grad([s, y], [x], [gs, gy])
+    v, m = _block_ref(x.detach(), None, pre, None, None, 1.0, gy, gs)
+    _close(dx, v["dx"], 2 * K_ROW, m["dx"])
+    with torch.no_grad():
+        assert not T.block_norm(x, None, pre)[1].requires_grad
+
+
+@gpu
+def test_clip_grad_norm_of_parameters(ops):
+    from geodiffuser_amd import training as T
+    m = torch.nn.Sequential(torch.nn.Linear(30, 40), torch.nn.LayerNorm(40), torch.nn.Linear(40, 3)).to(DEV)
+    m[1].bias.requires_grad_(False)
+    m(torch.randn(5, 30, device=DEV)).square().sum().backward()
+    ref = [p.grad.clone() for p in m.parameters() if p.grad is not None]
+    n = T.clip_grad_norm_(m.parameters(), 0.3)
+    total = float(_norm_ref(ref))
+    assert total > 0.3 and abs(float(n) - total) <= 2 * U32 * total
+    for p, r in zip([p for p in m.parameters() if p.grad is not None], ref):
+        want = r.double() * (0.3 / (total + 1e-6))
+        _close(p.grad, want, 2, want.abs())
+    assert float(T.clip_grad_norm_(torch.nn.Parameter(torch.zeros(3)), 1.0)) == 0.0
+
+
+@gpu
+def test_null_text_optimisation_with_clipped_gradients(ops):
+    """NullInversion(max_grad_norm=...): the embedding's gradient is clipped before each Adam step.  Adam divides by the gradient's own size, so a
+    clip to a size far above its epsilon changes little, and one far below it nearly stops the optimisation; without it nothing changes."""
+    import cases
+    from geodiffuser_amd.diffusion import load_model
+    from geodiffuser_amd.inversion import NullInversion
+    p, tok, sched = load_model(device="cuda:0", tiny=True, dtype=torch.float16)
+    c = cases.NULL_TEXT
+    traj = [torch.from_numpy(a).cuda().half() for a in cases.null_text_inputs()]
+
+    def run(limit):
+        ni = NullInversion(p, num_ddim_steps=c["steps"], device="cuda:0", guidance_scale=c["guidance"], max_grad_norm=limit)
+        ni.init_prompt("")
+        return torch.cat(ni.null_optimization(traj, c["inner"], c["eps"])).float() - ni.context[:1].float()
+
+    free, loose, tight = run(None), run(1e9), run(1e-12)
+    assert torch.isfinite(tight).all() and float(loose.norm()) > 0.5 * float(free.norm()) > 0
+    assert float(tight.norm()) < 0.05 * float(free.norm())
