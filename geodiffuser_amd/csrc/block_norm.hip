@@ -18,28 +18,56 @@
 // the function that the forward computed, at the same traffic.
 #include "train_common.hpp"
 
+template <typename T> __device__ __forceinline__ uint32_t bits16(float x) {
+    if constexpr (sizeof(T) == 2) return __builtin_bit_cast(unsigned short, (T)x);
+    else return 0;
+}
+
 // How a thread's N channels lie in a row.  VEC: words of 16 bytes (8 or 4 channels), neighbouring threads on neighbouring words - needs
 // C * sizeof(T) and every pointer to be multiples of 16; otherwise element by element, neighbouring threads on neighbouring elements.
-template <typename T, int TPR, int N, bool VEC>
-struct bn_cols {
-    static constexpr int W = VEC ? (int)(16 / sizeof(T)) : 1;
+// An object holds them as they are stored (words: packed, half the registers for 16-bit types), so that a load is under way until a value
+// is asked for.
+template <typename T, int TPR, int N, bool VEC> struct bn_part {
+    static constexpr int W = VEC ? word16<T>::N : 1;
     static __device__ __forceinline__ int col(int t, int i) { return ((i / W) * TPR + t) * W + i % W; }
-    static __device__ __forceinline__ void load(const T* __restrict__ p, int t, int C, float* v) {
+    u32x4 word[VEC ? N / word16<T>::N : 1];
+    T one[VEC ? 1 : N];
+    __device__ __forceinline__ void load(const T* __restrict__ p, int t, int C) {
+        if constexpr (VEC) {
 #pragma unroll
-        for (int i = 0; i < N; i += W) {
-            const int c = col(t, i);
-            if (c < C) {
-                if constexpr (VEC) {
-                    const word16<T> a = *(const word16<T>*)(p + c);
-#pragma unroll
-                    for (int j = 0; j < W; ++j) v[i + j] = (float)a.v[j];
-                } else {
-                    v[i] = (float)p[c];
-                }
-            } else {
-#pragma unroll
-                for (int j = 0; j < W; ++j) v[i + j] = 0.f;
+            for (int i = 0; i < N; i += W) {
+                const int c = col(t, i);
+                word[i / W] = u32x4{0, 0, 0, 0};
+                if (c < C) word[i / W] = *(const u32x4*)(p + c);
             }
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int c = col(t, i);
+                one[i] = (T)0.f;
+                if (c < C) one[i] = p[c];
+            }
+        }
+    }
+    __device__ __forceinline__ void fill(float x) {
+        if constexpr (VEC) {
+            const uint32_t bits = sizeof(T) == 4 ? __builtin_bit_cast(uint32_t, x) : 0x10001u * bits16<T>(x);
+#pragma unroll
+            for (int i = 0; i < N / W; ++i) word[i] = u32x4{bits, bits, bits, bits};
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) one[i] = (T)x;
+        }
+    }
+    __device__ __forceinline__ float operator[](int i) const {
+        if constexpr (!VEC) return (float)one[i];
+        else if constexpr (sizeof(T) == 4) {
+            const uint32_t u = word[i / 4][i % 4];
+            return __builtin_bit_cast(float, u);
+        }
+        else {
+            const uint32_t two = word[i / 8][i % 8 / 2];
+            return (float)__builtin_bit_cast(T, (unsigned short)(i & 1 ? two >> 16 : two & 0xffffu));
         }
     }
     static __device__ __forceinline__ void store(T* __restrict__ p, int t, int C, const float* v) {
@@ -60,106 +88,113 @@ struct bn_cols {
     }
 };
 
-// sums of K values over the row's threads, in every one of them.  TPR > 64: `lds` holds 16 * K floats; the caller's row loop is uniform
-// over the workgroup, so the barriers are too.
+// sums of K values over the row's threads, in every one of them.  TPR > 64: through one half of `lds` (2 * K * 16 floats); the halves take
+// turns, so that one barrier a sum is enough (whoever writes a half again has passed the barrier of the sum between, behind its reads).
+// The caller's row loop is uniform over the workgroup.
 template <int TPR, int K>
-__device__ __forceinline__ void bn_row_sum(float* v, float* lds) {
+__device__ __forceinline__ void bn_row_sum(float* v, float* lds, int& turn) {
 #pragma unroll
-    for (int k = 0; k < K; ++k) v[k] = wave_sum(v[k]);
+    for (int k = 0; k < K; ++k) v[k] = wave_total(v[k]);
     if constexpr (TPR > 64) {
         constexpr int WAVES = TPR / 64;
-        __syncthreads();                                     // the previous sum has been read
+        float* half = lds + turn * 32;
+        turn ^= 1;
         if ((threadIdx.x & 63) == 0) {
 #pragma unroll
-            for (int k = 0; k < K; ++k) lds[k * WAVES + (threadIdx.x >> 6)] = v[k];
+            for (int k = 0; k < K; ++k) half[k * WAVES + (threadIdx.x >> 6)] = v[k];
         }
         __syncthreads();
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             float s = 0.f;
 #pragma unroll
-            for (int w = 0; w < WAVES; ++w) s += lds[k * WAVES + w];
+            for (int w = 0; w < WAVES; ++w) s += half[k * WAVES + w];
             v[k] = s;
         }
     }
 }
 
-// v -> (mean, 1 / deviation); mean is 0 for the rms norm
-template <typename COLS, int TPR, int N>
-__device__ __forceinline__ void bn_stats(const float* v, int t, int C, int kind, float eps, float* lds, float& mean, float& r) {
+// v -> (mean, 1 / deviation); mean is 0 for the rms norm.  Two passes over the registers: no cancellation for rows far from zero.
+template <typename PART, int TPR, int N>
+__device__ __forceinline__ void bn_stats(const float* v, int t, int C, int kind, float eps, float* lds, int& turn, float& mean, float& r) {
     mean = 0.f;
     if (kind == GD_NORM_LAYER) {
         float s = 0.f;
 #pragma unroll
         for (int i = 0; i < N; ++i) s += v[i];
-        bn_row_sum<TPR, 1>(&s, lds);
+        bn_row_sum<TPR, 1>(&s, lds, turn);
         mean = s / (float)C;
     }
     float q = 0.f;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        const float d = COLS::col(t, i) < C ? v[i] - mean : 0.f;
+        const float d = PART::col(t, i) < C ? v[i] - mean : 0.f;
         q = __builtin_fmaf(d, d, q);
     }
-    bn_row_sum<TPR, 1>(&q, lds);
+    bn_row_sum<TPR, 1>(&q, lds, turn);
     r = rsqrtf(q / (float)C + eps);
 }
 
 template <typename T, int TPR, int N, bool VEC>
 __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) k_block_norm(const gd_block_norm_t a) {
-    using COLS = bn_cols<T, TPR, N, VEC>;
+    using PART = bn_part<T, TPR, N, VEC>;
     constexpr int RPB = TPR < 256 ? 256 / TPR : 1;           // rows a workgroup
-    __shared__ float lds[16];
+    __shared__ float lds[64];
+    int turn = 0;
     const int t = threadIdx.x % TPR, C = a.C;
-    const long long row = (long long)blockIdx.x * RPB + threadIdx.x / TPR;
+    const long long row = (long long)blockIdx.x * RPB + (TPR < 256 ? __builtin_amdgcn_readfirstlane(threadIdx.x / TPR) : 0);
     if (row >= a.rows) return;                               // TPR >= 256: the whole workgroup has one row
-    float h[N], v[N], w[N];
-    COLS::load((const T*)a.x + row * C, t, C, h);
+    // everything that the row needs is on its way before the first sum waits for x
+    PART x, res, gate, og, ob, eg, eb;
+    x.load((const T*)a.x + row * C, t, C);
+    if (a.res) res.load((const T*)a.res + row * C, t, C);
+    if (a.post_gamma) og.load((const T*)a.post_gamma, t, C);
+    if (a.post_beta) ob.load((const T*)a.post_beta, t, C);
+    if (a.gate) gate.load((const T*)a.gate + (a.rows_per_gate == a.rows ? 0 : row / a.rows_per_gate) * a.gate_ld, t, C);
+    if (a.pre_gamma) eg.load((const T*)a.pre_gamma, t, C);
+    if (a.pre_beta) eb.load((const T*)a.pre_beta, t, C);
+    float h[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) h[i] = x[i];
     if (a.post_kind) {
         float mean, r;
-        bn_stats<COLS, TPR, N>(h, t, C, a.post_kind, a.post_eps, lds, mean, r);
+        bn_stats<PART, TPR, N>(h, t, C, a.post_kind, a.post_eps, lds, turn, mean, r);
         if (a.stats && t == 0) { a.stats[row * 4] = mean; a.stats[row * 4 + 1] = r; }
 #pragma unroll
-        for (int i = 0; i < N; ++i) h[i] = COLS::col(t, i) < C ? (h[i] - mean) * r : 0.f;
+        for (int i = 0; i < N; ++i) h[i] = PART::col(t, i) < C ? (h[i] - mean) * r : 0.f;
         if (a.post_gamma) {
-            COLS::load((const T*)a.post_gamma, t, C, w);
 #pragma unroll
-            for (int i = 0; i < N; ++i) h[i] *= w[i];
+            for (int i = 0; i < N; ++i) h[i] *= og[i];
         }
         if (a.post_beta) {
-            COLS::load((const T*)a.post_beta, t, C, w);
 #pragma unroll
-            for (int i = 0; i < N; ++i) h[i] += w[i];
+            for (int i = 0; i < N; ++i) h[i] += ob[i];
         }
     }
     if (a.gate) {
-        COLS::load((const T*)a.gate + (row / a.rows_per_gate) * a.gate_ld, t, C, w);
 #pragma unroll
-        for (int i = 0; i < N; ++i) h[i] *= w[i];
+        for (int i = 0; i < N; ++i) h[i] *= gate[i];
     }
     if (a.res) {
-        COLS::load((const T*)a.res + row * C, t, C, v);
 #pragma unroll
-        for (int i = 0; i < N; ++i) h[i] = __builtin_fmaf(a.res_scale, v[i], h[i]);
+        for (int i = 0; i < N; ++i) h[i] = __builtin_fmaf(a.res_scale, res[i], h[i]);
     }
-    if (a.s) COLS::store((T*)a.s + row * C, t, C, h);
+    if (a.s) PART::store((T*)a.s + row * C, t, C, h);
     if (!a.pre_kind) return;
     float mean, r;
-    bn_stats<COLS, TPR, N>(h, t, C, a.pre_kind, a.pre_eps, lds, mean, r);
+    bn_stats<PART, TPR, N>(h, t, C, a.pre_kind, a.pre_eps, lds, turn, mean, r);
     if (a.stats && t == 0) { a.stats[row * 4 + 2] = mean; a.stats[row * 4 + 3] = r; }
 #pragma unroll
     for (int i = 0; i < N; ++i) h[i] = (h[i] - mean) * r;
     if (a.pre_gamma) {
-        COLS::load((const T*)a.pre_gamma, t, C, w);
 #pragma unroll
-        for (int i = 0; i < N; ++i) h[i] *= w[i];
+        for (int i = 0; i < N; ++i) h[i] *= eg[i];
     }
     if (a.pre_beta) {
-        COLS::load((const T*)a.pre_beta, t, C, w);
 #pragma unroll
-        for (int i = 0; i < N; ++i) h[i] += w[i];
+        for (int i = 0; i < N; ++i) h[i] += eb[i];
     }
-    COLS::store((T*)a.y + row * C, t, C, h);
+    PART::store((T*)a.y + row * C, t, C, h);
 }
 
 // ---- backward -------------------------------------------------------------------------------------------------------------------------
@@ -177,7 +212,7 @@ struct bn_bwd_args {
 };
 
 // column sums of the workgroup's rows-in-parallel, then to the workspace (threads of the first row)
-template <typename COLS, int TPR, int N>
+template <typename PART, int TPR, int N>
 __device__ __forceinline__ void bn_flush(float* acc, float* __restrict__ out, int C, float* lds) {
     const int t = threadIdx.x % TPR;
     if constexpr (TPR < 256) {                               // one wave a row: the four waves' sums meet in LDS
@@ -185,17 +220,16 @@ __device__ __forceinline__ void bn_flush(float* acc, float* __restrict__ out, in
 #pragma unroll
         for (int i = 0; i < N; ++i) lds[(threadIdx.x >> 6) * (64 * N) + i * 64 + t] = acc[i];
         __syncthreads();
-        if (threadIdx.x < 64) {
+        // each wave adds and writes a quarter of the channels
 #pragma unroll
-            for (int i = 0; i < N; ++i) {
-                const int c = COLS::col(t, i);
-                if (c < C) out[c] = (lds[i * 64 + t] + lds[64 * N + i * 64 + t]) + (lds[2 * 64 * N + i * 64 + t] + lds[3 * 64 * N + i * 64 + t]);
-            }
+        for (int k = 0; k < N / 4; ++k) {
+            const int i = (threadIdx.x >> 6) * (N / 4) + k, c = PART::col(t, i);
+            if (c < C) out[c] = (lds[i * 64 + t] + lds[64 * N + i * 64 + t]) + (lds[2 * 64 * N + i * 64 + t] + lds[3 * 64 * N + i * 64 + t]);
         }
     } else {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int c = COLS::col(t, i);
+            const int c = PART::col(t, i);
             if (c < C) out[c] = acc[i];
         }
     }
@@ -203,143 +237,138 @@ __device__ __forceinline__ void bn_flush(float* acc, float* __restrict__ out, in
     for (int i = 0; i < N; ++i) acc[i] = 0.f;
 }
 
-template <typename T, int TPR, int N, bool VEC>
+// one row's data as the loop carries it from one turn to the next: its loads are under way while the row before it is worked on
+template <typename PART> struct bn_row {
+    PART x, res, gy, gs;
+    float stats[4];
+};
+
+// WRAP: there is a gate or a norm on x (their registers otherwise serve occupancy)
+template <typename T, int TPR, int N, bool VEC, bool WRAP>
 __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) k_block_norm_bwd(const bn_bwd_args b) {
-    using COLS = bn_cols<T, TPR, N, VEC>;
+    using PART = bn_part<T, TPR, N, VEC>;
     constexpr int RPB = TPR < 256 ? 256 / TPR : 1;
-    __shared__ float lds[TPR < 256 ? 4 * 64 * N : 32];
+    __shared__ float lds[TPR < 256 ? 4 * 64 * N : 64];
+    int turn = 0;
     const gd_block_norm_bwd_t& a = b.a;
-    const int t = threadIdx.x % TPR, C = a.f.C;
+    const int t = threadIdx.x % TPR, C = a.f.C, wave = TPR < 256 ? __builtin_amdgcn_readfirstlane(threadIdx.x / TPR) : 0;
     const long long r0 = (long long)blockIdx.x * b.rows_per_wg, r1 = r0 + b.rows_per_wg < a.f.rows ? r0 + b.rows_per_wg : a.f.rows;
-    float acc[BN_SUMS][N] = {}, acc_gate[N] = {};
-    const long long per = a.f.gate ? a.f.rows_per_gate : a.f.rows;
+    float pre_g[N] = {}, pre_b[N] = {}, post_g[N] = {}, post_b[N] = {}, dgate[N] = {};
+    PART og, ob, eg, gate;
+    if (a.f.pre_gamma) eg.load((const T*)a.f.pre_gamma, t, C); else eg.fill(1.f);
+    if constexpr (WRAP) {
+        if (a.f.post_gamma) og.load((const T*)a.f.post_gamma, t, C); else og.fill(1.f);
+        if (a.f.post_beta) ob.load((const T*)a.f.post_beta, t, C); else ob.fill(0.f);
+        gate.fill(1.f);
+    }
+    bn_row<PART> cur, next;
+    long long held = -1;                                     // the row in `next`
+    const auto fetch = [&](long long row) {
+        held = row;
+        next.x.load((const T*)a.f.x + row * C, t, C);
+        if (a.f.res) next.res.load((const T*)a.f.res + row * C, t, C); else next.res.fill(0.f);
+        if (a.gy) next.gy.load((const T*)a.gy + row * C, t, C); else next.gy.fill(0.f);
+        if (a.gs) next.gs.load((const T*)a.gs + row * C, t, C); else next.gs.fill(0.f);
+        if (a.f.stats) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) next.stats[k] = a.f.stats[row * 4 + k];
+        }
+    };
+    const long long per = WRAP && a.f.gate ? a.f.rows_per_gate : a.f.rows;
+    if (r0 + wave < r1) fetch(r0 + wave);
     for (long long g0 = r0; g0 < r1;) {
-        const long long gate_row = g0 / per;
+        const long long gate_row = per == a.f.rows ? 0 : g0 / per;
         const long long g1 = (gate_row + 1) * per < r1 ? (gate_row + 1) * per : r1;
-        for (long long base = g0; base < g1; base += RPB) {
-            const long long row = base + threadIdx.x / TPR;
-            if (row < g1) {                                  // (TPR >= 256: the same for the whole workgroup)
-                float h[N], xh[N], sv[N], w[N], d[N];
-                // forward again: xh = normalised x, h = post(x), sv = the sum
-                COLS::load((const T*)a.f.x + row * C, t, C, xh);
-                float post_r = 1.f;
-                if (a.f.post_kind) {
-                    const float mean = a.f.stats[row * 4];
-                    post_r = a.f.stats[row * 4 + 1];
+        if constexpr (WRAP) {
+            if (a.f.gate) gate.load((const T*)a.f.gate + gate_row * a.f.gate_ld, t, C);
+        }
+        for (long long row = g0 + wave; row < g1; row += RPB) {        // (TPR >= 256: the same rows for the whole workgroup)
+            if (held != row) fetch(row);                     // (a wave that had no row of the gate before)
+            cur = next;
+            // the row behind this one: of this gate, or the first of the next gate's rows
+            const long long then = row + RPB < g1 ? row + RPB : g1 + wave;
+            if (then < r1) fetch(then);
+            float d[N], sv[N], xh[N];
+            // forward again: xh = normalised x, h = post(x), sv = the sum
+            const float post_mean = WRAP && a.f.post_kind ? cur.stats[0] : 0.f, post_r = WRAP && a.f.post_kind ? cur.stats[1] : 1.f;
 #pragma unroll
-                    for (int i = 0; i < N; ++i) h[i] = xh[i] = COLS::col(t, i) < C ? (xh[i] - mean) * post_r : 0.f;
-                    if (a.f.post_gamma) {
-                        COLS::load((const T*)a.f.post_gamma, t, C, w);
+            for (int i = 0; i < N; ++i) {
+                xh[i] = PART::col(t, i) < C ? (cur.x[i] - post_mean) * post_r : 0.f;
+                float h = xh[i];
+                if constexpr (WRAP) h = gate[i] * __builtin_fmaf(h, og[i], ob[i]);
+                sv[i] = __builtin_fmaf(a.f.res_scale, cur.res[i], h);
+            }
+            // ds
+            if (a.gy) {
+                const float mean = cur.stats[2], r = cur.stats[3];
+                float m[2] = {0.f, 0.f};
 #pragma unroll
-                        for (int i = 0; i < N; ++i) h[i] *= w[i];
-                    }
-                    if (a.f.post_beta) {
-                        COLS::load((const T*)a.f.post_beta, t, C, w);
-#pragma unroll
-                        for (int i = 0; i < N; ++i) h[i] += w[i];
-                    }
-                } else {
-#pragma unroll
-                    for (int i = 0; i < N; ++i) h[i] = xh[i];
+                for (int i = 0; i < N; ++i) {
+                    sv[i] = PART::col(t, i) < C ? (sv[i] - mean) * r : 0.f;
+                    const float g = cur.gy[i];
+                    pre_g[i] = __builtin_fmaf(g, sv[i], pre_g[i]);
+                    pre_b[i] += g;
+                    d[i] = g * eg[i];
+                    m[0] += d[i];
+                    m[1] = __builtin_fmaf(d[i], sv[i], m[1]);
                 }
-                float gate[N];
-                if (a.f.gate) {
-                    COLS::load((const T*)a.f.gate + gate_row * a.f.gate_ld, t, C, gate);
+                bn_row_sum<TPR, 2>(m, lds, turn);
+                const float m0 = a.f.pre_kind == GD_NORM_LAYER ? m[0] / (float)C : 0.f, m1 = m[1] / (float)C;
 #pragma unroll
-                    for (int i = 0; i < N; ++i) sv[i] = gate[i] * h[i];
-                } else {
+                for (int i = 0; i < N; ++i) d[i] = PART::col(t, i) < C ? __builtin_fmaf(r, d[i] - m0 - sv[i] * m1, cur.gs[i]) : 0.f;
+            } else {
 #pragma unroll
-                    for (int i = 0; i < N; ++i) sv[i] = h[i];
-                }
-                if (a.f.res) {
-                    COLS::load((const T*)a.f.res + row * C, t, C, w);
+                for (int i = 0; i < N; ++i) d[i] = cur.gs[i];
+            }
+            if (a.dres) {
+                float w[N];
 #pragma unroll
-                    for (int i = 0; i < N; ++i) sv[i] = __builtin_fmaf(a.f.res_scale, w[i], sv[i]);
-                }
-                // ds
-                if (a.gy) {
-                    const float mean = a.f.stats[row * 4 + 2], r = a.f.stats[row * 4 + 3];
-                    COLS::load((const T*)a.gy + row * C, t, C, d);
-                    float m[2] = {0.f, 0.f};
-                    if (a.f.pre_gamma) {
-                        COLS::load((const T*)a.f.pre_gamma, t, C, w);
-                    } else {
+                for (int i = 0; i < N; ++i) w[i] = a.f.res_scale * d[i];
+                PART::store((T*)a.dres + row * C, t, C, w);
+            }
+            if constexpr (WRAP) {
+                float m[2] = {0.f, 0.f};
 #pragma unroll
-                        for (int i = 0; i < N; ++i) w[i] = 1.f;
-                    }
-#pragma unroll
-                    for (int i = 0; i < N; ++i) {
-                        sv[i] = COLS::col(t, i) < C ? (sv[i] - mean) * r : 0.f;
-                        acc[BN_PRE_G][i] = __builtin_fmaf(d[i], sv[i], acc[BN_PRE_G][i]);
-                        acc[BN_PRE_B][i] += d[i];
-                        d[i] *= w[i];
-                        m[0] += d[i];
-                        m[1] = __builtin_fmaf(d[i], sv[i], m[1]);
-                    }
-                    bn_row_sum<TPR, 2>(m, lds);
-                    const float m0 = a.f.pre_kind == GD_NORM_LAYER ? m[0] / (float)C : 0.f, m1 = m[1] / (float)C;
-#pragma unroll
-                    for (int i = 0; i < N; ++i) d[i] = r * (d[i] - m0 - sv[i] * m1);
-                    if (a.gs) {
-                        COLS::load((const T*)a.gs + row * C, t, C, w);
-#pragma unroll
-                        for (int i = 0; i < N; ++i) d[i] += w[i];
-                    }
-                } else {
-                    COLS::load((const T*)a.gs + row * C, t, C, d);
-                }
-                if (a.dres) {
-#pragma unroll
-                    for (int i = 0; i < N; ++i) w[i] = a.f.res_scale * d[i];
-                    COLS::store((T*)a.dres + row * C, t, C, w);
-                }
-                if (a.f.gate) {
-#pragma unroll
-                    for (int i = 0; i < N; ++i) {
-                        if (COLS::col(t, i) < C) acc_gate[i] = __builtin_fmaf(d[i], h[i], acc_gate[i]);
-                        d[i] *= gate[i];
-                    }
-                }
-                if (a.f.post_kind) {
-                    float m[2] = {0.f, 0.f};
-                    if (a.f.post_gamma) {
-                        COLS::load((const T*)a.f.post_gamma, t, C, w);
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < N; ++i) w[i] = 1.f;
-                    }
-#pragma unroll
-                    for (int i = 0; i < N; ++i) {
-                        if (COLS::col(t, i) >= C) d[i] = 0.f;
-                        acc[BN_POST_G][i] = __builtin_fmaf(d[i], xh[i], acc[BN_POST_G][i]);
-                        acc[BN_POST_B][i] += d[i];
-                        d[i] *= w[i];
+                for (int i = 0; i < N; ++i) {
+                    dgate[i] = __builtin_fmaf(d[i], __builtin_fmaf(xh[i], og[i], ob[i]), dgate[i]);
+                    d[i] *= gate[i];
+                    post_g[i] = __builtin_fmaf(d[i], xh[i], post_g[i]);
+                    post_b[i] += d[i];
+                    if (a.f.post_kind) {
+                        d[i] *= og[i];
                         m[0] += d[i];
                         m[1] = __builtin_fmaf(d[i], xh[i], m[1]);
                     }
-                    bn_row_sum<TPR, 2>(m, lds);
+                }
+                if (a.f.post_kind) {
+                    bn_row_sum<TPR, 2>(m, lds, turn);
                     const float m0 = a.f.post_kind == GD_NORM_LAYER ? m[0] / (float)C : 0.f, m1 = m[1] / (float)C;
 #pragma unroll
                     for (int i = 0; i < N; ++i) d[i] = post_r * (d[i] - m0 - xh[i] * m1);
                 }
-                if (a.dx) COLS::store((T*)a.dx + row * C, t, C, d);
             }
+            if (a.dx) PART::store((T*)a.dx + row * C, t, C, d);
         }
-        if (b.gate_sums) bn_flush<COLS, TPR, N>(acc_gate, b.gate_sums + ((long long)blockIdx.x + gate_row) * C, C, lds);
+        if constexpr (WRAP) {
+            if (b.gate_sums) bn_flush<PART, TPR, N>(dgate, b.gate_sums + ((long long)blockIdx.x + gate_row) * C, C, lds);
+        }
         g0 = g1;
     }
-#pragma unroll
-    for (int k = 0; k < BN_SUMS; ++k)
-        if (b.sums[k]) bn_flush<COLS, TPR, N>(acc[k], b.sums[k] + (long long)blockIdx.x * C, C, lds);
+    if (b.sums[BN_PRE_G]) bn_flush<PART, TPR, N>(pre_g, b.sums[BN_PRE_G] + (long long)blockIdx.x * C, C, lds);
+    if (b.sums[BN_PRE_B]) bn_flush<PART, TPR, N>(pre_b, b.sums[BN_PRE_B] + (long long)blockIdx.x * C, C, lds);
+    if constexpr (WRAP) {
+        if (b.sums[BN_POST_G]) bn_flush<PART, TPR, N>(post_g, b.sums[BN_POST_G] + (long long)blockIdx.x * C, C, lds);
+        if (b.sums[BN_POST_B]) bn_flush<PART, TPR, N>(post_b, b.sums[BN_POST_B] + (long long)blockIdx.x * C, C, lds);
+    }
 }
 
 // out[c] = sum over the slots of one sum.  blockIdx.y < BN_SUMS: a sum over all workgroups; above: the gate row blockIdx.y - BN_SUMS, which
-// workgroups floor(g per / R) .. floor((g per + per - 1) / R) have.  64 channels a workgroup, 16 slots side by side.
+// workgroups floor(g per / R) .. floor((g per + per - 1) / R) have.  16 channels a workgroup, 64 slots side by side.
 template <typename T>
 __global__ void __launch_bounds__(1024) k_block_norm_cols(const bn_bwd_args b, int workgroups) {
-    __shared__ float lds[16][65];
+    __shared__ float lds[64][17];
     const gd_block_norm_bwd_t& a = b.a;
-    const int C = a.f.C, c = blockIdx.x * 64 + (threadIdx.x & 63), lane = threadIdx.x >> 6;
+    const int C = a.f.C, c = blockIdx.x * 16 + (threadIdx.x & 15), lane = threadIdx.x >> 4;
     const float* src;
     T* out;
     long long lo = 0, hi = workgroups;
@@ -356,14 +385,16 @@ __global__ void __launch_bounds__(1024) k_block_norm_cols(const bn_bwd_args b, i
         out = (T*)a.dgate + g * C;
     }
     float s = 0.f;
-    if (c < C)
-        for (long long i = lo + lane; i < hi; i += 16) s += src[i * C + c];
-    lds[lane][threadIdx.x & 63] = s;
+    if (c < C) {
+#pragma unroll 8
+        for (long long i = lo + lane; i < hi; i += 64) s += src[i * C + c];
+    }
+    lds[lane][threadIdx.x & 15] = s;
     __syncthreads();
     if (lane == 0 && c < C) {
         s = lds[0][threadIdx.x];
-#pragma unroll
-        for (int w = 1; w < 16; ++w) s += lds[w][threadIdx.x];
+#pragma unroll 8
+        for (int w = 1; w < 64; ++w) s += lds[w][threadIdx.x];
         out[c] = to_storage<T>(s);
     }
 }
@@ -377,14 +408,14 @@ static bool bn_vec(const gd_block_norm_t& f, int elem) {
 
 #define BN_MAX_C 16384
 
-// threads a row: a wave up to 1024 channels (no barrier), then 256 up to 4096, then 1024; 8 channels a thread where they suffice
+// threads a row: a wave up to 1024 channels (no barrier), then more of them; 8 channels a thread where they suffice
 #define BN_SHAPE(C, X)                                                                                        \
     do {                                                                                                      \
         if ((C) <= 512) X(64, 8);                                                                             \
         else if ((C) <= 1024) X(64, 16);                                                                      \
         else if ((C) <= 2048) X(256, 8);                                                                      \
-        else if ((C) <= 4096) X(256, 16);                                                                     \
-        else if ((C) <= 8192) X(1024, 8);                                                                     \
+        else if ((C) <= 4096) X(512, 8);                                                                      \
+        else if ((C) <= 8192) X(512, 16);                                                                     \
         else X(1024, 16);                                                                                     \
     } while (0)
 
@@ -454,16 +485,19 @@ static void bn_launch_bwd(const gd_block_norm_bwd_t& a, float* ws, hipStream_t s
         any |= dst[k] != nullptr;
     }
     b.gate_sums = a.dgate ? ws + (size_t)BN_SUMS * wg0 * a.f.C : nullptr;
+    const bool wrap = a.f.gate || a.f.post_kind;
     const bool vec = bn_vec(a.f, sizeof(T)) && bn_aligned(a.gy) && bn_aligned(a.gs) && bn_aligned(a.dx) && bn_aligned(a.dres);
 #define BN_GO(TPR, N)                                                                                         \
     do {                                                                                                      \
-        if (vec) k_block_norm_bwd<T, TPR, N, true><<<wg, TPR < 256 ? 256 : TPR, 0, st>>>(b);                  \
-        else k_block_norm_bwd<T, TPR, N, false><<<wg, TPR < 256 ? 256 : TPR, 0, st>>>(b);                     \
+        constexpr int threads = TPR < 256 ? 256 : TPR;                                                        \
+        if (!vec) k_block_norm_bwd<T, TPR, N, false, true><<<wg, threads, 0, st>>>(b);                        \
+        else if (wrap) k_block_norm_bwd<T, TPR, N, true, true><<<wg, threads, 0, st>>>(b);                    \
+        else k_block_norm_bwd<T, TPR, N, true, false><<<wg, threads, 0, st>>>(b);                             \
     } while (0)
     BN_SHAPE(a.f.C, BN_GO);
 #undef BN_GO
     const int gates = a.dgate ? (int)(a.f.rows / a.f.rows_per_gate) : 0;
-    if (any || gates) k_block_norm_cols<T><<<dim3((a.f.C + 63) / 64, BN_SUMS + gates), 1024, 0, st>>>(b, wg);
+    if (any || gates) k_block_norm_cols<T><<<dim3((a.f.C + 15) / 16, BN_SUMS + gates), 1024, 0, st>>>(b, wg);
 }
 
 extern "C" int gd_block_norm_bwd(const gd_block_norm_bwd_t* a, void* workspace, size_t workspace_bytes, int dtype, void* stream) {

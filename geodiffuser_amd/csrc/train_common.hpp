@@ -15,3 +15,18 @@ template <typename T> __device__ __forceinline__ T to_storage(float x) {
     if constexpr (sizeof(T) == 2) asm("" : "+v"(x));
     return (T)x;
 }
+
+// Sum over the wave's 64 lanes on the VALU's cross-lane paths (DPP), the same in every lane: four steps inside rows of 16 lanes, two
+// broadcasts across them.  (A shuffle goes through LDS: six of them are ten times the latency, and a row's norm is a chain of sums.)
+template <int CTRL, int ROWS> __device__ __forceinline__ float dpp_of(float v) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, ROWS, 0xf, false));
+}
+__device__ __forceinline__ float wave_total(float v) {
+    v += dpp_of<0xB1, 0xf>(v);      // quad_perm [1, 0, 3, 2]
+    v += dpp_of<0x4E, 0xf>(v);      // quad_perm [2, 3, 0, 1]
+    v += dpp_of<0x141, 0xf>(v);     // row_half_mirror
+    v += dpp_of<0x140, 0xf>(v);     // row_mirror
+    v += dpp_of<0x142, 0xa>(v);     // row_bcast15 into rows 1 and 3 (others add 0)
+    v += dpp_of<0x143, 0xc>(v);     // row_bcast31 into rows 2 and 3
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
+}
