@@ -1111,13 +1111,13 @@ def _dt(t: torch.Tensor, name: str) -> int:
     return dt
 
 
-def _like(t: Optional[torch.Tensor], name: str, ref: torch.Tensor, shape) -> int:
-    """Address of t (0: None), which has to be contiguous, on ref's device, of its dtype and of ``shape``."""
+def _like(t: Optional[torch.Tensor], name: str, dtype, dev: int, shape) -> int:
+    """Address of t (0: None), which has to be contiguous, of ``dtype`` and ``shape``, on GPU ``dev``."""
     if t is None:
         return 0
-    _need(t, name, ref.dtype)
-    if t.shape != shape or t.device != ref.device:
-        raise _lib.GeodiffError(f"{name}: expected shape {tuple(shape)} on {ref.device}, got {tuple(t.shape)} on {t.device}")
+    if t.dtype is not dtype or t.get_device() != dev or t.shape != shape or not t.is_contiguous():
+        _need(t, name, dtype)
+        raise _lib.GeodiffError(f"{name}: expected shape {tuple(shape)} on cuda:{dev}, got {tuple(t.shape)} on {t.device}")
     return t.data_ptr()
 
 
@@ -1140,7 +1140,7 @@ def embed_tokens(ids, table, pos=None, scale: float = 1.0):
     if table.dim() != 2 or (pos is not None and (pos.dim() != 2 or pos.shape[0] < L)):
         raise _lib.GeodiffError("embed_tokens: table is [V, C], pos is [>= L, C]")
     V, C = table.shape
-    pp = 0 if pos is None else _like(pos, "pos", table, (pos.shape[0], C))
+    pp = 0 if pos is None else _like(pos, "pos", table.dtype, table.get_device(), (pos.shape[0], C))
     y = torch.empty(*shape, C, dtype=table.dtype, device=table.device)
     n = ids.numel()
     if n and C:
@@ -1196,42 +1196,42 @@ class Norm(NamedTuple):
 _NORM_KINDS = {"layer": _lib.GD_NORM_LAYER, "rms": _lib.GD_NORM_RMS}
 
 
-def _norm_args(norm: Optional[Norm], name: str, x: torch.Tensor, C: int):
-    """-> kind, address of gamma, address of beta, eps"""
-    if norm is None:
-        return 0, 0, 0, 0.0
-    kind = _NORM_KINDS.get(norm.kind)
-    if kind is None:
-        raise _lib.GeodiffError(f"block_norm: {name} norm must be 'layer' or 'rms', got {norm.kind!r}")
-    return kind, _like(norm.gamma, name + " gamma", x, (C,)), _like(norm.beta, name + " beta", x, (C,)), norm.eps
-
-
-def _block_norm_args(x, res, pre, post, gate, res_scale, s: int, y: int, stats: int):
-    """-> (gd_block_norm_t, rows, C, rows of the gate); s, y, stats: addresses."""
+def _block_norm_x(x):
+    """-> dtype code, shape, C, rows, GPU of block_norm's x"""
+    _need(x, "x")
     shape = x.shape
-    C = shape[-1]
-    rows = x.numel() // C
-    pre_kind, pre_g, pre_b, pre_eps = _norm_args(pre, "pre", x, C)
-    post_kind, post_g, post_b, post_eps = _norm_args(post, "post", x, C)
+    C = shape[-1] if shape else 0
+    if C == 0:
+        raise _lib.GeodiffError("block_norm: x is [..., C]")
+    return _dt(x, "x"), shape, C, x.numel() // C, x.get_device()
+
+
+def _block_norm_args(x, shape, C, rows, dev, res, pre, post, gate, res_scale, s: int, y: int, stats: int):
+    """-> (gd_block_norm_t, rows of the gate); s, y, stats: addresses."""
+    dtype, vec = x.dtype, (C,)
+    pre_kind = pre_g = pre_b = post_kind = post_g = post_b = 0
+    pre_eps = post_eps = 0.0
+    if pre is not None:
+        kind, gamma, beta, pre_eps = pre
+        pre_kind, pre_g, pre_b = _NORM_KINDS.get(kind), _like(gamma, "pre gamma", dtype, dev, vec), _like(beta, "pre beta", dtype, dev, vec)
+    if post is not None:
+        kind, gamma, beta, post_eps = post
+        post_kind, post_g, post_b = _NORM_KINDS.get(kind), _like(gamma, "post gamma", dtype, dev, vec), _like(beta, "post beta", dtype, dev, vec)
+    if pre_kind is None or post_kind is None:
+        raise _lib.GeodiffError("block_norm: a norm's kind must be 'layer' or 'rms'")
     gp, per, ld, gate_rows = 0, rows, C, 1
     if gate is not None:
-        per_sample = gate.dim() == 2 and x.dim() >= 2
-        if (gate.device != x.device or gate.dtype != x.dtype or gate.shape != ((shape[0], C) if per_sample else (C,)) or gate.stride(-1) != 1
-                or (per_sample and gate.shape[0] > 1 and gate.stride(0) < C)):
+        per_sample = gate.dim() == 2 and len(shape) >= 2
+        if (gate.dtype is not dtype or gate.get_device() != dev or gate.shape != ((shape[0], C) if per_sample else vec)
+                or not (gate.is_contiguous() or (per_sample and gate.stride(1) == 1 and gate.stride(0) >= C))):
             raise _lib.GeodiffError("block_norm: gate is [C] or [x.shape[0], C] of x's dtype and device, its rows contiguous")
         gp = gate.data_ptr()
         if per_sample and shape[0]:
             gate_rows, per = shape[0], rows // shape[0]
-            ld = gate.stride(0) if gate_rows > 1 else C
-    return _lib.GdBlockNorm(x.data_ptr(), _like(res, "res", x, shape), gp, post_g, post_b, pre_g, pre_b, s, y, stats, rows, per, ld, C, post_kind, pre_kind, post_eps, pre_eps,
+            if gate_rows > 1:
+                ld = gate.stride(0)
+    return _lib.GdBlockNorm(x.data_ptr(), _like(res, "res", dtype, dev, shape), gp, post_g, post_b, pre_g, pre_b, s, y, stats, rows, per, ld, C, post_kind, pre_kind, post_eps, pre_eps,
                             res_scale), gate_rows
-
-
-def _block_norm_x(x):
-    _need(x, "x")
-    if x.dim() < 1 or x.shape[-1] == 0:
-        raise _lib.GeodiffError("block_norm: x is [..., C]")
-    return _dt(x, "x")
 
 
 def block_norm(x, res, pre: Optional[Norm], post: Optional[Norm] = None, gate=None, res_scale: float = 1.0):
@@ -1243,16 +1243,16 @@ def block_norm(x, res, pre: Optional[Norm], post: Optional[Norm] = None, gate=No
     with a row for each sample (its rows may be strided); pre / post: ``Norm`` or None (pre None: y is None).  y is computed from the
     unrounded sum; stats [rows, 4] f32 is what ``block_norm_bwd`` needs."""
     lib = _lib.load()
-    dt = _block_norm_x(x)
+    dt, shape, C, rows, dev = _block_norm_x(x)
     plain = res is None and gate is None and post is None
     if plain and pre is None:
         raise _lib.GeodiffError("block_norm: nothing to compute")
     s = x if plain else torch.empty_like(x)
     y = torch.empty_like(x) if pre is not None else None
-    stats = torch.empty(x.numel() // x.shape[-1], 4, dtype=torch.float32, device=x.device)
-    a, _ = _block_norm_args(x, res, pre, post, gate, res_scale, 0 if plain else s.data_ptr(), _ip(y), stats.data_ptr())
-    if a.rows:
-        _launch(lib.gd_block_norm, "gd_block_norm", x.get_device(), ctypes.byref(a), dt)
+    stats = torch.empty(rows, 4, dtype=torch.float32, device=x.device)
+    a, _ = _block_norm_args(x, shape, C, rows, dev, res, pre, post, gate, res_scale, 0 if plain else s.data_ptr(), _ip(y), stats.data_ptr())
+    if rows:
+        _launch(lib.gd_block_norm, "gd_block_norm", dev, ctypes.byref(a), dt)
     return s, y, stats
 
 
@@ -1265,49 +1265,38 @@ def block_norm_bwd(x, res, gy, gs, stats, pre: Optional[Norm], post: Optional[No
     there.  -> {"dx", "dres", "dgate", "dpost_gamma", "dpost_beta", "dpre_gamma", "dpre_beta"}: None where the call has no such input,
     or where ``need`` (names of the ones that are wanted; default: all) leaves it out."""
     lib = _lib.load()
-    dt = _block_norm_x(x)
+    dt, shape, C, rows, dev = _block_norm_x(x)
+    dtype = x.dtype
     if gy is None and gs is None:
         raise _lib.GeodiffError("block_norm_bwd: gy or gs is needed")
     if gy is not None and pre is None:
         raise _lib.GeodiffError("block_norm_bwd: gy without the norm that made y")
     if need is not None and not set(need) <= set(_BLOCK_NORM_GRADS):
         raise _lib.GeodiffError(f"block_norm_bwd: need names {_BLOCK_NORM_GRADS}")
-    _need(stats, "stats", torch.float32)
-    shape = x.shape
-    C = shape[-1]
-    rows = x.numel() // C
-    if stats.shape != (rows, 4) or stats.device != x.device:
-        raise _lib.GeodiffError("block_norm_bwd: stats are not those of this call's forward")
-    f, gate_rows = _block_norm_args(x, res, pre, post, gate, res_scale, 0, 0, stats.data_ptr())
-    pgy, pgs = _like(gy, "gy", x, shape), _like(gs, "gs", x, shape)
-    out = dict.fromkeys(_BLOCK_NORM_GRADS)
-    want = [k for k, t in zip(_BLOCK_NORM_GRADS, (x, res, gate, post and post.gamma, post and post.beta, pre and pre.gamma, pre and pre.beta))
-            if t is not None and (need is None or k in need)]
-    rows_of = [gate_rows if k == "dgate" else 1 for k in want if k not in ("dx", "dres")]
-    for k in want[:2]:
-        if k in ("dx", "dres"):
-            out[k] = torch.empty_like(x)
-    if rows_of:
-        # the sums over rows: rows of one buffer
-        small = iter((torch.zeros if rows == 0 else torch.empty)(sum(rows_of), C, dtype=x.dtype, device=x.device).split(rows_of))
-        for k in want:
-            if k == "dgate":
-                out[k] = next(small).view(gate.shape)
-            elif k not in ("dx", "dres"):
-                out[k] = next(small)[0]
-    if rows == 0 or not want:
-        return out
-    if gy is None:
-        # nothing reaches y's norm: its parameters' gradients are zeros, and the kernel is not asked for them
-        for k in ("dpre_gamma", "dpre_beta"):
-            if out[k] is not None:
-                out[k].zero_()
-    ptr = [_ip(out[k]) if gy is not None or not k.startswith("dpre") else 0 for k in _BLOCK_NORM_GRADS]
-    nbytes = lib.gd_block_norm_bwd_workspace_bytes(rows, C, gate_rows if ptr[2] else 0) if any(ptr[2:]) else 0
+    f, gate_rows = _block_norm_args(x, shape, C, rows, dev, res, pre, post, gate, res_scale, 0, 0, _like(stats, "stats", torch.float32, dev, (rows, 4)))
+    pgy, pgs = _like(gy, "gy", dtype, dev, shape), _like(gs, "gs", dtype, dev, shape)
+    out, ptr, sums = {}, [], False
+    for k, t in (("dx", x), ("dres", res), ("dgate", gate), ("dpost_gamma", post and post[1]), ("dpost_beta", post and post[2]), ("dpre_gamma", pre and pre[1]),
+                 ("dpre_beta", pre and pre[2])):
+        if t is None or (need is not None and k not in need):
+            out[k] = None
+            ptr.append(0)
+        elif rows == 0 or (gy is None and k[:4] == "dpre"):
+            # no rows, or nothing reaches y's norm: zeros, and the kernel is not asked for them
+            out[k] = torch.zeros(t.shape, dtype=dtype, device=t.device)
+            ptr.append(0)
+        else:
+            d = out[k] = torch.empty_like(t) if k != "dgate" else torch.empty(t.shape, dtype=dtype, device=t.device)
+            ptr.append(d.data_ptr())
+            sums = sums or (k != "dx" and k != "dres")
     if not any(ptr):
         return out
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
-    _launch(lib.gd_block_norm_bwd, "gd_block_norm_bwd", x.get_device(), ctypes.byref(_lib.GdBlockNormBwd(f, pgy, pgs, *ptr)), _ip(ws), nbytes, dt)
+    nbytes, pws = 0, 0
+    if sums:
+        nbytes = lib.gd_block_norm_bwd_workspace_bytes(rows, C, gate_rows if ptr[2] else 0)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+        pws = ws.data_ptr()
+    _launch(lib.gd_block_norm_bwd, "gd_block_norm_bwd", dev, ctypes.byref(_lib.GdBlockNormBwd(f, pgy, pgs, *ptr)), pws, nbytes, dt)
     return out
 
 
