@@ -159,7 +159,8 @@ SIGNATURES = {
     "gd_embed": (c_int, [c_void_p, c_int, c_int64, c_void_p, c_int64, c_void_p, c_int, c_int, c_float, c_void_p, c_int, c_void_p]),
     "gd_embed_bwd_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int]),
     "gd_embed_bwd": (c_int, [c_void_p, c_int, c_int64, c_void_p, c_int64, c_int, c_int64, c_float, c_void_p, c_void_p, c_size_t, c_int, c_void_p]),
-    "gd_embed_pos_bwd": (c_int, [c_void_p, c_int64, c_int, c_int, c_int, c_void_p, c_int, c_void_p]),
+    "gd_embed_pos_bwd_workspace_bytes": (c_size_t, [c_int64, c_int, c_int]),
+    "gd_embed_pos_bwd": (c_int, [c_void_p, c_int64, c_int, c_int, c_int, c_void_p, c_void_p, c_size_t, c_int, c_void_p]),
     "gd_block_norm": (c_int, [POINTER(GdBlockNorm), c_int, c_void_p]),
     "gd_block_norm_bwd_workspace_bytes": (c_size_t, [c_int64, c_int, c_int64]),
     "gd_block_norm_bwd": (c_int, [POINTER(GdBlockNormBwd), c_void_p, c_size_t, c_int, c_void_p]),

@@ -160,7 +160,7 @@ __global__ void __launch_bounds__(256) k_embed_bwd_scan(const em_ids ids, int n,
 
 // ---- many positions: the positions sorted by token ---------------------------------------------------------------------------------------
 // A stable least-significant-digit radix sort of (token, position), 8 bits a pass, two launches each.  Ids that add nothing get the key
-// `vocab` and end up last.  A workgroup counts / moves EM_SORT_KEYS consecutive entries or more, each of its four waves a run of them; the
+// `vocab` and end up last.  A workgroup counts / moves EM_SORT_KEYS consecutive entries or more, each of its sixteen waves a run of them; the
 // rank among equal digits of a round of 64 is a match of the digit's bits over the wave, so that the order of equal tokens is that of their
 // positions.  The scatter's workgroups each add up the whole table of counts themselves (at most EM_SORT_BLOCKS rows of 256): a launch
 // less than a scan would need.
@@ -169,14 +169,14 @@ __global__ void __launch_bounds__(256) k_embed_bwd_scan(const em_ids ids, int n,
 
 struct em_sort {
     long long n;
-    int per_block;              // a multiple of 256
+    int per_block;              // a multiple of 1024
     int blocks;
 };
 
 static em_sort em_sort_of(long long n) {
     long long blocks = (n + EM_SORT_KEYS - 1) / EM_SORT_KEYS;
     if (blocks > EM_SORT_BLOCKS) blocks = EM_SORT_BLOCKS;
-    const long long per = ((n + blocks - 1) / blocks + 255) / 256 * 256;
+    const long long per = ((n + blocks - 1) / blocks + 1023) / 1024 * 1024;
     return em_sort{n, (int)per, (int)((n + per - 1) / per)};
 }
 
@@ -216,49 +216,61 @@ __device__ __forceinline__ void em_count(const em_keys& k, long long lo, long lo
     }
 }
 
-__global__ void __launch_bounds__(256) k_embed_sort_count(const em_keys k, const em_sort s, int shift, int* __restrict__ table, uint32_t* __restrict__ there, int there_words) {
-    __shared__ int counts[4][256];
-    const int wave = threadIdx.x >> 6;
-    for (int i = threadIdx.x; i < 4 * 256; i += 256) counts[0][i] = 0;
+__global__ void __launch_bounds__(1024) k_embed_sort_count(const em_keys k, const em_sort s, int shift, int* __restrict__ table, uint32_t* __restrict__ there, int there_words) {
+    __shared__ int counts[16][256];
+    const int tid = threadIdx.x, wave = tid >> 6;
+    for (int i = tid; i < 16 * 256; i += 1024) counts[0][i] = 0;
     // the first pass also clears the marks of the tokens that occur, for the last one
-    for (int i = blockIdx.x * 256 + threadIdx.x; i < there_words; i += gridDim.x * 256) there[i] = 0;
+    for (int i = blockIdx.x * 1024 + tid; i < there_words; i += gridDim.x * 1024) there[i] = 0;
     __syncthreads();
-    const long long run = s.per_block / 4, lo = (long long)blockIdx.x * s.per_block + wave * run, hi = lo + run < s.n ? lo + run : s.n;
+    const long long run = s.per_block / 16, lo = (long long)blockIdx.x * s.per_block + wave * run, hi = lo + run < s.n ? lo + run : s.n;
     em_count(k, lo, hi, shift, counts[wave]);
     __syncthreads();
-    table[blockIdx.x * 256 + threadIdx.x] = counts[0][threadIdx.x] + counts[1][threadIdx.x] + counts[2][threadIdx.x] + counts[3][threadIdx.x];
+    if (tid < 256) {
+        int c = 0;
+#pragma unroll
+        for (int w = 0; w < 16; ++w) c += counts[w][tid];
+        table[blockIdx.x * 256 + tid] = c;
+    }
 }
 
-__global__ void __launch_bounds__(256) k_embed_sort_move(const em_keys k, const em_sort s, int shift, const int* __restrict__ table, uint32_t* __restrict__ key_out,
-                                                         uint32_t* __restrict__ pos_out, unsigned char* __restrict__ there) {
-    __shared__ int counts[4][256], scan[256];
-    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
-    for (int i = tid; i < 4 * 256; i += 256) counts[0][i] = 0;
-    // thread = digit: how many entries of it lie in earlier workgroups, and in all
+__global__ void __launch_bounds__(1024) k_embed_sort_move(const em_keys k, const em_sort s, int shift, const int* __restrict__ table, uint32_t* __restrict__ key_out,
+                                                          uint32_t* __restrict__ pos_out, unsigned char* __restrict__ there) {
+    __shared__ int counts[16][256], part[4][2][256], scan[256];
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, d0 = tid & 255, q = tid >> 8;
+    for (int i = tid; i < 16 * 256; i += 1024) counts[0][i] = 0;
+    // how many entries of digit d0 lie in earlier workgroups, and in all: four threads share a digit
     int before = 0, all = 0;
 #pragma unroll 8
-    for (int b = 0; b < s.blocks; ++b) {
-        const int c = table[b * 256 + tid];
+    for (int b = q; b < s.blocks; b += 4) {
+        const int c = table[b * 256 + d0];
         before += b < (int)blockIdx.x ? c : 0;
         all += c;
     }
-    scan[tid] = all;
+    part[q][0][d0] = before;
+    part[q][1][d0] = all;
     __syncthreads();
-    const long long run = s.per_block / 4, lo = (long long)blockIdx.x * s.per_block + wave * run, hi = lo + run < s.n ? lo + run : s.n;
+    const long long run = s.per_block / 16, lo = (long long)blockIdx.x * s.per_block + wave * run, hi = lo + run < s.n ? lo + run : s.n;
     em_count(k, lo, hi, shift, counts[wave]);
+    before = part[0][0][d0] + part[1][0][d0] + part[2][0][d0] + part[3][0][d0];
+    all = part[0][1][d0] + part[1][1][d0] + part[2][1][d0] + part[3][1][d0];
+    if (q == 0) scan[d0] = all;
+    __syncthreads();
 #pragma unroll
     for (int o = 1; o < 256; o <<= 1) {                      // inclusive scan over the digits
-        const int v = tid >= o ? scan[tid - o] : 0;
+        const int v = q == 0 && d0 >= o ? scan[d0 - o] : 0;
         __syncthreads();
-        scan[tid] += v;
+        if (q == 0) scan[d0] += v;
         __syncthreads();
     }
-    int at = scan[tid] - all + before;                       // first place of this digit's entries of this workgroup
+    if (q == 0) {
+        int at = scan[d0] - all + before;                    // first place of this digit's entries of this workgroup
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-        const int c = counts[w][tid];
-        counts[w][tid] = at;
-        at += c;
+        for (int w = 0; w < 16; ++w) {
+            const int c = counts[w][d0];
+            counts[w][d0] = at;
+            at += c;
+        }
     }
     __syncthreads();
     volatile int* place = counts[wave];
@@ -281,9 +293,10 @@ __global__ void __launch_bounds__(256) k_embed_sort_move(const em_keys k, const 
     }
 }
 
-// Sums over the sorted entries: a wave takes `tile` of them (at most 64) and one slice of channels, and writes each token whose entries all
-// lie in its tile.  A token that goes on beyond a border of the tile leaves a partial sum: `head` if its first entry lies before the
-// tile, `tail` if it begins in it.  The workgroups behind those write the zero rows.
+// Sums over the sorted entries: a wave takes a tile of them (at most 64) and one slice of channels, and writes the tokens that begin in its
+// tile.  A token that goes on into the next tile but not beyond it is finished by the wave of the tile where it begins (the next one
+// leaves it out); one that goes on further leaves a partial sum in each of its tiles: `tail` in the first, `head` in the others.  The
+// workgroups behind those write the zero rows.
 struct em_sum {
     const uint32_t *key, *pos;
     const unsigned char* there;
@@ -292,58 +305,79 @@ struct em_sum {
     int tile, tiles, slices, C;
     unsigned vocab;
     float scale;
+
+    // tile u begins with an entry of `key` that is not its first: the token goes on into u
+    __device__ __forceinline__ bool goes_on(long long u, uint32_t k) const { return u > 0 && u < tiles && key[u * tile] == k && key[u * tile - 1] == k; }
 };
 
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) k_embed_bwd_sum(const em_sum a, const T* __restrict__ dy, T* __restrict__ dtable) {
     using COLS = em_cols<T, VEC>;
     constexpr int N = COLS::N, AHEAD = 8;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, C = a.C;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), C = a.C;
     const long long items = (long long)a.tiles * a.slices;
     const long long item_blocks = (items + 3) / 4;
     if (blockIdx.x < item_blocks) {
         const long long item = (long long)blockIdx.x * 4 + wave;
         if (item >= items) return;
         const int t = (int)(item / a.slices), sl = (int)(item % a.slices);
-        const long long e0 = (long long)t * a.tile;
-        // lane = entry: its key, its position, whether it is its token's last one
-        const bool mine = lane < a.tile && e0 + lane < a.n;
+        const long long e0 = (long long)t * a.tile, e1 = e0 + a.tile;
+        // lane = entry: its key, its position; the next tile's beside them
+        const bool mine = lane < a.tile && e0 + lane < a.n, theirs = lane < a.tile && e1 + lane < a.n;
         const uint32_t key = mine ? a.key[e0 + lane] : a.vocab, pos = mine ? a.pos[e0 + lane] : 0;
+        const uint32_t key2 = theirs ? a.key[e1 + lane] : a.vocab, pos2 = theirs ? a.pos[e1 + lane] : 0;
         const uint32_t next = mine && e0 + lane + 1 < a.n ? a.key[e0 + lane + 1] : 0xffffffffu;
-        const uint32_t prev = e0 > 0 ? a.key[e0 - 1] : 0xffffffffu;
-        const unsigned long long ends = __ballot(key != next);
+        const uint32_t first = __builtin_amdgcn_readfirstlane(key);
+        const bool from_before = a.goes_on(t, first), long_before = from_before && a.goes_on(t - 1, first);
+        const bool far = a.goes_on((long long)t + 2, key2) && lane == 0;              // the next tile's first token goes on behind it
+        unsigned long long ends = __ballot(key != next);     // entries that are their token's last
         const int live = __popcll(__ballot(key < a.vocab));  // sorted: the entries without a row of the table are the last ones
-        bool from_before = prev == (uint32_t)__builtin_amdgcn_readfirstlane((int)key);
+        if (live == 0) return;
+        const uint32_t last = __builtin_amdgcn_readlane(key, live - 1);
+        int e = 0, stop = live;
+        bool partial = false;                                // the token at the front is one of the long ones
+        if (from_before) {
+            if (!long_before && (ends & (~0ull >> (64 - live)))) e = __builtin_ctzll(ends) + 1;      // finished by the tile before: it began there and ends here
+            else partial = true;
+        }
+        const bool goes = !((ends >> (live - 1)) & 1);
+        const bool own_last = !from_before || (ends & ((1ull << (live - 1)) - 1)) != 0;      // the last token begins in this tile
+        if (goes && own_last && !__any(far && key2 == last)) {
+            // short: the next tile's entries of it are ours
+            const unsigned long long more = __ballot(theirs && key2 == last);
+            stop = live + (~more ? __builtin_ctzll(~more) : 64);
+        }
+        const auto at = [&](int k) { return (uint32_t)(k < a.tile ? __builtin_amdgcn_readlane(pos, k) : __builtin_amdgcn_readlane(pos2, k - a.tile)); };
         float acc[N] = {};
-        for (int e = 0; e < live; e += AHEAD) {
+        for (; e < stop; e += AHEAD) {
             float v[AHEAD][N];
 #pragma unroll
-            for (int j = 0; j < AHEAD; ++j) {                // (the last entry again instead of a branch between the loads)
-                const int at = e + j < live ? e + j : live - 1;
-                COLS::load(dy + (long long)(uint32_t)__builtin_amdgcn_readlane((int)pos, at) * C, sl, lane, C, v[j]);
-            }
+            for (int j = 0; j < AHEAD; ++j)                  // (the last entry again instead of a branch between the loads)
+                COLS::load(dy + (long long)at(e + j < stop ? e + j : stop - 1) * C, sl, lane, C, v[j]);
 #pragma unroll
             for (int j = 0; j < AHEAD; ++j) {
-                if (e + j >= live) break;
+                const int k = e + j;
+                if (k >= stop) break;
 #pragma unroll
                 for (int i = 0; i < N; ++i) acc[i] += v[j][i];
-                if ((ends >> (e + j)) & 1) {
-                    if (from_before) {
+                if (stop > live ? k == stop - 1 || (k < live && ((ends >> k) & 1)) : (ends >> k) & 1) {
+                    if (partial) {
 #pragma unroll
                         for (int i = 0; i < N; ++i) if (COLS::col(sl, lane, i) < C) a.head[(long long)t * C + COLS::col(sl, lane, i)] = acc[i];
                     } else {
 #pragma unroll
                         for (int i = 0; i < N; ++i) acc[i] *= a.scale;
-                        COLS::store(dtable + (long long)(uint32_t)__builtin_amdgcn_readlane((int)key, e + j) * C, sl, lane, C, acc);
+                        const uint32_t row = __builtin_amdgcn_readlane(key, k < live ? k : live - 1);
+                        COLS::store(dtable + (long long)row * C, sl, lane, C, acc);
                     }
 #pragma unroll
                     for (int i = 0; i < N; ++i) acc[i] = 0.f;
-                    from_before = false;
+                    partial = false;
                 }
             }
         }
-        if (live > 0 && !((ends >> (live - 1)) & 1)) {
-            float* part = from_before ? a.head : a.tail;
+        if (goes && stop == live) {
+            float* part = partial ? a.head : a.tail;
 #pragma unroll
             for (int i = 0; i < N; ++i) if (COLS::col(sl, lane, i) < C) part[(long long)t * C + COLS::col(sl, lane, i)] = acc[i];
         }
@@ -356,54 +390,51 @@ __global__ void __launch_bounds__(256) k_embed_bwd_sum(const em_sum a, const T* 
             for (int sl = 0; sl < a.slices; ++sl) COLS::store(dtable + (v0 + r) * C, sl, lane, C, zero);
 }
 
-// The tokens whose entries go over a tile's border: the tail of the tile where they begin + the heads of the tiles that they go on into.
-// Most go over one border: the first workgroups each look at one tile's end and take up to EM_LONG - 1 heads, 1024 channels wide.
-// A token with more (padding has half of all tiles) is the work of the workgroups behind them, 16 channels and 64 tiles side by side: among
-// EM_LONG tiles in a row one has a multiple of EM_LONG as its number, and the first such tile's workgroups do it.
+// The tokens that go on for two tiles and more: the tail of the tile where they begin + the heads of the others.  Up to EM_LONG - 1 heads:
+// a workgroup for each tile and 1024 channels, the heads one after another.
 #define EM_LONG 64
 
-// tile u begins with an entry of `key` and so ends tile u - 1
-__device__ __forceinline__ bool em_goes_on(const em_sum& a, long long u, uint32_t key) {
-    return u > 0 && u < a.tiles && a.key[u * a.tile] == key && a.key[u * a.tile - 1] == key;
-}
-
 template <typename T>
-__global__ void __launch_bounds__(1024) k_embed_bwd_join(const em_sum a, int wide, T* __restrict__ dtable) {
-    __shared__ float lds[64][17];
-    const int tid = threadIdx.x, lane = tid & 63, C = a.C;
-    if ((int)blockIdx.x < a.tiles * wide) {
-        const int t = blockIdx.x / wide, c = (blockIdx.x % wide) * 1024 + tid;
-        if (t + 1 >= a.tiles) return;
-        const uint32_t key = a.key[(long long)(t + 1) * a.tile];
-        if (key >= a.vocab || !em_goes_on(a, t + 1, key) || (a.key[(long long)t * a.tile] == key && em_goes_on(a, t, key))) return;
-        const unsigned long long on = __ballot(em_goes_on(a, (long long)t + 1 + lane, key));
-        if (~on == 0) return;
-        const int more = __builtin_ctzll(~on);
+__global__ void __launch_bounds__(256) k_embed_bwd_join(const em_sum a, T* __restrict__ dtable) {
+    const int t = blockIdx.x, lane = threadIdx.x & 63, C = a.C;
+    const uint32_t key = a.key[(long long)(t + 1) * a.tile];                    // (the last tile has no workgroup)
+    if (key >= a.vocab || !a.goes_on(t + 1, key) || !a.goes_on(t + 2, key) || a.goes_on(t, key)) return;
+    const unsigned long long on = __ballot(a.goes_on((long long)t + 1 + lane, key));
+    if (~on == 0) return;
+    const int more = __builtin_ctzll(~on);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const int c = blockIdx.y * 1024 + k * 256 + threadIdx.x;
         if (c >= C) return;
         float s = a.tail[(long long)t * C + c];
 #pragma unroll 8
         for (int u = 1; u <= more; ++u) s += a.head[(long long)(t + u) * C + c];
         dtable[(long long)key * C + c] = to_storage<T>(s * a.scale);
-        return;
     }
-    const int groups = (C + 15) / 16, b = blockIdx.x - a.tiles * wide;
-    const long long q = (long long)(b / groups + 1) * EM_LONG;
-    if (q >= a.tiles) return;
+}
+
+// EM_LONG heads and more (padding has half of all tiles): 16 channels and 64 tiles side by side a workgroup.  Among EM_LONG tiles in a row one
+// has a multiple of EM_LONG as its number, and the workgroups of the first such tile do the work.
+template <typename T>
+__global__ void __launch_bounds__(1024) k_embed_bwd_join_long(const em_sum a, T* __restrict__ dtable) {
+    __shared__ float lds[64][17];
+    const int tid = threadIdx.x, lane = tid & 63, C = a.C;
+    const long long q = (long long)(blockIdx.x + 1) * EM_LONG;
     const uint32_t key = a.key[q * a.tile];
     if (key >= a.vocab) return;
-    const unsigned long long back = __ballot(em_goes_on(a, q - lane, key));      // every wave of the workgroup finds the same
+    const unsigned long long back = __ballot(a.goes_on(q - lane, key));         // every wave of the workgroup finds the same
     if (!(back & 1)) return;
     const int c0 = ~back ? __builtin_ctzll(~back) : EM_LONG;
-    if (c0 == EM_LONG && em_goes_on(a, q - EM_LONG, key)) return;               // an earlier multiple of EM_LONG has it
+    if (c0 == EM_LONG && a.goes_on(q - EM_LONG, key)) return;                   // an earlier multiple of EM_LONG has it
     const long long t = q - c0;
     long long more = 0;
     for (long long u = t + 1;; u += 1024) {
-        const int n = __syncthreads_count(em_goes_on(a, u + tid, key));
+        const int n = __syncthreads_count(a.goes_on(u + tid, key));
         more += n;
         if (n < 1024) break;
     }
     if (more < EM_LONG) return;
-    const int part = tid >> 4, c = (b % groups) * 16 + (tid & 15);
+    const int part = tid >> 4, c = blockIdx.y * 16 + (tid & 15);
     float s = 0.f;
     if (c < C) {
 #pragma unroll 8
@@ -419,25 +450,57 @@ __global__ void __launch_bounds__(1024) k_embed_bwd_join(const em_sum a, int wid
     }
 }
 
-// dP: one workgroup a (position row, slice); the four waves share the sequences
+// dP is the column sum of dy as a [B, L * C] matrix.  A thread has one word (16 bytes; VEC) or element of a row and adds EM_POS_ROWS sequences
+// or more of it; the workgroups of one column lie blockIdx.y apart and leave their sums in `part` [gridDim.y, L * C], where there is
+// more than one.
+#define EM_POS_ROWS 64
+
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(256) k_embed_pos_bwd(const T* __restrict__ dy, long long B, int L, int C, T* __restrict__ dpos) {
-    using COLS = em_cols<T, VEC>;
-    constexpr int N = COLS::N;
-    __shared__ float lds[4][64 * N];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = blockIdx.x, sl = blockIdx.y;
+__global__ void __launch_bounds__(256) k_embed_pos_bwd(const T* __restrict__ dy, long long B, long long width, long long out_width, long long per, float* __restrict__ part,
+                                                       T* __restrict__ dpos) {
+    constexpr int N = VEC ? word16<T>::N : 1;
+    const long long at = ((long long)blockIdx.x * 256 + threadIdx.x) * N;
+    if (at >= out_width) return;
     float acc[N] = {};
-    if (l < L) {
-#pragma unroll 4
-        for (long long b = wave; b < B; b += 4) {
-            float v[N];
-            COLS::load(dy + (b * L + l) * C, sl, lane, C, v);
+    if (at < width) {
+        const long long b0 = (long long)blockIdx.y * per, b1 = b0 + per < B ? b0 + per : B;
+        const T* p = dy + b0 * width + at;
+#pragma unroll 8
+        for (long long b = b0; b < b1; ++b, p += width) {
+            if constexpr (VEC) {
+                const word16<T> w = *(const word16<T>*)p;
 #pragma unroll
-            for (int i = 0; i < N; ++i) acc[i] += v[i];
+                for (int i = 0; i < N; ++i) acc[i] += (float)w.v[i];
+            } else {
+                acc[0] += (float)p[0];
+            }
         }
     }
-    em_fold<N>(acc, lds, wave, lane);
-    if (wave == 0) COLS::store(dpos + (long long)l * C, sl, lane, C, acc);
+    if (part) {
+        if (at < width) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) part[(long long)blockIdx.y * width + at + i] = acc[i];
+        }
+    } else if constexpr (VEC) {
+        word16<T> w;
+#pragma unroll
+        for (int i = 0; i < N; ++i) w.v[i] = to_storage<T>(acc[i]);
+        *(word16<T>*)(dpos + at) = w;
+    } else {
+        dpos[at] = to_storage<T>(acc[0]);
+    }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) k_embed_pos_join(const float* __restrict__ part, int parts, long long width, long long out_width, T* __restrict__ dpos) {
+    const long long at = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (at >= out_width) return;
+    float s = 0.f;
+    if (at < width) {
+#pragma unroll 8
+        for (int k = 0; k < parts; ++k) s += part[k * width + at];
+    }
+    dpos[at] = to_storage<T>(s);
 }
 
 static bool em_vec(int C, int elem, const void* a, const void* b, const void* c = nullptr) {
@@ -527,40 +590,73 @@ extern "C" int gd_embed_bwd(const void* ids, int ids64, int64_t n, const void* d
         EM_LAUNCH(dtype, vec, (k_embed_bwd_scan<T, VEC><<<(unsigned)grid, 256, 0, st>>>(in, (int)n, (const T*)dy, (int)vocab, C, padding, scale, (T*)dtable)));
     } else {
         const long long grid = ((long long)p.tiles * slices + 3) / 4 + zeros;
-        GD_REQUIRE(grid < (1ll << 31) && (long long)p.tiles * ((C + 1023) / 1024 + 1) + (long long)(p.tiles / EM_LONG) * ((C + 15) / 16) < (1ll << 31), GD_EUNSUPPORTED,
-                   "gd_embed_bwd: too many positions for this width");
+        GD_REQUIRE(grid < (1ll << 31) && (C + 15) / 16 <= 65535, GD_EUNSUPPORTED, "gd_embed_bwd: too many positions for this width");
         char* const ws = (char*)workspace;
         em_keys k = {in, nullptr, nullptr, (unsigned)vocab, padding};
         for (int i = 0; i < p.passes; ++i) {
             const bool last = i + 1 == p.passes;
             uint32_t *const key = (uint32_t*)(ws + p.key[i & 1]), *const pos = (uint32_t*)(ws + p.pos[i & 1]);
-            k_embed_sort_count<<<p.sort.blocks, 256, 0, st>>>(k, p.sort, 8 * i, (int*)(ws + p.table), (uint32_t*)(ws + p.there), i == 0 ? (int)((vocab + 3) / 4) : 0);
-            k_embed_sort_move<<<p.sort.blocks, 256, 0, st>>>(k, p.sort, 8 * i, (const int*)(ws + p.table), key, pos, last ? (unsigned char*)(ws + p.there) : nullptr);
+            k_embed_sort_count<<<p.sort.blocks, 1024, 0, st>>>(k, p.sort, 8 * i, (int*)(ws + p.table), (uint32_t*)(ws + p.there), i == 0 ? (int)((vocab + 3) / 4) : 0);
+            k_embed_sort_move<<<p.sort.blocks, 1024, 0, st>>>(k, p.sort, 8 * i, (const int*)(ws + p.table), key, pos, last ? (unsigned char*)(ws + p.there) : nullptr);
             k.key = key;
             k.pos = pos;
         }
         const em_sum a = {k.key, k.pos, (const unsigned char*)(ws + p.there), (float*)(ws + p.head), (float*)(ws + p.tail), n, p.tile, p.tiles, slices, C, (unsigned)vocab, scale};
         EM_LAUNCH(dtype, vec, (k_embed_bwd_sum<T, VEC><<<(unsigned)grid, 256, 0, st>>>(a, (const T*)dy, (T*)dtable)));
-        const int wide = (C + 1023) / 1024;
-        const unsigned joins = (unsigned)((long long)p.tiles * wide + (long long)((p.tiles - 1) / EM_LONG) * ((C + 15) / 16));
-        if (p.tiles > 1) {
-            if (dtype == GD_F32) k_embed_bwd_join<float><<<joins, 1024, 0, st>>>(a, wide, (float*)dtable);
-            else if (dtype == GD_F16) k_embed_bwd_join<f16_t><<<joins, 1024, 0, st>>>(a, wide, (f16_t*)dtable);
-            else k_embed_bwd_join<bf16_t><<<joins, 1024, 0, st>>>(a, wide, (bf16_t*)dtable);
+        if (p.tiles > 2) {
+            const dim3 joins(p.tiles - 1, (C + 1023) / 1024);
+            if (dtype == GD_F32) k_embed_bwd_join<float><<<joins, 256, 0, st>>>(a, (float*)dtable);
+            else if (dtype == GD_F16) k_embed_bwd_join<f16_t><<<joins, 256, 0, st>>>(a, (f16_t*)dtable);
+            else k_embed_bwd_join<bf16_t><<<joins, 256, 0, st>>>(a, (bf16_t*)dtable);
+        }
+        if (p.tiles > EM_LONG) {
+            const dim3 joins((p.tiles - 1) / EM_LONG, (C + 15) / 16);
+            if (dtype == GD_F32) k_embed_bwd_join_long<float><<<joins, 1024, 0, st>>>(a, (float*)dtable);
+            else if (dtype == GD_F16) k_embed_bwd_join_long<f16_t><<<joins, 1024, 0, st>>>(a, (f16_t*)dtable);
+            else k_embed_bwd_join_long<bf16_t><<<joins, 1024, 0, st>>>(a, (bf16_t*)dtable);
         }
     }
     GD_CHECK_LAUNCH("gd_embed_bwd");
     return GD_OK;
 }
 
-extern "C" int gd_embed_pos_bwd(const void* dy, int64_t B, int L, int C, int pos_rows, void* dpos, int dtype, void* stream) {
-    const int rc = em_check(B * (L > 0 ? L : 0), 1, C, dtype, "gd_embed_pos_bwd");
+// sequences a workgroup adds, and how many workgroups share a column: as many as give each EM_POS_ROWS, at most 32 (every further one is
+// another row of sums to write and read)
+static int em_pos_parts(long long B, long long* per) {
+    long long parts = B / EM_POS_ROWS;
+    parts = parts < 1 ? 1 : parts > 32 ? 32 : parts;
+    *per = (B + parts - 1) / parts;
+    return *per > 0 ? (int)((B + *per - 1) / *per) : 1;
+}
+
+extern "C" size_t gd_embed_pos_bwd_workspace_bytes(int64_t B, int L, int C) {
+    long long per;
+    if (B < 0 || L <= 0 || C <= 0) return 0;
+    const int parts = em_pos_parts(B, &per);
+    return parts > 1 ? sizeof(float) * (size_t)parts * L * C : 0;
+}
+
+extern "C" int gd_embed_pos_bwd(const void* dy, int64_t B, int L, int C, int pos_rows, void* dpos, void* workspace, size_t workspace_bytes, int dtype, void* stream) {
+    GD_REQUIRE(dpos && B >= 0 && L >= 0 && pos_rows >= L && pos_rows > 0 && (B == 0 || L == 0 || dy), GD_EINVAL, "gd_embed_pos_bwd: bad argument");
+    const int rc = em_check(0, 1, C, dtype, "gd_embed_pos_bwd");
     if (rc != GD_OK) return rc;
-    GD_REQUIRE(dpos && B >= 0 && L >= 0 && pos_rows >= L && pos_rows > 0 && (B * L == 0 || dy), GD_EINVAL, "gd_embed_pos_bwd: bad argument");
-    const bool vec = em_vec(C, EM_ELEM(dtype), dy, dpos);
-    const int slice = vec ? 64 * (16 / EM_ELEM(dtype)) : 512;
+    const size_t need = gd_embed_pos_bwd_workspace_bytes(B, L, C);
+    GD_REQUIRE(!need || (workspace && workspace_bytes >= need), GD_EWORKSPACE, "gd_embed_pos_bwd: workspace of %zu bytes needed", need);
+    long long per;
+    const int parts = em_pos_parts(B, &per);
+    const long long width = (long long)L * C, out_width = (long long)pos_rows * C;
+    const bool vec = width * EM_ELEM(dtype) % 16 == 0 && out_width * EM_ELEM(dtype) % 16 == 0 && (((uintptr_t)dy | (uintptr_t)dpos) & 15) == 0;
+    const long long words = (out_width + (vec ? 16 / EM_ELEM(dtype) : 1) - 1) / (vec ? 16 / EM_ELEM(dtype) : 1), grid = (words + 255) / 256;
+    GD_REQUIRE((out_width + 255) / 256 < (1ll << 31), GD_EUNSUPPORTED, "gd_embed_pos_bwd: too many positions for this width");
+    float* const part = parts > 1 ? (float*)workspace : nullptr;
     hipStream_t st = as_stream(stream);
-    EM_LAUNCH(dtype, vec, (k_embed_pos_bwd<T, VEC><<<dim3((unsigned)pos_rows, (C + slice - 1) / slice), 256, 0, st>>>((const T*)dy, B, L, C, (T*)dpos)));
+    EM_LAUNCH(dtype, vec, (k_embed_pos_bwd<T, VEC><<<dim3((unsigned)grid, parts), 256, 0, st>>>((const T*)dy, B, width, out_width, per, part, (T*)dpos)));
+    if (parts > 1) {
+        const unsigned g = (unsigned)((out_width + 255) / 256);
+        if (dtype == GD_F32) k_embed_pos_join<float><<<g, 256, 0, st>>>(part, parts, width, out_width, (float*)dpos);
+        else if (dtype == GD_F16) k_embed_pos_join<f16_t><<<g, 256, 0, st>>>(part, parts, width, out_width, (f16_t*)dpos);
+        else k_embed_pos_join<bf16_t><<<g, 256, 0, st>>>(part, parts, width, out_width, (bf16_t*)dpos);
+    }
     GD_CHECK_LAUNCH("gd_embed_pos_bwd");
     return GD_OK;
 }

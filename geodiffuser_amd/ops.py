@@ -1181,7 +1181,10 @@ def embed_positions_bwd(dy, pos_rows: int):
     L, C = dy.shape[-2:]
     d = torch.empty(pos_rows, C, dtype=dy.dtype, device=dy.device)
     if pos_rows and C:
-        _launch(lib.gd_embed_pos_bwd, "gd_embed_pos_bwd", dy.get_device(), dy.data_ptr(), dy.numel() // (L * C) if L else 0, L, C, pos_rows, d.data_ptr(), dt)
+        B = dy.numel() // (L * C) if L else 0
+        nbytes = lib.gd_embed_pos_bwd_workspace_bytes(B, L, C)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dy.device) if nbytes else None
+        _launch(lib.gd_embed_pos_bwd, "gd_embed_pos_bwd", dy.get_device(), dy.data_ptr(), B, L, C, pos_rows, d.data_ptr(), _ip(ws), nbytes, dt)
     return d
 
 

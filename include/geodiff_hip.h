@@ -551,7 +551,8 @@ size_t gd_embed_bwd_workspace_bytes(int64_t n, int64_t vocab, int C);
 int gd_embed_bwd(const void* ids, int ids64, int64_t n, const void* dy, int64_t vocab, int C, int64_t padding, float scale, void* dtable,
                  void* workspace, size_t workspace_bytes, int dtype, void* stream);
 /* dpos[l] = sum over b of dy[b, l], dy [B, L, C]; rows L .. pos_rows - 1 become zeros. */
-int gd_embed_pos_bwd(const void* dy, int64_t B, int L, int C, int pos_rows, void* dpos, int dtype, void* stream);
+size_t gd_embed_pos_bwd_workspace_bytes(int64_t B, int L, int C);
+int gd_embed_pos_bwd(const void* dy, int64_t B, int L, int C, int pos_rows, void* dpos, void* workspace, size_t workspace_bytes, int dtype, void* stream);
 
 /* h = post(x);  s = res_scale * res + gate * h;  y = pre(s) for rows of C <= 16384 channels.
  *   kinds: GD_NORM_NONE, GD_NORM_LAYER (xh = (v - mean) / sqrt(var + eps)), GD_NORM_RMS (xh = v / sqrt(mean v^2 + eps)), then

@@ -130,6 +130,22 @@ def test_embedding_gradient(ops, dtype, n, V, C, kind):
 
 
 @gpu
+@pytest.mark.parametrize("n", [1030, 9000, 70000, 140000, 300000])
+@pytest.mark.parametrize("seed", range(4))
+def test_embedding_gradient_of_every_run_length(ops, n, seed):
+    """Tokens that occur just as often as fills, ends at, goes one over a tile of 8 .. 64 sorted entries, two tiles, many."""
+    g = _gen(seed)
+    lengths = [1, 2, 7, 8, 9, 15, 16, 17, 24, 31, 32, 33, 48, 63, 64, 65, 127, 128, 129, 192, 193, 257, 1025, 5000]
+    counts = []
+    while sum(counts) < n:
+        counts.append(lengths[int(torch.randint(0, len(lengths) if seed else 12, (1,), generator=g))])
+    counts[-1] -= sum(counts) - n
+    ids = torch.repeat_interleave(torch.arange(len(counts)) * 2, torch.tensor(counts))[torch.randperm(n, generator=g)].to(DEV)
+    _check_embed_bwd(ops, ids, _randn(g, n, 24), 2 * len(counts))
+    _check_embed_bwd(ops, ids, _randn(g, n, 9, dtype=torch.bfloat16), 2 * len(counts), padding_idx=2 * len(counts) - 2)
+
+
+@gpu
 @pytest.mark.parametrize("n", [6, 300, 9000])
 def test_embedding_gradient_skips_padding_and_foreign_ids(ops, n):
     g = _gen(n)
