@@ -384,11 +384,7 @@ __global__ void __launch_bounds__(1024) k_block_norm_cols(const bn_bwd_args b, i
         src = b.gate_sums + g * C;
         out = (T*)a.dgate + g * C;
     }
-    float s = 0.f;
-    if (c < C) {
-#pragma unroll 8
-        for (long long i = lo + lane; i < hi; i += 64) s += src[i * C + c];
-    }
+    float s = c < C ? sum_strided(src + c, C, (int)lo + lane, (int)hi, 64) : 0.f;
     lds[lane][threadIdx.x & 15] = s;
     __syncthreads();
     if (lane == 0 && c < C) {

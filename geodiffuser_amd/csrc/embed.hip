@@ -126,12 +126,14 @@ __global__ void __launch_bounds__(256) k_embed_bwd_scan(const em_ids ids, int n,
             }
             if (mine) list[at + __popcll(mask & ((1ull << lane) - 1))] = j;
             __syncthreads();
-#pragma unroll 4
-            for (int m = wave; m < total; m += 4) {
-                float v[N];
-                COLS::load(dy + (long long)list[m] * C, sl, lane, C, v);
+            for (int m = wave; m < total; m += 16) {         // (behind the last: the first again, adding nothing)
+                float v[4][N];
 #pragma unroll
-                for (int i = 0; i < N; ++i) acc[i] += v[i];
+                for (int j = 0; j < 4; ++j) COLS::load(dy + (long long)list[m + 4 * j < total ? m + 4 * j : m] * C, sl, lane, C, v[j]);
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+#pragma unroll
+                    for (int i = 0; i < N; ++i) acc[i] += m + 4 * j < total ? v[j][i] : 0.f;
             }
             __syncthreads();
         }
@@ -305,9 +307,6 @@ struct em_sum {
     int tile, tiles, slices, C;
     unsigned vocab;
     float scale;
-
-    // tile u begins with an entry of `key` that is not its first: the token goes on into u
-    __device__ __forceinline__ bool goes_on(long long u, uint32_t k) const { return u > 0 && u < tiles && key[u * tile] == k && key[u * tile - 1] == k; }
 };
 
 template <typename T, bool VEC>
@@ -327,9 +326,11 @@ __global__ void __launch_bounds__(256) k_embed_bwd_sum(const em_sum a, const T* 
         const uint32_t key = mine ? a.key[e0 + lane] : a.vocab, pos = mine ? a.pos[e0 + lane] : 0;
         const uint32_t key2 = theirs ? a.key[e1 + lane] : a.vocab, pos2 = theirs ? a.pos[e1 + lane] : 0;
         const uint32_t next = mine && e0 + lane + 1 < a.n ? a.key[e0 + lane + 1] : 0xffffffffu;
+        // (the entries are sorted: two equal ones have only equal ones between them)
+        const uint32_t prev = e0 > 0 ? a.key[e0 - 1] : 0xffffffffu, before = e0 > a.tile ? a.key[e0 - a.tile - 1] : 0xffffffffu;
+        const uint32_t behind = e1 + a.tile < a.n ? a.key[e1 + a.tile] : 0xffffffffu;
         const uint32_t first = __builtin_amdgcn_readfirstlane(key);
-        const bool from_before = a.goes_on(t, first), long_before = from_before && a.goes_on(t - 1, first);
-        const bool far = a.goes_on((long long)t + 2, key2) && lane == 0;              // the next tile's first token goes on behind it
+        const bool from_before = prev == first, long_before = before == first;
         unsigned long long ends = __ballot(key != next);     // entries that are their token's last
         const int live = __popcll(__ballot(key < a.vocab));  // sorted: the entries without a row of the table are the last ones
         if (live == 0) return;
@@ -342,7 +343,7 @@ __global__ void __launch_bounds__(256) k_embed_bwd_sum(const em_sum a, const T* 
         }
         const bool goes = !((ends >> (live - 1)) & 1);
         const bool own_last = !from_before || (ends & ((1ull << (live - 1)) - 1)) != 0;      // the last token begins in this tile
-        if (goes && own_last && !__any(far && key2 == last)) {
+        if (goes && own_last && behind != last) {
             // short: the next tile's entries of it are ours
             const unsigned long long more = __ballot(theirs && key2 == last);
             stop = live + (~more ? __builtin_ctzll(~more) : 64);
@@ -397,20 +398,36 @@ __global__ void __launch_bounds__(256) k_embed_bwd_sum(const em_sum a, const T* 
 template <typename T>
 __global__ void __launch_bounds__(256) k_embed_bwd_join(const em_sum a, T* __restrict__ dtable) {
     const int t = blockIdx.x, lane = threadIdx.x & 63, C = a.C;
-    const uint32_t key = a.key[(long long)(t + 1) * a.tile];                    // (the last tile has no workgroup)
-    if (key >= a.vocab || !a.goes_on(t + 1, key) || !a.goes_on(t + 2, key) || a.goes_on(t, key)) return;
-    const unsigned long long on = __ballot(a.goes_on((long long)t + 1 + lane, key));
+    const long long e1 = (long long)(t + 1) * a.tile;                           // (the last two tiles have no workgroup)
+    const uint32_t key = a.key[e1], in_tile = a.key[e1 - 1], behind = a.key[e1 + a.tile], before = t > 0 ? a.key[(long long)t * a.tile - 1] : 0xffffffffu;
+    if (key >= a.vocab || in_tile != key || behind != key || before == key) return;
+    const long long u = (long long)t + 1 + lane;
+    const unsigned long long on = __ballot(u < a.tiles && a.key[u * a.tile] == key);
     if (~on == 0) return;
     const int more = __builtin_ctzll(~on);
+    const int c0 = blockIdx.y * 1024 + threadIdx.x;
+    float s[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        const int c = blockIdx.y * 1024 + k * 256 + threadIdx.x;
-        if (c >= C) return;
-        float s = a.tail[(long long)t * C + c];
-#pragma unroll 8
-        for (int u = 1; u <= more; ++u) s += a.head[(long long)(t + u) * C + c];
-        dtable[(long long)key * C + c] = to_storage<T>(s * a.scale);
+    for (int i = 0; i < 4; ++i) {
+        const int c = c0 + 256 * i < C ? c0 + 256 * i : C - 1;
+        s[i] = a.tail[(long long)t * C + c];
     }
+    for (int k = 1; k <= more; k += 4) {                     // (what lies behind the last head reads it again and adds nothing)
+        float v[4][4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float* p = a.head + (long long)(t + (k + j <= more ? k + j : more)) * C;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[j][i] = p[c0 + 256 * i < C ? c0 + 256 * i : C - 1];
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[i] += k + j <= more ? v[j][i] : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (c0 + 256 * i < C) dtable[(long long)key * C + c0 + 256 * i] = to_storage<T>(s[i] * a.scale);
 }
 
 // EM_LONG heads and more (padding has half of all tiles): 16 channels and 64 tiles side by side a workgroup.  Among EM_LONG tiles in a row one
@@ -420,26 +437,29 @@ __global__ void __launch_bounds__(1024) k_embed_bwd_join_long(const em_sum a, T*
     __shared__ float lds[64][17];
     const int tid = threadIdx.x, lane = tid & 63, C = a.C;
     const long long q = (long long)(blockIdx.x + 1) * EM_LONG;
-    const uint32_t key = a.key[q * a.tile];
-    if (key >= a.vocab) return;
-    const unsigned long long back = __ballot(a.goes_on(q - lane, key));         // every wave of the workgroup finds the same
-    if (!(back & 1)) return;
-    const int c0 = ~back ? __builtin_ctzll(~back) : EM_LONG;
-    if (c0 == EM_LONG && a.goes_on(q - EM_LONG, key)) return;                   // an earlier multiple of EM_LONG has it
-    const long long t = q - c0;
-    long long more = 0;
-    for (long long u = t + 1;; u += 1024) {
-        const int n = __syncthreads_count(a.goes_on(u + tid, key));
-        more += n;
-        if (n < 1024) break;
+    const uint32_t key = a.key[q * a.tile], before = a.key[q * a.tile - 1];
+    // whether tile q - lane begins inside the run (not with its first entry); the same in every wave
+    const long long e = (q - lane) * a.tile;
+    const bool inside = a.key[e] == key && a.key[e - 1] == key;
+    const bool earlier = q > EM_LONG && a.key[(q - EM_LONG) * a.tile - 1] == key;
+    if (key >= a.vocab || before != key || earlier) return;                     // (earlier: the multiple of EM_LONG before this one has it)
+    const unsigned long long back = __ballot(inside);
+    const long long t = q - (~back ? __builtin_ctzll(~back) : EM_LONG);         // the tile where the run begins
+    // its tiles: every step-th one of those that are left, then those behind the last that belongs to it
+    const long long left = a.tiles - (t + 1), step = (left + 1023) / 1024;
+    const long long seen = __syncthreads_count(tid * step < left && a.key[(t + 1 + tid * step) * a.tile] == key);
+    long long more = (seen - 1) * step;
+    for (long long o = more; o < more + step; o += 1024) {
+        const int n = __syncthreads_count(o + tid < left && o + tid < more + step && a.key[(t + 1 + o + tid) * a.tile] == key);
+        if (n < 1024 || o + 1024 >= more + step) {
+            more = o + n;
+            break;
+        }
     }
     if (more < EM_LONG) return;
     const int part = tid >> 4, c = blockIdx.y * 16 + (tid & 15);
     float s = 0.f;
-    if (c < C) {
-#pragma unroll 8
-        for (long long u = part; u < more; u += 64) s += a.head[(t + 1 + u) * C + c];
-    }
+    if (c < C) s = sum_strided(a.head + (t + 1) * C + c, C, part, (int)more, 64);
     lds[part][tid & 15] = s;
     __syncthreads();
     if (part == 0 && c < C) {
@@ -455,6 +475,8 @@ __global__ void __launch_bounds__(1024) k_embed_bwd_join_long(const em_sum a, T*
 // more than one.
 #define EM_POS_ROWS 64
 
+template <typename T, int N> struct alignas(N * sizeof(T)) em_piece { T v[N]; };
+
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) k_embed_pos_bwd(const T* __restrict__ dy, long long B, long long width, long long out_width, long long per, float* __restrict__ part,
                                                        T* __restrict__ dpos) {
@@ -464,16 +486,15 @@ __global__ void __launch_bounds__(256) k_embed_pos_bwd(const T* __restrict__ dy,
     float acc[N] = {};
     if (at < width) {
         const long long b0 = (long long)blockIdx.y * per, b1 = b0 + per < B ? b0 + per : B;
-        const T* p = dy + b0 * width + at;
-#pragma unroll 8
-        for (long long b = b0; b < b1; ++b, p += width) {
-            if constexpr (VEC) {
-                const word16<T> w = *(const word16<T>*)p;
+        const T* p = dy + at;
+        for (long long b = b0; b < b1; b += 8) {
+            em_piece<T, N> w[8];
 #pragma unroll
-                for (int i = 0; i < N; ++i) acc[i] += (float)w.v[i];
-            } else {
-                acc[0] += (float)p[0];
-            }
+            for (int j = 0; j < 8; ++j) w[j] = *(const em_piece<T, N>*)(p + (b + j < b1 ? b + j : b0) * width);
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+#pragma unroll
+                for (int i = 0; i < N; ++i) acc[i] += b + j < b1 ? (float)w[j].v[i] : 0.f;
         }
     }
     if (part) {
@@ -495,12 +516,7 @@ template <typename T>
 __global__ void __launch_bounds__(256) k_embed_pos_join(const float* __restrict__ part, int parts, long long width, long long out_width, T* __restrict__ dpos) {
     const long long at = (long long)blockIdx.x * 256 + threadIdx.x;
     if (at >= out_width) return;
-    float s = 0.f;
-    if (at < width) {
-#pragma unroll 8
-        for (int k = 0; k < parts; ++k) s += part[k * width + at];
-    }
-    dpos[at] = to_storage<T>(s);
+    dpos[at] = to_storage<T>(at < width ? sum_strided(part + at, width, 0, parts, 1) : 0.f);
 }
 
 static bool em_vec(int C, int elem, const void* a, const void* b, const void* c = nullptr) {
@@ -604,7 +620,7 @@ extern "C" int gd_embed_bwd(const void* ids, int ids64, int64_t n, const void* d
         const em_sum a = {k.key, k.pos, (const unsigned char*)(ws + p.there), (float*)(ws + p.head), (float*)(ws + p.tail), n, p.tile, p.tiles, slices, C, (unsigned)vocab, scale};
         EM_LAUNCH(dtype, vec, (k_embed_bwd_sum<T, VEC><<<(unsigned)grid, 256, 0, st>>>(a, (const T*)dy, (T*)dtable)));
         if (p.tiles > 2) {
-            const dim3 joins(p.tiles - 1, (C + 1023) / 1024);
+            const dim3 joins(p.tiles - 2, (C + 1023) / 1024);
             if (dtype == GD_F32) k_embed_bwd_join<float><<<joins, 256, 0, st>>>(a, (float*)dtable);
             else if (dtype == GD_F16) k_embed_bwd_join<f16_t><<<joins, 256, 0, st>>>(a, (f16_t*)dtable);
             else k_embed_bwd_join<bf16_t><<<joins, 256, 0, st>>>(a, (bf16_t*)dtable);

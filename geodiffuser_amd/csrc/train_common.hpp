@@ -30,3 +30,17 @@ __device__ __forceinline__ float wave_total(float v) {
     v += dpp_of<0x143, 0xc>(v);     // row_bcast31 into rows 2 and 3
     return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
 }
+
+// p[first * pitch] + p[(first + step) * pitch] + ... up to (not with) index `end`, in that order, eight loads at a time.  The indices of the
+// last round that lie behind the end read the first one again: a loop for the rest would wait for each of its loads.
+__device__ __forceinline__ float sum_strided(const float* __restrict__ p, long long pitch, int first, int end, int step) {
+    float s = 0.f;
+    for (int k = first; k < end; k += 8 * step) {
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = p[(long long)(k + j * step < end ? k + j * step : first) * pitch];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s += k + j * step < end ? v[j] : 0.f;
+    }
+    return s;
+}
