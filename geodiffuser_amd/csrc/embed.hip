@@ -391,83 +391,77 @@ __global__ void __launch_bounds__(256) k_embed_bwd_sum(const em_sum a, const T* 
             for (int sl = 0; sl < a.slices; ++sl) COLS::store(dtable + (v0 + r) * C, sl, lane, C, zero);
 }
 
-// The tokens that go on for two tiles and more: the tail of the tile where they begin + the heads of the others.  Up to EM_LONG - 1 heads:
-// a workgroup for each tile and 1024 channels, the heads one after another.
-#define EM_LONG 64
+// The tokens that go on for two tiles and more: the tail of the tile where they begin + the heads of the others (padding has half of all
+// tiles).  Tiles form groups of EM_GROUP.  The first launch finishes the tokens whose tiles lie in one group; of the others it adds up, group
+// by group, the heads from the group's first tile on (into that tile's head), and the tail and heads of the group where they begin (into the
+// tail).  The second launch adds those, one for each group.  All rows are read whole: a CU has a bounded number of cache lines on their way.
+#define EM_GROUP 64
+
+// rows [lo, hi) of `rows`, channel c: 16 at a time (behind the last: the first again, adding nothing)
+__device__ __forceinline__ float em_rows(const float* __restrict__ rows, long long lo, long long hi, long long step, int C, int c) {
+    float s = 0.f;
+    for (long long k = lo; k < hi; k += 16 * step) {
+        float v[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) v[j] = rows[(k + j * step < hi ? k + j * step : lo) * C + c];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) s += k + j * step < hi ? v[j] : 0.f;
+    }
+    return s;
+}
+
+// whether the run of `key` has begun before tile u and goes on into it (the entries are sorted; u in range)
+__device__ __forceinline__ bool em_into(const em_sum& a, long long u, uint32_t key) { return u > 0 && a.key[u * a.tile - 1] == key && a.key[u * a.tile] == key; }
 
 template <typename T>
 __global__ void __launch_bounds__(256) k_embed_bwd_join(const em_sum a, T* __restrict__ dtable) {
-    const int t = blockIdx.x, lane = threadIdx.x & 63, C = a.C;
-    const long long e1 = (long long)(t + 1) * a.tile;                           // (the last two tiles have no workgroup)
-    const uint32_t key = a.key[e1], in_tile = a.key[e1 - 1], behind = a.key[e1 + a.tile], before = t > 0 ? a.key[(long long)t * a.tile - 1] : 0xffffffffu;
-    if (key >= a.vocab || in_tile != key || behind != key || before == key) return;
-    const long long u = (long long)t + 1 + lane;
-    const unsigned long long on = __ballot(u < a.tiles && a.key[u * a.tile] == key);
-    if (~on == 0) return;
-    const int more = __builtin_ctzll(~on);
-    const int c0 = blockIdx.y * 1024 + threadIdx.x;
-    float s[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int c = c0 + 256 * i < C ? c0 + 256 * i : C - 1;
-        s[i] = a.tail[(long long)t * C + c];
+    const int lane = threadIdx.x & 63, C = a.C;
+    const int wide = (C + 255) / 256, groups = a.tiles > EM_GROUP ? (a.tiles + EM_GROUP - 1) / EM_GROUP : 0;
+    if ((int)blockIdx.x >= groups * wide) {
+        const int t = blockIdx.x - groups * wide;            // (a run of three tiles begins in front of the last two)
+        const long long e1 = (long long)(t + 1) * a.tile, q = (t / EM_GROUP + 1) * EM_GROUP;
+        const uint32_t key = a.key[e1], in_tile = a.key[e1 - 1], behind = a.key[e1 + a.tile], before = t > 0 ? a.key[(long long)t * a.tile - 1] : 0xffffffffu;
+        const bool crosses = q < a.tiles && a.key[q * a.tile] == key;
+        if (key >= a.vocab || in_tile != key || behind != key || before == key || crosses) return;
+        const long long u = (long long)t + 1 + lane;
+        const int more = __builtin_ctzll(~__ballot(u < a.tiles && u < q && a.key[u * a.tile] == key));
+        for (int c = threadIdx.x; c < C; c += 256)
+            dtable[(long long)key * C + c] = to_storage<T>((a.tail[(long long)t * C + c] + em_rows(a.head, t + 1, t + 1 + more, 1, C, c)) * a.scale);
+        return;
     }
-    for (int k = 1; k <= more; k += 4) {                     // (what lies behind the last head reads it again and adds nothing)
-        float v[4][4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float* p = a.head + (long long)(t + (k + j <= more ? k + j : more)) * C;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[j][i] = p[c0 + 256 * i < C ? c0 + 256 * i : C - 1];
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) s[i] += k + j <= more ? v[j][i] : 0.f;
+    const int c = blockIdx.x / groups * 256 + threadIdx.x;
+    const long long q = (long long)(blockIdx.x % groups) * EM_GROUP, q2 = q + EM_GROUP, u = q + lane;
+    const uint32_t key = a.key[q * a.tile];
+    if (q > 0 && key < a.vocab && a.key[q * a.tile - 1] == key) {
+        const unsigned long long on = __ballot(u < a.tiles && a.key[u * a.tile] == key);
+        const int m = ~on ? __builtin_ctzll(~on) : 64;
+        if (m > 1 && c < C) a.head[q * C + c] = em_rows(a.head, q, q + m, 1, C, c);
     }
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-        if (c0 + 256 * i < C) dtable[(long long)key * C + c0 + 256 * i] = to_storage<T>(s[i] * a.scale);
+    if (q2 >= a.tiles) return;
+    const uint32_t key2 = a.key[q2 * a.tile];
+    if (key2 >= a.vocab || a.key[q2 * a.tile - 1] != key2 || (q > 0 && a.key[q * a.tile - 1] == key2)) return;
+    const int m = __popcll(__ballot(em_into(a, u, key2)));  // the group's last m tiles (not its first: the run begins behind that one's start)
+    if (m > 0 && c < C) a.tail[(q2 - 1 - m) * C + c] += em_rows(a.head, q2 - m, q2, 1, C, c);
 }
 
-// EM_LONG heads and more (padding has half of all tiles): 16 channels and 64 tiles side by side a workgroup.  Among EM_LONG tiles in a row one
-// has a multiple of EM_LONG as its number, and the workgroups of the first such tile do the work.
 template <typename T>
-__global__ void __launch_bounds__(1024) k_embed_bwd_join_long(const em_sum a, T* __restrict__ dtable) {
-    __shared__ float lds[64][17];
-    const int tid = threadIdx.x, lane = tid & 63, C = a.C;
-    const long long q = (long long)(blockIdx.x + 1) * EM_LONG;
-    const uint32_t key = a.key[q * a.tile], before = a.key[q * a.tile - 1];
-    // whether tile q - lane begins inside the run (not with its first entry); the same in every wave
-    const long long e = (q - lane) * a.tile;
-    const bool inside = a.key[e] == key && a.key[e - 1] == key;
-    const bool earlier = q > EM_LONG && a.key[(q - EM_LONG) * a.tile - 1] == key;
-    if (key >= a.vocab || before != key || earlier) return;                     // (earlier: the multiple of EM_LONG before this one has it)
-    const unsigned long long back = __ballot(inside);
-    const long long t = q - (~back ? __builtin_ctzll(~back) : EM_LONG);         // the tile where the run begins
-    // its tiles: every step-th one of those that are left, then those behind the last that belongs to it
-    const long long left = a.tiles - (t + 1), step = (left + 1023) / 1024;
-    const long long seen = __syncthreads_count(tid * step < left && a.key[(t + 1 + tid * step) * a.tile] == key);
-    long long more = (seen - 1) * step;
-    for (long long o = more; o < more + step; o += 1024) {
-        const int n = __syncthreads_count(o + tid < left && o + tid < more + step && a.key[(t + 1 + o + tid) * a.tile] == key);
-        if (n < 1024 || o + 1024 >= more + step) {
-            more = o + n;
+__global__ void __launch_bounds__(256) k_embed_bwd_join_groups(const em_sum a, T* __restrict__ dtable) {
+    const int lane = threadIdx.x & 63, C = a.C, c = blockIdx.y * 256 + threadIdx.x;
+    const long long q = (long long)(blockIdx.x + 1) * EM_GROUP, g = q - EM_GROUP;
+    const uint32_t key = a.key[q * a.tile], behind = q + 1 < a.tiles ? a.key[(q + 1) * a.tile] : 0xffffffffu;
+    if (key >= a.vocab || a.key[q * a.tile - 1] != key || (g > 0 && a.key[g * a.tile - 1] == key)) return;
+    const int m = __popcll(__ballot(em_into(a, g + lane, key)));
+    if (m == 0 && behind != key) return;                     // two tiles: finished by the wave of the first one
+    long long groups = 0;
+    for (;; groups += 64) {
+        const long long u = q + (groups + lane) * EM_GROUP;
+        const unsigned long long on = __ballot(u < a.tiles && a.key[u * a.tile] == key);
+        if (~on) {
+            groups += __builtin_ctzll(~on);
             break;
         }
     }
-    if (more < EM_LONG) return;
-    const int part = tid >> 4, c = blockIdx.y * 16 + (tid & 15);
-    float s = 0.f;
-    if (c < C) s = sum_strided(a.head + (t + 1) * C + c, C, part, (int)more, 64);
-    lds[part][tid & 15] = s;
-    __syncthreads();
-    if (part == 0 && c < C) {
-        s = a.tail[t * C + c];
-#pragma unroll 8
-        for (int w = 0; w < 64; ++w) s += lds[w][tid];
-        dtable[(long long)key * C + c] = to_storage<T>(s * a.scale);
-    }
+    if (c < C) dtable[(long long)key * C + c] = to_storage<T>((a.tail[(q - 1 - m) * C + c] + em_rows(a.head, q, q + groups * EM_GROUP, EM_GROUP, C, c)) * a.scale);
 }
 
 // dP is the column sum of dy as a [B, L * C] matrix.  A thread has one word (16 bytes; VEC) or element of a row and adds EM_POS_ROWS sequences
@@ -606,7 +600,7 @@ extern "C" int gd_embed_bwd(const void* ids, int ids64, int64_t n, const void* d
         EM_LAUNCH(dtype, vec, (k_embed_bwd_scan<T, VEC><<<(unsigned)grid, 256, 0, st>>>(in, (int)n, (const T*)dy, (int)vocab, C, padding, scale, (T*)dtable)));
     } else {
         const long long grid = ((long long)p.tiles * slices + 3) / 4 + zeros;
-        GD_REQUIRE(grid < (1ll << 31) && (C + 15) / 16 <= 65535, GD_EUNSUPPORTED, "gd_embed_bwd: too many positions for this width");
+        GD_REQUIRE(grid < (1ll << 31) && (long long)p.tiles * ((C + 255) / 256) < (1ll << 30), GD_EUNSUPPORTED, "gd_embed_bwd: too many positions for this width");
         char* const ws = (char*)workspace;
         em_keys k = {in, nullptr, nullptr, (unsigned)vocab, padding};
         for (int i = 0; i < p.passes; ++i) {
@@ -619,17 +613,18 @@ extern "C" int gd_embed_bwd(const void* ids, int ids64, int64_t n, const void* d
         }
         const em_sum a = {k.key, k.pos, (const unsigned char*)(ws + p.there), (float*)(ws + p.head), (float*)(ws + p.tail), n, p.tile, p.tiles, slices, C, (unsigned)vocab, scale};
         EM_LAUNCH(dtype, vec, (k_embed_bwd_sum<T, VEC><<<(unsigned)grid, 256, 0, st>>>(a, (const T*)dy, (T*)dtable)));
+        const unsigned wide = (unsigned)((C + 255) / 256), groups = (unsigned)((p.tiles + EM_GROUP - 1) / EM_GROUP);
         if (p.tiles > 2) {
-            const dim3 joins(p.tiles - 2, (C + 1023) / 1024);
+            const unsigned joins = (p.tiles - 2) + (groups > 1 ? groups * wide : 0);
             if (dtype == GD_F32) k_embed_bwd_join<float><<<joins, 256, 0, st>>>(a, (float*)dtable);
             else if (dtype == GD_F16) k_embed_bwd_join<f16_t><<<joins, 256, 0, st>>>(a, (f16_t*)dtable);
             else k_embed_bwd_join<bf16_t><<<joins, 256, 0, st>>>(a, (bf16_t*)dtable);
         }
-        if (p.tiles > EM_LONG) {
-            const dim3 joins((p.tiles - 1) / EM_LONG, (C + 15) / 16);
-            if (dtype == GD_F32) k_embed_bwd_join_long<float><<<joins, 1024, 0, st>>>(a, (float*)dtable);
-            else if (dtype == GD_F16) k_embed_bwd_join_long<f16_t><<<joins, 1024, 0, st>>>(a, (f16_t*)dtable);
-            else k_embed_bwd_join_long<bf16_t><<<joins, 1024, 0, st>>>(a, (bf16_t*)dtable);
+        if (groups > 1) {
+            const dim3 joins(groups - 1, wide);
+            if (dtype == GD_F32) k_embed_bwd_join_groups<float><<<joins, 256, 0, st>>>(a, (float*)dtable);
+            else if (dtype == GD_F16) k_embed_bwd_join_groups<f16_t><<<joins, 256, 0, st>>>(a, (f16_t*)dtable);
+            else k_embed_bwd_join_groups<bf16_t><<<joins, 256, 0, st>>>(a, (bf16_t*)dtable);
         }
     }
     GD_CHECK_LAUNCH("gd_embed_bwd");
