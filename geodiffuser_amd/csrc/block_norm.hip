@@ -70,7 +70,7 @@ template <typename T, int TPR, int N, bool VEC> struct bn_part {
             return (float)__builtin_bit_cast(T, (unsigned short)(i & 1 ? two >> 16 : two & 0xffffu));
         }
     }
-    static __device__ __forceinline__ void store(T* __restrict__ p, int t, int C, const float* v) {
+    static __device__ __forceinline__ void store(T* p, int t, int C, const float* v, bool stream) {
 #pragma unroll
         for (int i = 0; i < N; i += W) {
             const int c = col(t, i);
@@ -79,7 +79,7 @@ template <typename T, int TPR, int N, bool VEC> struct bn_part {
                     word16<T> a;
 #pragma unroll
                     for (int j = 0; j < W; ++j) a.v[j] = to_storage<T>(v[i + j]);
-                    *(word16<T>*)(p + c) = a;
+                    store16(p + c, a, stream);
                 } else {
                     p[c] = to_storage<T>(v[i]);
                 }
@@ -136,7 +136,7 @@ __device__ __forceinline__ void bn_stats(const float* v, int t, int C, int kind,
 }
 
 template <typename T, int TPR, int N, bool VEC>
-__global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) k_block_norm(const gd_block_norm_t a) {
+__global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) k_block_norm(const gd_block_norm_t a, bool stream) {
     using PART = bn_part<T, TPR, N, VEC>;
     constexpr int RPB = TPR < 256 ? 256 / TPR : 1;           // rows a workgroup
     __shared__ float lds[64];
@@ -179,7 +179,7 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) k_block_norm(const gd_b
 #pragma unroll
         for (int i = 0; i < N; ++i) h[i] = __builtin_fmaf(a.res_scale, res[i], h[i]);
     }
-    if (a.s) PART::store((T*)a.s + row * C, t, C, h);
+    if (a.s) PART::store((T*)a.s + row * C, t, C, h, stream);
     if (!a.pre_kind) return;
     float mean, r;
     bn_stats<PART, TPR, N>(h, t, C, a.pre_kind, a.pre_eps, lds, turn, mean, r);
@@ -194,7 +194,7 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) k_block_norm(const gd_b
 #pragma unroll
         for (int i = 0; i < N; ++i) h[i] += eb[i];
     }
-    PART::store((T*)a.y + row * C, t, C, h);
+    PART::store((T*)a.y + row * C, t, C, h, stream);
 }
 
 // ---- backward -------------------------------------------------------------------------------------------------------------------------
@@ -209,6 +209,7 @@ struct bn_bwd_args {
     float* sums[BN_SUMS];       // [workgroups, C] or null
     float* gate_sums;           // [workgroups + gate rows - 1, C] or null
     long long rows_per_wg;
+    bool stream;
 };
 
 // column sums of the workgroup's rows-in-parallel, then to the workspace (threads of the first row)
@@ -324,7 +325,7 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) k_block_norm_bwd(const 
                 float w[N];
 #pragma unroll
                 for (int i = 0; i < N; ++i) w[i] = a.f.res_scale * d[i];
-                PART::store((T*)a.dres + row * C, t, C, w);
+                PART::store((T*)a.dres + row * C, t, C, w, b.stream);
             }
             if constexpr (WRAP) {
                 float m[2] = {0.f, 0.f};
@@ -347,7 +348,7 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) k_block_norm_bwd(const 
                     for (int i = 0; i < N; ++i) d[i] = post_r * (d[i] - m0 - xh[i] * m1);
                 }
             }
-            if (a.dx) PART::store((T*)a.dx + row * C, t, C, d);
+            if (a.dx) PART::store((T*)a.dx + row * C, t, C, d, b.stream);
         }
         if constexpr (WRAP) {
             if (b.gate_sums) bn_flush<PART, TPR, N>(dgate, b.gate_sums + ((long long)blockIdx.x + gate_row) * C, C, lds);
@@ -430,13 +431,13 @@ static int bn_check(const gd_block_norm_t* f, int dtype, const char* who) {
 
 template <typename T>
 static void bn_launch(const gd_block_norm_t& a, hipStream_t st) {
-    const bool vec = bn_vec(a, sizeof(T));
+    const bool vec = bn_vec(a, sizeof(T)), stream = streams_past_cache((double)a.rows * a.C * sizeof(T) * (1 + !!a.res + !!a.s + !!a.y));
 #define BN_GO(TPR, N)                                                                                         \
     do {                                                                                                      \
         constexpr int rpb = TPR < 256 ? 256 / TPR : 1;                                                        \
         const unsigned grid = (unsigned)((a.rows + rpb - 1) / rpb);                                           \
-        if (vec) k_block_norm<T, TPR, N, true><<<grid, rpb * TPR, 0, st>>>(a);                                \
-        else k_block_norm<T, TPR, N, false><<<grid, rpb * TPR, 0, st>>>(a);                                   \
+        if (vec) k_block_norm<T, TPR, N, true><<<grid, rpb * TPR, 0, st>>>(a, stream);                                \
+        else k_block_norm<T, TPR, N, false><<<grid, rpb * TPR, 0, st>>>(a, stream);                                   \
     } while (0)
     BN_SHAPE(a.C, BN_GO);
 #undef BN_GO
@@ -471,6 +472,7 @@ template <typename T>
 static void bn_launch_bwd(const gd_block_norm_bwd_t& a, float* ws, hipStream_t st) {
     bn_bwd_args b;
     b.a = a;
+    b.stream = streams_past_cache((double)a.f.rows * a.f.C * sizeof(T) * (1 + !!a.f.res + !!a.gy + !!a.gs + !!a.dx + !!a.dres));
     const long long wg0 = bn_workgroups(a.f.rows);
     b.rows_per_wg = (a.f.rows + wg0 - 1) / wg0;
     const int wg = (int)((a.f.rows + b.rows_per_wg - 1) / b.rows_per_wg);

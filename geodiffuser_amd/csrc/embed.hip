@@ -29,13 +29,13 @@ struct em_cols {
             }
         }
     }
-    static __device__ __forceinline__ void store(T* __restrict__ p, int slice, int lane, int C, const float* v) {
+    static __device__ __forceinline__ void store(T* p, int slice, int lane, int C, const float* v, bool stream) {
         if constexpr (VEC) {
             const int c = col(slice, lane, 0);
             word16<T> a;
 #pragma unroll
             for (int i = 0; i < N; ++i) a.v[i] = to_storage<T>(v[i]);
-            if (c < C) *(word16<T>*)(p + c) = a;
+            if (c < C) store16(p + c, a, stream);
         } else {
 #pragma unroll
             for (int i = 0; i < N; ++i) {
@@ -55,7 +55,7 @@ struct em_ids {
 // one wave a row; an id outside the table gives a row of NaN (there is no such row, and no way to raise from here)
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) k_embed(const em_ids ids, long long n, const T* __restrict__ table, const T* __restrict__ pos, int L, int V, int C,
-                                               float scale, T* __restrict__ y) {
+                                               float scale, bool stream, T* __restrict__ y) {
     using COLS = em_cols<T, VEC>;
     const int lane = threadIdx.x & 63;
     const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -72,7 +72,7 @@ __global__ void __launch_bounds__(256) k_embed(const em_ids ids, long long n, co
         for (int i = 0; i < COLS::N; ++i) {
             v[i] = in ? __builtin_fmaf(scale, v[i], q[i]) : __builtin_nanf("");
         }
-        COLS::store(y + row * C, sl, lane, C, v);
+        COLS::store(y + row * C, sl, lane, C, v, stream);
     }
 }
 
@@ -96,7 +96,7 @@ __device__ __forceinline__ void em_fold(float* v, float (*lds)[64 * N], int wave
 // The workgroups behind them: EM_ZERO_ROWS rows of the table each, zeros where no position has the row's token.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) k_embed_bwd_scan(const em_ids ids, int n, const T* __restrict__ dy, int V, int C, long long padding, float scale,
-                                                        T* __restrict__ dtable) {
+                                                        bool stream, T* __restrict__ dtable) {
     using COLS = em_cols<T, VEC>;
     constexpr int N = COLS::N;
     __shared__ float lds[4][64 * N];
@@ -141,7 +141,7 @@ __global__ void __launch_bounds__(256) k_embed_bwd_scan(const em_ids ids, int n,
         if (wave == 0) {
 #pragma unroll
             for (int i = 0; i < N; ++i) acc[i] *= scale;
-            COLS::store(dtable + id * C, sl, lane, C, acc);
+            COLS::store(dtable + id * C, sl, lane, C, acc, stream);
         }
         return;
     }
@@ -157,7 +157,7 @@ __global__ void __launch_bounds__(256) k_embed_bwd_scan(const em_ids ids, int n,
     const float zero[N] = {};
     for (int r = wave; r < EM_ZERO_ROWS; r += 4)
         if (v0 + r < V && !there[r])
-            for (int sl = 0; sl < slices; ++sl) COLS::store(dtable + (v0 + r) * C, sl, lane, C, zero);
+            for (int sl = 0; sl < slices; ++sl) COLS::store(dtable + (v0 + r) * C, sl, lane, C, zero, stream);
 }
 
 // ---- many positions: the positions sorted by token ---------------------------------------------------------------------------------------
@@ -307,6 +307,7 @@ struct em_sum {
     int tile, tiles, slices, C;
     unsigned vocab;
     float scale;
+    bool stream;
 };
 
 template <typename T, bool VEC>
@@ -369,7 +370,7 @@ __global__ void __launch_bounds__(256) k_embed_bwd_sum(const em_sum a, const T* 
 #pragma unroll
                         for (int i = 0; i < N; ++i) acc[i] *= a.scale;
                         const uint32_t row = __builtin_amdgcn_readlane(key, k < live ? k : live - 1);
-                        COLS::store(dtable + (long long)row * C, sl, lane, C, acc);
+                        COLS::store(dtable + (long long)row * C, sl, lane, C, acc, a.stream);
                     }
 #pragma unroll
                     for (int i = 0; i < N; ++i) acc[i] = 0.f;
@@ -388,7 +389,7 @@ __global__ void __launch_bounds__(256) k_embed_bwd_sum(const em_sum a, const T* 
     const long long v0 = ((long long)blockIdx.x - item_blocks) * EM_ZERO_ROWS;
     for (int r = wave; r < EM_ZERO_ROWS; r += 4)
         if (v0 + r < a.vocab && !a.there[v0 + r])
-            for (int sl = 0; sl < a.slices; ++sl) COLS::store(dtable + (v0 + r) * C, sl, lane, C, zero);
+            for (int sl = 0; sl < a.slices; ++sl) COLS::store(dtable + (v0 + r) * C, sl, lane, C, zero, a.stream);
 }
 
 // The tokens that go on for two tiles and more: the tail of the tile where they begin + the heads of the others (padding has half of all
@@ -543,7 +544,8 @@ extern "C" int gd_embed(const void* ids, int ids64, int64_t n, const void* table
     GD_REQUIRE(!pos || L > 0, GD_EINVAL, "gd_embed: position rows need the sequence length");
     const bool vec = em_vec(C, EM_ELEM(dtype), table, y, pos);
     hipStream_t st = as_stream(stream);
-    EM_LAUNCH(dtype, vec, (k_embed<T, VEC><<<(unsigned)((n + 3) / 4), 256, 0, st>>>(em_ids{ids, ids64}, n, (const T*)table, (const T*)pos, L, (int)vocab, C, scale, (T*)y)));
+    EM_LAUNCH(dtype, vec, (k_embed<T, VEC><<<(unsigned)((n + 3) / 4), 256, 0, st>>>(em_ids{ids, ids64}, n, (const T*)table, (const T*)pos, L, (int)vocab, C, scale,
+                      streams_past_cache((double)EM_ELEM(dtype) * C * ((double)n + (n < vocab ? n : vocab))), (T*)y)));
     GD_CHECK_LAUNCH("gd_embed");
     return GD_OK;
 }
@@ -590,6 +592,7 @@ extern "C" int gd_embed_bwd(const void* ids, int ids64, int64_t n, const void* d
     const bool vec = em_vec(C, EM_ELEM(dtype), dy, dtable);
     const int slice = vec ? 64 * (16 / EM_ELEM(dtype)) : 512, slices = (C + slice - 1) / slice;
     const long long zeros = (vocab + EM_ZERO_ROWS - 1) / EM_ZERO_ROWS;
+    const bool past = streams_past_cache((double)EM_ELEM(dtype) * C * ((double)n + vocab));
     const em_plan p = em_plan_of(n, vocab, C);
     GD_REQUIRE(!p.bytes || (workspace && workspace_bytes >= p.bytes && ((uintptr_t)workspace & 15) == 0), GD_EWORKSPACE, "gd_embed_bwd: workspace of %zu bytes needed", p.bytes);
     hipStream_t st = as_stream(stream);
@@ -597,7 +600,7 @@ extern "C" int gd_embed_bwd(const void* ids, int ids64, int64_t n, const void* d
     if (!p.bytes) {
         const long long grid = n * slices + zeros;
         GD_REQUIRE(grid < (1ll << 31), GD_EUNSUPPORTED, "gd_embed_bwd: table too large");
-        EM_LAUNCH(dtype, vec, (k_embed_bwd_scan<T, VEC><<<(unsigned)grid, 256, 0, st>>>(in, (int)n, (const T*)dy, (int)vocab, C, padding, scale, (T*)dtable)));
+        EM_LAUNCH(dtype, vec, (k_embed_bwd_scan<T, VEC><<<(unsigned)grid, 256, 0, st>>>(in, (int)n, (const T*)dy, (int)vocab, C, padding, scale, past, (T*)dtable)));
     } else {
         const long long grid = ((long long)p.tiles * slices + 3) / 4 + zeros;
         GD_REQUIRE(grid < (1ll << 31) && (long long)p.tiles * ((C + 255) / 256) < (1ll << 30), GD_EUNSUPPORTED, "gd_embed_bwd: too many positions for this width");
@@ -611,7 +614,7 @@ extern "C" int gd_embed_bwd(const void* ids, int ids64, int64_t n, const void* d
             k.key = key;
             k.pos = pos;
         }
-        const em_sum a = {k.key, k.pos, (const unsigned char*)(ws + p.there), (float*)(ws + p.head), (float*)(ws + p.tail), n, p.tile, p.tiles, slices, C, (unsigned)vocab, scale};
+        const em_sum a = {k.key, k.pos, (const unsigned char*)(ws + p.there), (float*)(ws + p.head), (float*)(ws + p.tail), n, p.tile, p.tiles, slices, C, (unsigned)vocab, scale, past};
         EM_LAUNCH(dtype, vec, (k_embed_bwd_sum<T, VEC><<<(unsigned)grid, 256, 0, st>>>(a, (const T*)dy, (T*)dtable)));
         const unsigned wide = (unsigned)((C + 255) / 256), groups = (unsigned)((p.tiles + EM_GROUP - 1) / EM_GROUP);
         if (p.tiles > 2) {

@@ -99,16 +99,16 @@ __device__ __forceinline__ double gc_norm_chunk(const void* src, long long n, in
 }
 
 template <typename T>
-__device__ __forceinline__ void gc_scale_chunk(const void* src, void* dst, long long n, int chunk, float f) {
+__device__ __forceinline__ void gc_scale_chunk(const void* src, void* dst, long long n, int chunk, float f, bool stream) {
     const T* p = (const T*)src;
     T* q = (T*)dst;
     if (((uintptr_t)src & 15) == ((uintptr_t)dst & 15)) {
         gc_range<T>(n, chunk, gc_head<T>(src),
             [&](long long i) {
-                word16<T> x = *(const word16<T>*)(p + i);
+                word16<T> x = __builtin_bit_cast(word16<T>, __builtin_nontemporal_load((const u32x4*)(p + i)));      // the last use
 #pragma unroll
                 for (int j = 0; j < word16<T>::N; ++j) x.v[j] = to_storage<T>((float)x.v[j] * f);
-                *(word16<T>*)(q + i) = x;
+                store16(q + i, x, stream);
             },
             [&](long long i) { q[i] = to_storage<T>((float)p[i] * f); });
     } else {                                                // source and destination never share a boundary: element by element
@@ -130,13 +130,13 @@ __device__ __forceinline__ double gc_norm_table(const gc_table& t, double acc) {
     return acc;
 }
 
-__device__ __forceinline__ void gc_scale_table(const gc_table& t, float f) {
-    for (int c = blockIdx.x; c < t.start[t.count]; c += gridDim.x) {
+__device__ __forceinline__ void gc_scale_table(const gc_table& t, float f, bool stream) {
+    for (int c = t.start[t.count] - 1 - (int)blockIdx.x; c >= 0; c -= gridDim.x) {
         const int k = gc_find(t, c), local = c - t.start[k];
         if (f == 1.0f && t.dst[k] == t.src[k]) continue;    // g * 1 is g: nothing to write in place
-        if (t.dtype[k] == GD_F32) gc_scale_chunk<float>(t.src[k], t.dst[k], t.n[k], local, f);
-        else if (t.dtype[k] == GD_F16) gc_scale_chunk<f16_t>(t.src[k], t.dst[k], t.n[k], local, f);
-        else gc_scale_chunk<bf16_t>(t.src[k], t.dst[k], t.n[k], local, f);
+        if (t.dtype[k] == GD_F32) gc_scale_chunk<float>(t.src[k], t.dst[k], t.n[k], local, f, stream);
+        else if (t.dtype[k] == GD_F16) gc_scale_chunk<f16_t>(t.src[k], t.dst[k], t.n[k], local, f, stream);
+        else gc_scale_chunk<bf16_t>(t.src[k], t.dst[k], t.n[k], local, f, stream);
     }
 }
 
@@ -170,11 +170,11 @@ __global__ void __launch_bounds__(256) k_grad_norm_total(const double* __restric
 }
 
 template <bool INF>
-__global__ void __launch_bounds__(256) k_grad_clip(const gc_table t, const double* __restrict__ part, int parts, float max_norm, float* __restrict__ norm) {
+__global__ void __launch_bounds__(256) k_grad_clip(const gc_table t, const double* __restrict__ part, int parts, float max_norm, bool stream, float* __restrict__ norm) {
     __shared__ double lds[4];
     const double v = gc_total<INF>(part, parts, lds);
     if (blockIdx.x == 0 && threadIdx.x == 0) norm[0] = (float)v;
-    gc_scale_table(t, gc_factor(v, max_norm));
+    gc_scale_table(t, gc_factor(v, max_norm), stream);
 }
 
 // tensors [at, ..) into one launch's table; -> how many were taken.  Tensors of no elements take a place but no chunk.
@@ -201,6 +201,8 @@ static int gc_launch(const void* const* src, void* const* dst, const int64_t* n,
                      hipStream_t st) {
     gc_table t;
     int parts = 0;
+    double bytes = 0;
+    for (int i = 0; i < count; ++i) bytes += (double)n[i] * (dtype[i] == GD_F32 ? 4 : 2) * (dst && dst[i] != src[i] ? 2 : 1);
     for (int at = 0; at < count || at == 0; at += GC_TENSORS) {
         gc_fill(t, src, dst, n, dtype, at, count);
         // one table: as many workgroups as it has chunks; several: all of them, since every launch adds to the first one's partials
@@ -211,10 +213,11 @@ static int gc_launch(const void* const* src, void* const* dst, const int64_t* n,
     if (!dst) {
         k_grad_norm_total<INF><<<1, 256, 0, st>>>(part, parts, norm);
     } else {
-        for (int at = 0; at < count || at == 0; at += GC_TENSORS) {
+        // backwards: what the norm read last is still in the memory-side cache
+        for (int at = (count > 0 ? (count - 1) / GC_TENSORS : 0) * GC_TENSORS; at >= 0; at -= GC_TENSORS) {
             if (count > GC_TENSORS) gc_fill(t, src, dst, n, dtype, at, count);
             const int chunks = t.start[t.count];
-            k_grad_clip<INF><<<chunks < 1 ? 1 : chunks < GC_GRID ? chunks : GC_GRID, 256, 0, st>>>(t, part, parts, max_norm, norm);
+            k_grad_clip<INF><<<chunks < 1 ? 1 : chunks < GC_GRID ? chunks : GC_GRID, 256, 0, st>>>(t, part, parts, max_norm, streams_past_cache(bytes), norm);
         }
     }
     GD_CHECK_LAUNCH("gd_grad_norm");
