@@ -69,28 +69,38 @@ __device__ __forceinline__ int gc_find(const gc_table& t, int chunk) {
 // elements in front of the first 16-byte boundary of p (0 .. 7)
 template <typename T> __device__ __forceinline__ int gc_head(const void* p) { return (int)((16 - ((uintptr_t)p & 15)) & 15) / (int)sizeof(T); }
 
-// f(element index, 16 bytes) over whole 16-byte words of [lo, hi), g(element index) over the rest; `head` = elements in front of the first
-// boundary of the tensor.  Chunk 0 of a tensor also takes the head.
-template <typename T, typename F, typename G>
-__device__ __forceinline__ void gc_range(long long n, int chunk, int head, F&& f, G&& g) {
+// f(element index, 16 bytes) over whole 16-byte words of chunk `chunk` (CHUNK elements), g(element index) over the rest; `head` = elements in
+// front of the first boundary of the tensor.  Chunk 0 of a tensor also takes the head.  BATCH words a thread are loaded at a time (behind
+// the last: the thread's first one again, not handed on).
+template <typename T, int CHUNK, int BATCH, typename F, typename G>
+__device__ __forceinline__ void gc_range(const T* p, long long n, int chunk, int head, bool last_use, F&& f, G&& g) {
     constexpr int V = word16<T>::N;
     if (head > n) head = (int)n;
-    const long long lo = head + (long long)chunk * GC_CHUNK;
-    const long long hi = lo + GC_CHUNK < n ? lo + GC_CHUNK : n;
+    const long long lo = head + (long long)chunk * CHUNK;
+    const long long hi = lo + CHUNK < n ? lo + CHUNK : n;
     if (chunk == 0 && (int)threadIdx.x < head) g((long long)threadIdx.x);
     const int words = hi > lo ? (int)((hi - lo) / V) : 0;
-#pragma unroll 4
-    for (int i = threadIdx.x; i < words; i += blockDim.x) f(lo + (long long)i * V);
+    const u32x4* const w = (const u32x4*)(p + lo);
+    for (int i = threadIdx.x; i < words; i += BATCH * blockDim.x) {
+        u32x4 x[BATCH];
+#pragma unroll
+        for (int j = 0; j < BATCH; ++j) {
+            const u32x4* at = w + (i + j * (int)blockDim.x < words ? i + j * (int)blockDim.x : i);
+            x[j] = last_use ? __builtin_nontemporal_load(at) : *at;
+        }
+#pragma unroll
+        for (int j = 0; j < BATCH; ++j)
+            if (i + j * (int)blockDim.x < words) f(lo + (long long)(i + j * (int)blockDim.x) * V, __builtin_bit_cast(word16<T>, x[j]));
+    }
     const long long tail = lo + (long long)words * V + threadIdx.x;
     if (tail < hi) g(tail);
 }
 
-template <typename T, bool INF>
+template <typename T, int CHUNK, bool INF>
 __device__ __forceinline__ double gc_norm_chunk(const void* src, long long n, int chunk, double acc) {
     const T* p = (const T*)src;
-    gc_range<T>(n, chunk, gc_head<T>(src),
-        [&](long long i) {
-            const word16<T> x = *(const word16<T>*)(p + i);
+    gc_range<T, CHUNK, (int)sizeof(T) * 2>(p, n, chunk, gc_head<T>(src), false,
+        [&](long long, word16<T> x) {
 #pragma unroll
             for (int j = 0; j < word16<T>::N; ++j) acc = gc_add<INF>(acc, (float)x.v[j]);
         },
@@ -98,14 +108,13 @@ __device__ __forceinline__ double gc_norm_chunk(const void* src, long long n, in
     return acc;
 }
 
-template <typename T>
+template <typename T, int CHUNK>
 __device__ __forceinline__ void gc_scale_chunk(const void* src, void* dst, long long n, int chunk, float f, bool stream) {
     const T* p = (const T*)src;
     T* q = (T*)dst;
     if (((uintptr_t)src & 15) == ((uintptr_t)dst & 15)) {
-        gc_range<T>(n, chunk, gc_head<T>(src),
-            [&](long long i) {
-                word16<T> x = __builtin_bit_cast(word16<T>, __builtin_nontemporal_load((const u32x4*)(p + i)));      // the last use
+        gc_range<T, CHUNK, (int)sizeof(T) * 2>(p, n, chunk, gc_head<T>(src), true,
+            [&](long long i, word16<T> x) {
 #pragma unroll
                 for (int j = 0; j < word16<T>::N; ++j) x.v[j] = to_storage<T>((float)x.v[j] * f);
                 store16(q + i, x, stream);
@@ -113,30 +122,31 @@ __device__ __forceinline__ void gc_scale_chunk(const void* src, void* dst, long 
             [&](long long i) { q[i] = to_storage<T>((float)p[i] * f); });
     } else {                                                // source and destination never share a boundary: element by element
         const int head = gc_head<T>(src) < n ? gc_head<T>(src) : (int)n;
-        const long long lo = chunk == 0 ? 0 : head + (long long)chunk * GC_CHUNK;
-        const long long end = head + (long long)(chunk + 1) * GC_CHUNK, hi = end < n ? end : n;
+        const long long lo = chunk == 0 ? 0 : head + (long long)chunk * CHUNK;
+        const long long end = head + (long long)(chunk + 1) * CHUNK, hi = end < n ? end : n;
         for (long long i = lo + threadIdx.x; i < hi; i += blockDim.x) q[i] = to_storage<T>((float)p[i] * f);
     }
 }
 
-template <bool INF>
+template <int CHUNK, bool INF>
 __device__ __forceinline__ double gc_norm_table(const gc_table& t, double acc) {
     for (int c = blockIdx.x; c < t.start[t.count]; c += gridDim.x) {
         const int k = gc_find(t, c), local = c - t.start[k];
-        if (t.dtype[k] == GD_F32) acc = gc_norm_chunk<float, INF>(t.src[k], t.n[k], local, acc);
-        else if (t.dtype[k] == GD_F16) acc = gc_norm_chunk<f16_t, INF>(t.src[k], t.n[k], local, acc);
-        else acc = gc_norm_chunk<bf16_t, INF>(t.src[k], t.n[k], local, acc);
+        if (t.dtype[k] == GD_F32) acc = gc_norm_chunk<float, CHUNK, INF>(t.src[k], t.n[k], local, acc);
+        else if (t.dtype[k] == GD_F16) acc = gc_norm_chunk<f16_t, CHUNK, INF>(t.src[k], t.n[k], local, acc);
+        else acc = gc_norm_chunk<bf16_t, CHUNK, INF>(t.src[k], t.n[k], local, acc);
     }
     return acc;
 }
 
+template <int CHUNK>
 __device__ __forceinline__ void gc_scale_table(const gc_table& t, float f, bool stream) {
     for (int c = t.start[t.count] - 1 - (int)blockIdx.x; c >= 0; c -= gridDim.x) {
         const int k = gc_find(t, c), local = c - t.start[k];
         if (f == 1.0f && t.dst[k] == t.src[k]) continue;    // g * 1 is g: nothing to write in place
-        if (t.dtype[k] == GD_F32) gc_scale_chunk<float>(t.src[k], t.dst[k], t.n[k], local, f, stream);
-        else if (t.dtype[k] == GD_F16) gc_scale_chunk<f16_t>(t.src[k], t.dst[k], t.n[k], local, f, stream);
-        else gc_scale_chunk<bf16_t>(t.src[k], t.dst[k], t.n[k], local, f, stream);
+        if (t.dtype[k] == GD_F32) gc_scale_chunk<float, CHUNK>(t.src[k], t.dst[k], t.n[k], local, f, stream);
+        else if (t.dtype[k] == GD_F16) gc_scale_chunk<f16_t, CHUNK>(t.src[k], t.dst[k], t.n[k], local, f, stream);
+        else gc_scale_chunk<bf16_t, CHUNK>(t.src[k], t.dst[k], t.n[k], local, f, stream);
     }
 }
 
@@ -150,7 +160,7 @@ __device__ __forceinline__ float gc_factor(double norm, float max_norm) {
 template <bool INF>
 __global__ void __launch_bounds__(256) k_grad_norm(const gc_table t, int first, double* __restrict__ part) {
     __shared__ double lds[4];
-    const double v = gc_block<INF>(gc_norm_table<INF>(t, 0.0), lds);
+    const double v = gc_block<INF>(gc_norm_table<GC_CHUNK, INF>(t, 0.0), lds);
     if (threadIdx.x == 0) part[blockIdx.x] = first ? v : gc_combine<INF>(part[blockIdx.x], v);
 }
 
@@ -174,11 +184,26 @@ __global__ void __launch_bounds__(256) k_grad_clip(const gc_table t, const doubl
     __shared__ double lds[4];
     const double v = gc_total<INF>(part, parts, lds);
     if (blockIdx.x == 0 && threadIdx.x == 0) norm[0] = (float)v;
-    gc_scale_table(t, gc_factor(v, max_norm), stream);
+    gc_scale_table<GC_CHUNK>(t, gc_factor(v, max_norm), stream);
+}
+
+// A few tensors of few elements: one workgroup does both steps, the chunks being whole tensors.  At 315 KB (an embedding of 77 x 1024 f32) it
+// takes 12.8 us for 4.7 + 5.2 us of two launches, but a call every 13.3 us for 15.9: the second launch costs the host 3.3 us.  The two
+// meet at about 400 KB; and one tensor after another costs it 2 us each.
+#define GC_SMALL_BYTES (384 * 1024)
+#define GC_SMALL_TENSORS 4
+#define GC_SMALL (1 << 18)      /* elements: no tensor of a small call is cut */
+template <bool INF>
+__global__ void __launch_bounds__(1024) k_grad_clip_small(const gc_table t, float max_norm, int scale, float* __restrict__ norm) {
+    __shared__ double lds[16];
+    double v = gc_block<INF>(gc_norm_table<GC_SMALL, INF>(t, 0.0), lds);
+    if (!INF) v = sqrt(v);
+    if (threadIdx.x == 0) norm[0] = (float)v;
+    if (scale) gc_scale_table<GC_SMALL>(t, gc_factor(v, max_norm), false);
 }
 
 // tensors [at, ..) into one launch's table; -> how many were taken.  Tensors of no elements take a place but no chunk.
-static int gc_fill(gc_table& t, const void* const* src, void* const* dst, const int64_t* n, const int32_t* dtype, int at, int count) {
+static int gc_fill(gc_table& t, const void* const* src, void* const* dst, const int64_t* n, const int32_t* dtype, int at, int count, int chunk) {
     const int k = count - at < GC_TENSORS ? count - at : GC_TENSORS;
     long long chunks = 0;
     t.count = k;
@@ -188,7 +213,7 @@ static int gc_fill(gc_table& t, const void* const* src, void* const* dst, const 
         t.n[i] = n[at + i];
         t.dtype[i] = (unsigned char)dtype[at + i];
         t.start[i] = (int)chunks;
-        chunks += (n[at + i] + GC_CHUNK - 1) / GC_CHUNK;
+        chunks += (n[at + i] + chunk - 1) / chunk;
     }
     t.start[k] = (int)chunks;
     return k;
@@ -201,10 +226,20 @@ static int gc_launch(const void* const* src, void* const* dst, const int64_t* n,
                      hipStream_t st) {
     gc_table t;
     int parts = 0;
-    double bytes = 0;
-    for (int i = 0; i < count; ++i) bytes += (double)n[i] * (dtype[i] == GD_F32 ? 4 : 2) * (dst && dst[i] != src[i] ? 2 : 1);
+    double bytes = 0, read = 0;
+    for (int i = 0; i < count; ++i) {
+        const double size = (double)n[i] * (dtype[i] == GD_F32 ? 4 : 2);
+        read += size;
+        bytes += dst && dst[i] != src[i] ? 2 * size : size;
+    }
+    if (count <= GC_SMALL_TENSORS && read <= GC_SMALL_BYTES) {
+        gc_fill(t, src, dst, n, dtype, 0, count, GC_SMALL);
+        k_grad_clip_small<INF><<<1, 1024, 0, st>>>(t, max_norm, dst != nullptr, norm);
+        GD_CHECK_LAUNCH("gd_grad_norm");
+        return GD_OK;
+    }
     for (int at = 0; at < count || at == 0; at += GC_TENSORS) {
-        gc_fill(t, src, dst, n, dtype, at, count);
+        gc_fill(t, src, dst, n, dtype, at, count, GC_CHUNK);
         // one table: as many workgroups as it has chunks; several: all of them, since every launch adds to the first one's partials
         const int grid = count <= GC_TENSORS && t.start[t.count] < GC_GRID ? (t.start[t.count] > 0 ? t.start[t.count] : 1) : GC_GRID;
         k_grad_norm<INF><<<grid, 256, 0, st>>>(t, at == 0, part);
@@ -215,7 +250,7 @@ static int gc_launch(const void* const* src, void* const* dst, const int64_t* n,
     } else {
         // backwards: what the norm read last is still in the memory-side cache
         for (int at = (count > 0 ? (count - 1) / GC_TENSORS : 0) * GC_TENSORS; at >= 0; at -= GC_TENSORS) {
-            if (count > GC_TENSORS) gc_fill(t, src, dst, n, dtype, at, count);
+            if (count > GC_TENSORS) gc_fill(t, src, dst, n, dtype, at, count, GC_CHUNK);
             const int chunks = t.start[t.count];
             k_grad_clip<INF><<<chunks < 1 ? 1 : chunks < GC_GRID ? chunks : GC_GRID, 256, 0, st>>>(t, part, parts, max_norm, streams_past_cache(bytes), norm);
         }
