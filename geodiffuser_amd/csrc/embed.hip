@@ -52,92 +52,125 @@ struct em_ids {
     __device__ __forceinline__ long long operator[](long long i) const { return wide ? ((const long long*)p)[i] : (long long)((const int*)p)[i]; }
 };
 
-// one wave a row; an id outside the table gives a row of NaN (there is no such row, and no way to raise from here)
+template <typename T, int N> struct alignas(N * sizeof(T)) em_piece { T v[N]; };
+
+// How a wave covers rows of `units` words (VEC) or elements: 2^shift lanes a row, 64 >> shift rows at a time
+static int em_lane_shift(int units) {
+    int s = 0;
+    while (s < 6 && (1 << s) < units) ++s;
+    return s;
+}
+
+// An id outside the table gives a row of NaN (there is no such row, and no way to raise from here).
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) k_embed(const em_ids ids, long long n, const T* __restrict__ table, const T* __restrict__ pos, int L, int V, int C,
-                                               float scale, bool stream, T* __restrict__ y) {
-    using COLS = em_cols<T, VEC>;
-    const int lane = threadIdx.x & 63;
-    const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+                                               float scale, bool stream, int shift, T* y) {
+    constexpr int W = VEC ? word16<T>::N : 1, BATCH = 4;
+    const int lane = threadIdx.x & 63, units = C / W, lanes = 1 << shift;
+    const long long row = (((long long)blockIdx.x * 4 + (threadIdx.x >> 6)) << (6 - shift)) + (lane >> shift);
     if (row >= n) return;
     const long long id = ids[row];
     const bool in = id >= 0 && id < V;
-    const T* src = table + (in ? id : 0) * C;
-    const T* ps = pos ? pos + (row % L) * C : nullptr;
-    for (int sl = 0; sl * COLS::SLICE < C; ++sl) {
-        float v[COLS::N], q[COLS::N] = {};
-        COLS::load(src, sl, lane, C, v);
-        if (ps) COLS::load(ps, sl, lane, C, q);
+    const em_piece<T, W>* src = (const em_piece<T, W>*)(table + (in ? id : 0) * C);
+    const em_piece<T, W>* ps = pos ? (const em_piece<T, W>*)(pos + (row % L) * C) : nullptr;
+    em_piece<T, W>* out = (em_piece<T, W>*)(y + row * C);
+    for (int u0 = 0; u0 < units; u0 += BATCH * lanes) {
+        em_piece<T, W> w[BATCH], q[BATCH];
+        const int u = u0 + (lane & (lanes - 1));
 #pragma unroll
-        for (int i = 0; i < COLS::N; ++i) {
-            v[i] = in ? __builtin_fmaf(scale, v[i], q[i]) : __builtin_nanf("");
+        for (int j = 0; j < BATCH; ++j)
+            if (u0 + j * lanes < units) {                    // (the same for the whole wave)
+                const int at = u + j * lanes < units ? u + j * lanes : 0;
+                w[j] = src[at];
+                if (ps) q[j] = ps[at];
+            }
+#pragma unroll
+        for (int j = 0; j < BATCH; ++j)
+            if (u + j * lanes < units) {
+                em_piece<T, W> o;
+#pragma unroll
+                for (int i = 0; i < W; ++i) o.v[i] = to_storage<T>(in ? __builtin_fmaf(scale, (float)w[j].v[i], ps ? (float)q[j].v[i] : 0.f) : __builtin_nanf(""));
+                if constexpr (VEC) store16(&out[u + j * lanes].v[0], __builtin_bit_cast(word16<T>, o), stream);
+                else out[u + j * lanes] = o;
+            }
+    }
+}
+
+// Zeros in those of the rows [v0, v0 + rows) of the table that `there` (of the row's offset) does not name.
+template <typename T, bool VEC, typename THERE>
+__device__ __forceinline__ void em_zero_rows(T* dtable, long long v0, int rows, int C, int shift, bool stream, THERE&& there) {
+    constexpr int W = VEC ? word16<T>::N : 1;
+    const int lane = threadIdx.x & 63, units = C / W, lanes = 1 << shift;
+    for (int r = ((threadIdx.x >> 6) << (6 - shift)) + (lane >> shift); r < rows; r += (blockDim.x >> 6) << (6 - shift)) {
+        if (there(r)) continue;
+        T* p = dtable + (v0 + r) * C;
+        for (int u = lane & (lanes - 1); u < units; u += lanes) {
+            if constexpr (VEC) store16(p + (long long)u * W, word16<T>{}, stream);
+            else p[u] = (T)0.f;
         }
-        COLS::store(y + row * C, sl, lane, C, v, stream);
     }
 }
 
-// sum of the four waves' values, in wave 0
-template <int N>
-__device__ __forceinline__ void em_fold(float* v, float (*lds)[64 * N], int wave, int lane) {
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < N; ++i) lds[wave][i * 64 + lane] = v[i];
-    __syncthreads();
-    if (wave == 0) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = (lds[0][i * 64 + lane] + lds[1][i * 64 + lane]) + (lds[2][i * 64 + lane] + lds[3][i * 64 + lane]);
-    }
+// rows of the table that a workgroup looks after for zeros: about 48 KB of them
+#define EM_ZERO_MAX 256
+static int em_zero_rows_of(int C, int elem) {
+    const int r = 48 * 1024 / (C * elem) / 16 * 16;
+    return r < 16 ? 16 : r > EM_ZERO_MAX ? EM_ZERO_MAX : r;
 }
+// positions that every workgroup may look through by itself, one a thread; with more, they are sorted first
+#define EM_SCAN_MAX 1024
 
-// rows of the table that a workgroup looks after for zeros
-#define EM_ZERO_ROWS 16
-
-// The first workgroups: (position, slice).  The one at a token's first position adds up all of that token's rows; the others end at once.
-// The workgroups behind them: EM_ZERO_ROWS rows of the table each, zeros where no position has the row's token.
+// The first workgroups: (position, slice).  The one at a token's first position adds up all of that token's rows, its 16 waves side by side; the
+// others end at once.  The workgroups behind them: zero_rows rows of the table each, zeros where no position has the row's token.
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(256) k_embed_bwd_scan(const em_ids ids, int n, const T* __restrict__ dy, int V, int C, long long padding, float scale,
-                                                        bool stream, T* __restrict__ dtable) {
+__global__ void __launch_bounds__(EM_SCAN_MAX) k_embed_bwd_scan(const em_ids ids, int n, const T* __restrict__ dy, int V, int C, long long padding, float scale,
+                                                                bool stream, int zero_rows, int shift, T* dtable) {
     using COLS = em_cols<T, VEC>;
-    constexpr int N = COLS::N;
-    __shared__ float lds[4][64 * N];
-    __shared__ int list[256], count[4];
+    constexpr int N = COLS::N, AHEAD = 4, WAVES = EM_SCAN_MAX / 64;
+    __shared__ float lds[WAVES][64 * N];
+    __shared__ int list[EM_SCAN_MAX], count[WAVES];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int slices = (C + COLS::SLICE - 1) / COLS::SLICE;
     const long long owners = (long long)n * slices;
+    const long long mine = tid < n ? ids[tid] : -1;
     if (blockIdx.x < owners) {
         const int first = (int)(blockIdx.x / slices), sl = (int)(blockIdx.x % slices);
         const long long id = ids[first];
         if (id < 0 || id >= V || id == padding) return;
-        bool before = false;
-        for (int j = tid; j < first; j += 256) before |= ids[j] == id;
-        if (__syncthreads_or(before)) return;
-        float acc[N] = {};
-        for (int base = first; base < n; base += 256) {
-            const int j = base + tid;
-            const bool mine = j < n && ids[j] == id;
-            const unsigned long long mask = __ballot(mine);
-            if (lane == 0) count[wave] = __popcll(mask);
-            __syncthreads();
-            int at = 0, total = 0;
+        const bool same = tid < n && mine == id;
+        if (__syncthreads_or(same && tid < first)) return;
+        const unsigned long long mask = __ballot(same);
+        if (lane == 0) count[wave] = __popcll(mask);
+        __syncthreads();
+        int at = 0, total = 0;
 #pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                if (w < wave) at += count[w];
-                total += count[w];
-            }
-            if (mine) list[at + __popcll(mask & ((1ull << lane) - 1))] = j;
-            __syncthreads();
-            for (int m = wave; m < total; m += 16) {         // (behind the last: the first again, adding nothing)
-                float v[4][N];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) COLS::load(dy + (long long)list[m + 4 * j < total ? m + 4 * j : m] * C, sl, lane, C, v[j]);
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-#pragma unroll
-                    for (int i = 0; i < N; ++i) acc[i] += m + 4 * j < total ? v[j][i] : 0.f;
-            }
-            __syncthreads();
+        for (int w = 0; w < WAVES; ++w) {
+            if (w < wave) at += count[w];
+            total += count[w];
         }
-        em_fold<N>(acc, lds, wave, lane);
+        if (same) list[at + __popcll(mask & ((1ull << lane) - 1))] = tid;
+        __syncthreads();
+        float acc[N] = {};
+        for (int m = wave; m < total; m += AHEAD * WAVES) {  // (behind the last: the first again, adding nothing)
+            float v[AHEAD][N];
+#pragma unroll
+            for (int j = 0; j < AHEAD; ++j) COLS::load(dy + (long long)list[m + WAVES * j < total ? m + WAVES * j : m] * C, sl, lane, C, v[j]);
+#pragma unroll
+            for (int j = 0; j < AHEAD; ++j)
+#pragma unroll
+                for (int i = 0; i < N; ++i) acc[i] += m + WAVES * j < total ? v[j][i] : 0.f;
+        }
+        // the waves that had a row, in their order
+        const int waves = total < WAVES ? total : WAVES;
+        if (waves > 1) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) lds[wave][i * 64 + lane] = acc[i];
+            __syncthreads();
+            if (wave == 0)
+                for (int w = 1; w < waves; ++w)
+#pragma unroll
+                    for (int i = 0; i < N; ++i) acc[i] += lds[w][i * 64 + lane];
+        }
         if (wave == 0) {
 #pragma unroll
             for (int i = 0; i < N; ++i) acc[i] *= scale;
@@ -145,19 +178,13 @@ __global__ void __launch_bounds__(256) k_embed_bwd_scan(const em_ids ids, int n,
         }
         return;
     }
-    const long long v0 = ((long long)blockIdx.x - owners) * EM_ZERO_ROWS;
-    int* there = list;
-    if (tid < EM_ZERO_ROWS) there[tid] = 0;
+    const long long v0 = ((long long)blockIdx.x - owners) * zero_rows;
+    const int rows = v0 + zero_rows < V ? zero_rows : (int)(V - v0);
+    if (tid < rows) list[tid] = 0;
     __syncthreads();
-    for (int j = tid; j < n; j += 256) {
-        const long long id = ids[j];
-        if (id >= v0 && id < v0 + EM_ZERO_ROWS && id != padding) there[id - v0] = 1;
-    }
+    if (mine >= v0 && mine < v0 + rows && mine != padding) list[mine - v0] = 1;
     __syncthreads();
-    const float zero[N] = {};
-    for (int r = wave; r < EM_ZERO_ROWS; r += 4)
-        if (v0 + r < V && !there[r])
-            for (int sl = 0; sl < slices; ++sl) COLS::store(dtable + (v0 + r) * C, sl, lane, C, zero, stream);
+    em_zero_rows<T, VEC>(dtable, v0, rows, C, shift, stream, [&](int r) { return list[r] != 0; });
 }
 
 // ---- many positions: the positions sorted by token ---------------------------------------------------------------------------------------
@@ -295,6 +322,84 @@ __global__ void __launch_bounds__(1024) k_embed_sort_move(const em_keys k, const
     }
 }
 
+// Up to EM_LDS_MAX positions and vocabularies below 2^20: the same sort by one workgroup in LDS, an entry in 32 bits (token above, position
+// below), one launch for all passes.  (The gradient of 4000 positions takes 31 us so and 36 us by the launches above, of 8000 42 and 37.)
+#define EM_LDS_MAX 4096
+#define EM_LDS_POS_BITS 12
+
+__global__ void __launch_bounds__(1024) k_embed_sort_lds(const em_keys k, int n, int passes, uint32_t* __restrict__ key_out, uint32_t* __restrict__ pos_out,
+                                                         unsigned char* __restrict__ there, int there_words) {
+    __shared__ uint32_t entry[2][EM_LDS_MAX];
+    __shared__ int counts[16][256], scan[256];
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+    for (int i = tid; i < there_words; i += 1024) ((uint32_t*)there)[i] = 0;
+#pragma unroll
+    for (int r = 0; r < EM_LDS_MAX / 1024; ++r) {
+        const int i = r * 1024 + tid;
+        if (i < n) entry[0][i] = k(i) << EM_LDS_POS_BITS | (uint32_t)i;
+    }
+    const int run = (n + 1023) / 1024 * 64, lo = wave * run, hi = lo + run < n ? lo + run : n;
+    for (int p = 0; p < passes; ++p) {
+        const uint32_t* from = entry[p & 1];
+        uint32_t* to = entry[(p + 1) & 1];
+        const int shift = EM_LDS_POS_BITS + 8 * p;
+        for (int i = tid; i < 16 * 256; i += 1024) counts[0][i] = 0;
+        __syncthreads();
+        volatile int* place = counts[wave];
+        for (int base = lo; base < hi; base += 64) {
+            const bool live = base + lane < hi;
+            const int d = live ? (int)(from[base + lane] >> shift) & 255 : 0;
+            const unsigned long long m = em_match(d, live);
+            if (live && (m & ((1ull << lane) - 1)) == 0) place[d] += __popcll(m);
+            __builtin_amdgcn_wave_barrier();
+        }
+        __syncthreads();
+        int all = 0;
+        if (tid < 256) {
+#pragma unroll
+            for (int w = 0; w < 16; ++w) all += counts[w][tid];
+            scan[tid] = all;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int o = 1; o < 256; o <<= 1) {
+            const int v = tid < 256 && tid >= o ? scan[tid - o] : 0;
+            __syncthreads();
+            if (tid < 256) scan[tid] += v;
+            __syncthreads();
+        }
+        if (tid < 256) {
+            int at = scan[tid] - all;
+#pragma unroll
+            for (int w = 0; w < 16; ++w) {
+                const int c = counts[w][tid];
+                counts[w][tid] = at;
+                at += c;
+            }
+        }
+        __syncthreads();
+        for (int base = lo; base < hi; base += 64) {
+            const bool live = base + lane < hi;
+            const uint32_t e = live ? from[base + lane] : 0;
+            const int d = (int)(e >> shift) & 255;
+            const unsigned long long m = em_match(d, live);
+            const int rank = __popcll(m & ((1ull << lane) - 1));
+            const int first = live ? place[d] : 0;
+            __builtin_amdgcn_wave_barrier();
+            if (live && rank == 0) place[d] = first + __popcll(m);
+            __builtin_amdgcn_wave_barrier();
+            if (live) to[first + rank] = e;
+        }
+        __syncthreads();
+    }
+    for (int i = tid; i < n; i += 1024) {
+        const uint32_t e = entry[passes & 1][i], key = e >> EM_LDS_POS_BITS;
+        key_out[i] = key;
+        pos_out[i] = e & (EM_LDS_MAX - 1);
+        if (key < k.vocab) there[key] = 1;
+    }
+}
+
 // Sums over the sorted entries: a wave takes a tile of them (at most 64) and one slice of channels, and writes the tokens that begin in its
 // tile.  A token that goes on into the next tile but not beyond it is finished by the wave of the tile where it begins (the next one
 // leaves it out); one that goes on further leaves a partial sum in each of its tiles: `tail` in the first, `head` in the others.  The
@@ -308,10 +413,11 @@ struct em_sum {
     unsigned vocab;
     float scale;
     bool stream;
+    int zero_rows, shift;
 };
 
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(256) k_embed_bwd_sum(const em_sum a, const T* __restrict__ dy, T* __restrict__ dtable) {
+__global__ void __launch_bounds__(256) k_embed_bwd_sum(const em_sum a, const T* __restrict__ dy, T* dtable) {
     using COLS = em_cols<T, VEC>;
     constexpr int N = COLS::N, AHEAD = 8;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), C = a.C;
@@ -385,11 +491,9 @@ __global__ void __launch_bounds__(256) k_embed_bwd_sum(const em_sum a, const T* 
         }
         return;
     }
-    const float zero[N] = {};
-    const long long v0 = ((long long)blockIdx.x - item_blocks) * EM_ZERO_ROWS;
-    for (int r = wave; r < EM_ZERO_ROWS; r += 4)
-        if (v0 + r < a.vocab && !a.there[v0 + r])
-            for (int sl = 0; sl < a.slices; ++sl) COLS::store(dtable + (v0 + r) * C, sl, lane, C, zero, a.stream);
+    const long long v0 = ((long long)blockIdx.x - item_blocks) * a.zero_rows;
+    const int rows = v0 + a.zero_rows < a.vocab ? a.zero_rows : (int)(a.vocab - v0);
+    em_zero_rows<T, VEC>(dtable, v0, rows, C, a.shift, a.stream, [&](int r) { return a.there[v0 + r] != 0; });
 }
 
 // The tokens that go on for two tiles and more: the tail of the tile where they begin + the heads of the others (padding has half of all
@@ -470,8 +574,6 @@ __global__ void __launch_bounds__(256) k_embed_bwd_join_groups(const em_sum a, T
 // more than one.
 #define EM_POS_ROWS 64
 
-template <typename T, int N> struct alignas(N * sizeof(T)) em_piece { T v[N]; };
-
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) k_embed_pos_bwd(const T* __restrict__ dy, long long B, long long width, long long out_width, long long per, float* __restrict__ part,
                                                        T* __restrict__ dpos) {
@@ -544,17 +646,17 @@ extern "C" int gd_embed(const void* ids, int ids64, int64_t n, const void* table
     GD_REQUIRE(!pos || L > 0, GD_EINVAL, "gd_embed: position rows need the sequence length");
     const bool vec = em_vec(C, EM_ELEM(dtype), table, y, pos);
     hipStream_t st = as_stream(stream);
-    EM_LAUNCH(dtype, vec, (k_embed<T, VEC><<<(unsigned)((n + 3) / 4), 256, 0, st>>>(em_ids{ids, ids64}, n, (const T*)table, (const T*)pos, L, (int)vocab, C, scale,
-                      streams_past_cache((double)EM_ELEM(dtype) * C * ((double)n + (n < vocab ? n : vocab))), (T*)y)));
+    const int shift = em_lane_shift(vec ? C * EM_ELEM(dtype) / 16 : C);
+    const long long waves = (n + (64 >> shift) - 1) >> (6 - shift);
+    const bool past = streams_past_cache((double)EM_ELEM(dtype) * C * ((double)n + (n < vocab ? n : vocab)));
+    EM_LAUNCH(dtype, vec, (k_embed<T, VEC><<<(unsigned)((waves + 3) / 4), 256, 0, st>>>(em_ids{ids, ids64}, n, (const T*)table, (const T*)pos, L, (int)vocab, C, scale, past, shift, (T*)y)));
     GD_CHECK_LAUNCH("gd_embed");
     return GD_OK;
 }
 
-// Up to here every workgroup may look through all ids by itself (one launch); above, they are sorted first.
-#define EM_SCAN_MAX 1024
-
 struct em_plan {
     em_sort sort;
+    bool in_lds;
     int passes, tile, tiles;
     size_t key[2], pos[2], table, there, head, tail, bytes;
 };
@@ -563,6 +665,7 @@ static em_plan em_plan_of(long long n, long long vocab, int C) {
     em_plan p = {};
     if (n <= EM_SCAN_MAX) return p;
     p.sort = em_sort_of(n);
+    p.in_lds = n <= EM_LDS_MAX && vocab < (1 << (32 - EM_LDS_POS_BITS));
     p.passes = 1;
     while (p.passes < 4 && ((unsigned long long)vocab >> (8 * p.passes))) ++p.passes;
     // 64 entries a tile; fewer where the tiles would not fill the chip's waves
@@ -591,7 +694,8 @@ extern "C" int gd_embed_bwd(const void* ids, int ids64, int64_t n, const void* d
     GD_REQUIRE(dtable && (n == 0 || (ids && dy)), GD_EINVAL, "gd_embed_bwd: null pointer");
     const bool vec = em_vec(C, EM_ELEM(dtype), dy, dtable);
     const int slice = vec ? 64 * (16 / EM_ELEM(dtype)) : 512, slices = (C + slice - 1) / slice;
-    const long long zeros = (vocab + EM_ZERO_ROWS - 1) / EM_ZERO_ROWS;
+    const int zero_rows = em_zero_rows_of(C, EM_ELEM(dtype)), shift = em_lane_shift(vec ? C * EM_ELEM(dtype) / 16 : C);
+    const long long zeros = (vocab + zero_rows - 1) / zero_rows;
     const bool past = streams_past_cache((double)EM_ELEM(dtype) * C * ((double)n + vocab));
     const em_plan p = em_plan_of(n, vocab, C);
     GD_REQUIRE(!p.bytes || (workspace && workspace_bytes >= p.bytes && ((uintptr_t)workspace & 15) == 0), GD_EWORKSPACE, "gd_embed_bwd: workspace of %zu bytes needed", p.bytes);
@@ -600,21 +704,29 @@ extern "C" int gd_embed_bwd(const void* ids, int ids64, int64_t n, const void* d
     if (!p.bytes) {
         const long long grid = n * slices + zeros;
         GD_REQUIRE(grid < (1ll << 31), GD_EUNSUPPORTED, "gd_embed_bwd: table too large");
-        EM_LAUNCH(dtype, vec, (k_embed_bwd_scan<T, VEC><<<(unsigned)grid, 256, 0, st>>>(in, (int)n, (const T*)dy, (int)vocab, C, padding, scale, past, (T*)dtable)));
+        EM_LAUNCH(dtype, vec, (k_embed_bwd_scan<T, VEC><<<(unsigned)grid, EM_SCAN_MAX, 0, st>>>(in, (int)n, (const T*)dy, (int)vocab, C, padding, scale, past, zero_rows, shift, (T*)dtable)));
     } else {
         const long long grid = ((long long)p.tiles * slices + 3) / 4 + zeros;
         GD_REQUIRE(grid < (1ll << 31) && (long long)p.tiles * ((C + 255) / 256) < (1ll << 30), GD_EUNSUPPORTED, "gd_embed_bwd: too many positions for this width");
         char* const ws = (char*)workspace;
         em_keys k = {in, nullptr, nullptr, (unsigned)vocab, padding};
-        for (int i = 0; i < p.passes; ++i) {
-            const bool last = i + 1 == p.passes;
-            uint32_t *const key = (uint32_t*)(ws + p.key[i & 1]), *const pos = (uint32_t*)(ws + p.pos[i & 1]);
-            k_embed_sort_count<<<p.sort.blocks, 1024, 0, st>>>(k, p.sort, 8 * i, (int*)(ws + p.table), (uint32_t*)(ws + p.there), i == 0 ? (int)((vocab + 3) / 4) : 0);
-            k_embed_sort_move<<<p.sort.blocks, 1024, 0, st>>>(k, p.sort, 8 * i, (const int*)(ws + p.table), key, pos, last ? (unsigned char*)(ws + p.there) : nullptr);
+        const int there_words = (int)((vocab + 3) / 4);
+        if (p.in_lds) {
+            uint32_t *const key = (uint32_t*)(ws + p.key[0]), *const pos = (uint32_t*)(ws + p.pos[0]);
+            k_embed_sort_lds<<<1, 1024, 0, st>>>(k, (int)n, p.passes, key, pos, (unsigned char*)(ws + p.there), there_words);
             k.key = key;
             k.pos = pos;
+        } else {
+            for (int i = 0; i < p.passes; ++i) {
+                const bool last = i + 1 == p.passes;
+                uint32_t *const key = (uint32_t*)(ws + p.key[i & 1]), *const pos = (uint32_t*)(ws + p.pos[i & 1]);
+                k_embed_sort_count<<<p.sort.blocks, 1024, 0, st>>>(k, p.sort, 8 * i, (int*)(ws + p.table), (uint32_t*)(ws + p.there), i == 0 ? there_words : 0);
+                k_embed_sort_move<<<p.sort.blocks, 1024, 0, st>>>(k, p.sort, 8 * i, (const int*)(ws + p.table), key, pos, last ? (unsigned char*)(ws + p.there) : nullptr);
+                k.key = key;
+                k.pos = pos;
+            }
         }
-        const em_sum a = {k.key, k.pos, (const unsigned char*)(ws + p.there), (float*)(ws + p.head), (float*)(ws + p.tail), n, p.tile, p.tiles, slices, C, (unsigned)vocab, scale, past};
+        const em_sum a = {k.key, k.pos, (const unsigned char*)(ws + p.there), (float*)(ws + p.head), (float*)(ws + p.tail), n, p.tile, p.tiles, slices, C, (unsigned)vocab, scale, past, zero_rows, shift};
         EM_LAUNCH(dtype, vec, (k_embed_bwd_sum<T, VEC><<<(unsigned)grid, 256, 0, st>>>(a, (const T*)dy, (T*)dtable)));
         const unsigned wide = (unsigned)((C + 255) / 256), groups = (unsigned)((p.tiles + EM_GROUP - 1) / EM_GROUP);
         if (p.tiles > 2) {
