@@ -245,6 +245,22 @@ __device__ __forceinline__ void em_count(const em_keys& k, long long lo, long lo
     }
 }
 
+// Exclusive sums over the digits: thread d < 256 gives its digit's count and gets the sum of those below.  All threads call it (it has
+// a barrier, behind which what they wrote to LDS before is seen).
+__device__ __forceinline__ int em_below(int c, int* sums) {
+    const int tid = threadIdx.x, lane = tid & 63;
+    int v = c;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int u = __shfl_up(v, o, 64);
+        if (lane >= o) v += u;
+    }
+    if (tid < 256 && lane == 63) sums[tid >> 6] = v;
+    __syncthreads();
+    const int w = tid >> 6;
+    return v - c + (w > 0 ? sums[0] : 0) + (w > 1 ? sums[1] : 0) + (w > 2 ? sums[2] : 0);
+}
+
 __global__ void __launch_bounds__(1024) k_embed_sort_count(const em_keys k, const em_sort s, int shift, int* __restrict__ table, uint32_t* __restrict__ there, int there_words) {
     __shared__ int counts[16][256];
     const int tid = threadIdx.x, wave = tid >> 6;
@@ -265,35 +281,52 @@ __global__ void __launch_bounds__(1024) k_embed_sort_count(const em_keys k, cons
 
 __global__ void __launch_bounds__(1024) k_embed_sort_move(const em_keys k, const em_sort s, int shift, const int* __restrict__ table, uint32_t* __restrict__ key_out,
                                                           uint32_t* __restrict__ pos_out, unsigned char* __restrict__ there) {
-    __shared__ int counts[16][256], part[4][2][256], scan[256];
+    __shared__ int counts[16][256], part[4][2][256], sums[4];
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, d0 = tid & 255, q = tid >> 8;
+    const long long run = s.per_block / 16, lo = (long long)blockIdx.x * s.per_block + wave * run, hi = lo + run < s.n ? lo + run : s.n;
+    // up to two rounds of entries (EM_SORT_KEYS a workgroup) stay in registers, loaded before anything else
+    const bool few = s.per_block <= EM_SORT_KEYS;
+    uint32_t key_of[2] = {}, pos_of[2] = {};
+    if (few) {
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            const long long i = lo + 64 * r + lane;
+            if (i < hi) {
+                key_of[r] = k(i);
+                pos_of[r] = k.key ? k.pos[i] : (uint32_t)i;
+            }
+        }
+    }
     for (int i = tid; i < 16 * 256; i += 1024) counts[0][i] = 0;
     // how many entries of digit d0 lie in earlier workgroups, and in all: four threads share a digit
     int before = 0, all = 0;
-#pragma unroll 8
-    for (int b = q; b < s.blocks; b += 4) {
-        const int c = table[b * 256 + d0];
-        before += b < (int)blockIdx.x ? c : 0;
-        all += c;
+    for (int b0 = q; b0 < s.blocks; b0 += 32) {
+        int c[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) c[j] = table[(b0 + 4 * j < s.blocks ? b0 + 4 * j : b0) * 256 + d0];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int b = b0 + 4 * j;
+            before += b < (int)blockIdx.x ? c[j] : 0;
+            all += b < s.blocks ? c[j] : 0;
+        }
     }
     part[q][0][d0] = before;
     part[q][1][d0] = all;
     __syncthreads();
-    const long long run = s.per_block / 16, lo = (long long)blockIdx.x * s.per_block + wave * run, hi = lo + run < s.n ? lo + run : s.n;
-    em_count(k, lo, hi, shift, counts[wave]);
+    volatile int* place = counts[wave];
+    int round = 0;
+    for (long long base = lo; base < hi; base += 64, ++round) {
+        const bool live = base + lane < hi;
+        const int d = live ? (int)((few ? key_of[round & 1] : k(base + lane)) >> shift) & 255 : 0;
+        const unsigned long long m = em_match(d, live);
+        if (live && (m & ((1ull << lane) - 1)) == 0) place[d] += __popcll(m);
+        __builtin_amdgcn_wave_barrier();
+    }
     before = part[0][0][d0] + part[1][0][d0] + part[2][0][d0] + part[3][0][d0];
     all = part[0][1][d0] + part[1][1][d0] + part[2][1][d0] + part[3][1][d0];
-    if (q == 0) scan[d0] = all;
-    __syncthreads();
-#pragma unroll
-    for (int o = 1; o < 256; o <<= 1) {                      // inclusive scan over the digits
-        const int v = q == 0 && d0 >= o ? scan[d0 - o] : 0;
-        __syncthreads();
-        if (q == 0) scan[d0] += v;
-        __syncthreads();
-    }
+    int at = em_below(all, sums) + before;                   // first place of this digit's entries of this workgroup
     if (q == 0) {
-        int at = scan[d0] - all + before;                    // first place of this digit's entries of this workgroup
 #pragma unroll
         for (int w = 0; w < 16; ++w) {
             const int c = counts[w][d0];
@@ -302,11 +335,11 @@ __global__ void __launch_bounds__(1024) k_embed_sort_move(const em_keys k, const
         }
     }
     __syncthreads();
-    volatile int* place = counts[wave];
-    for (long long base = lo; base < hi; base += 64) {
+    round = 0;
+    for (long long base = lo; base < hi; base += 64, ++round) {
         const long long i = base + lane;
         const bool live = i < hi;
-        const uint32_t key = live ? k(i) : 0;
+        const uint32_t key = few ? key_of[round & 1] : live ? k(i) : 0;
         const int d = (int)(key >> shift) & 255;
         const unsigned long long m = em_match(d, live);
         const int rank = __popcll(m & ((1ull << lane) - 1));
@@ -316,7 +349,7 @@ __global__ void __launch_bounds__(1024) k_embed_sort_move(const em_keys k, const
         __builtin_amdgcn_wave_barrier();
         if (live) {
             key_out[first + rank] = key;
-            pos_out[first + rank] = k.key ? k.pos[i] : (uint32_t)i;
+            pos_out[first + rank] = few ? pos_of[round & 1] : k.key ? k.pos[i] : (uint32_t)i;
             if (there && key < k.vocab) there[key] = 1;
         }
     }
@@ -330,7 +363,7 @@ __global__ void __launch_bounds__(1024) k_embed_sort_move(const em_keys k, const
 __global__ void __launch_bounds__(1024) k_embed_sort_lds(const em_keys k, int n, int passes, uint32_t* __restrict__ key_out, uint32_t* __restrict__ pos_out,
                                                          unsigned char* __restrict__ there, int there_words) {
     __shared__ uint32_t entry[2][EM_LDS_MAX];
-    __shared__ int counts[16][256], scan[256];
+    __shared__ int counts[16][256], sums[4];
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
     for (int i = tid; i < there_words; i += 1024) ((uint32_t*)there)[i] = 0;
 #pragma unroll
@@ -358,18 +391,9 @@ __global__ void __launch_bounds__(1024) k_embed_sort_lds(const em_keys k, int n,
         if (tid < 256) {
 #pragma unroll
             for (int w = 0; w < 16; ++w) all += counts[w][tid];
-            scan[tid] = all;
         }
-        __syncthreads();
-#pragma unroll
-        for (int o = 1; o < 256; o <<= 1) {
-            const int v = tid < 256 && tid >= o ? scan[tid - o] : 0;
-            __syncthreads();
-            if (tid < 256) scan[tid] += v;
-            __syncthreads();
-        }
+        int at = em_below(all, sums);
         if (tid < 256) {
-            int at = scan[tid] - all;
 #pragma unroll
             for (int w = 0; w < 16; ++w) {
                 const int c = counts[w][tid];
@@ -419,7 +443,7 @@ struct em_sum {
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) k_embed_bwd_sum(const em_sum a, const T* __restrict__ dy, T* dtable) {
     using COLS = em_cols<T, VEC>;
-    constexpr int N = COLS::N, AHEAD = 8;
+    constexpr int N = COLS::N, AHEAD = 4;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), C = a.C;
     const long long items = (long long)a.tiles * a.slices;
     const long long item_blocks = (items + 3) / 4;
@@ -668,9 +692,12 @@ static em_plan em_plan_of(long long n, long long vocab, int C) {
     p.in_lds = n <= EM_LDS_MAX && vocab < (1 << (32 - EM_LDS_POS_BITS));
     p.passes = 1;
     while (p.passes < 4 && ((unsigned long long)vocab >> (8 * p.passes))) ++p.passes;
-    // 64 entries a tile; fewer where the tiles would not fill the chip's waves
-    p.tile = 64;
-    while (p.tile > 8 && n / p.tile < 4096) p.tile /= 2;
+    // 64 entries a tile where they give each CU 32 waves (times the slices of 512 channels): a partial sum costs two entries' traffic.  With
+    // fewer waves shorter tiles, down to 8, until there are 16 a CU.  (157696 positions of 1024 channels: 64 a tile 153 us, 32 141 us;
+    // 600000: 353 and 379 us; 40000 of 768 channels: 32 a tile 67, 16 58, 8 65 us.)
+    const long long slices = (C + 511) / 512;
+    p.tile = n / 64 * slices >= 8192 ? 64 : 32;
+    while (p.tile > 8 && n / p.tile * slices < 4096) p.tile /= 2;
     p.tiles = (int)((n + p.tile - 1) / p.tile);
     size_t at = 0;
     const auto take = [&](size_t bytes) { const size_t here = at; at += (bytes + 255) / 256 * 256; return here; };
