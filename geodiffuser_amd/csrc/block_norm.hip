@@ -456,15 +456,16 @@ extern "C" int gd_block_norm(const gd_block_norm_t* f, int dtype, void* stream) 
     return GD_OK;
 }
 
-// Two workgroups of four waves a CU cover the row's latencies; every further one costs BN_SUMS more rows of partial sums to write and
-// add.  At least 4 rows each.
-static long long bn_workgroups(long long rows) {
-    const long long n = (rows + 3) / 4;
-    return n < 512 ? n : 512;
+// As many workgroups as are resident at once: one a CU for the kernels with 16 channels or 512 threads a row and more (their registers leave
+// one wave a SIMD), two for the others.  Every further one is another row of partial sums to write and add.  At least 4 rows each.
+// (16384 x 1024 bf16 with gate and both norms: 256 workgroups 46 us, 512 53, 1024 69; 4096 x 4096 bf16: 41, 47, 59; 16384 x 1280 f32: 119, 109, 116.)
+static long long bn_workgroups(long long rows, int C) {
+    const long long n = (rows + 3) / 4, most = (C > 512 && C <= 1024) || C > 2048 ? 256 : 512;
+    return n < most ? n : most;
 }
 
 extern "C" size_t gd_block_norm_bwd_workspace_bytes(int64_t rows, int C, int64_t gate_rows) {
-    const long long wg = bn_workgroups(rows);
+    const long long wg = bn_workgroups(rows, C);
     return sizeof(float) * (size_t)C * (size_t)(BN_SUMS * wg + (gate_rows > 0 ? wg + gate_rows - 1 : 0));
 }
 
@@ -473,7 +474,7 @@ static void bn_launch_bwd(const gd_block_norm_bwd_t& a, float* ws, hipStream_t s
     bn_bwd_args b;
     b.a = a;
     b.stream = streams_past_cache((double)a.f.rows * a.f.C * sizeof(T) * (1 + !!a.f.res + !!a.gy + !!a.gs + !!a.dx + !!a.dres));
-    const long long wg0 = bn_workgroups(a.f.rows);
+    const long long wg0 = bn_workgroups(a.f.rows, a.f.C);
     b.rows_per_wg = (a.f.rows + wg0 - 1) / wg0;
     const int wg = (int)((a.f.rows + b.rows_per_wg - 1) / b.rows_per_wg);
     void* const dst[BN_SUMS] = {a.dpre_gamma, a.dpre_beta, a.dpost_gamma, a.dpost_beta};
