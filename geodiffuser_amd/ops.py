@@ -5,6 +5,8 @@ tensor or a missing library raises.
 from __future__ import annotations
 
 import ctypes
+import math
+import operator
 import threading
 import os
 from typing import List, NamedTuple, Optional, Sequence, Tuple
@@ -1303,24 +1305,32 @@ def block_norm_bwd(x, res, gy, gs, stats, pre: Optional[Norm], post: Optional[No
     return out
 
 
+_tensor_dtype, _tensor_shape = operator.attrgetter("dtype"), operator.attrgetter("shape")
+
+
 def _grad_norm(grads, norm_type, max_norm, out):
     lib = _lib.load()
     grads = list(grads)
-    norm_type = float(norm_type)
-    if norm_type not in (2.0, float("inf")):
+    if norm_type != 2.0 and norm_type != math.inf:
         raise _lib.GeodiffError(f"grad_norm: norm_type must be 2 or inf, got {norm_type}")
     if not grads:
         raise _lib.GeodiffError("grad_norm: no tensors")
+    # (hundreds of tensors a call: each question goes over the whole list in one built-in loop)
+    devices = set(map(torch.Tensor.get_device, grads))
     dev = grads[0].get_device()
-    for t in grads:
-        if not t.is_cuda or t.get_device() != dev:
-            raise _lib.GeodiffError(f"grad_norm: expected GPU tensors of one device (the HIP path has no CPU fallback), got {t.device}")
-        if not t.is_contiguous() and not (t.dim() == 4 and t.is_contiguous(memory_format=torch.channels_last)):
-            raise _lib.GeodiffError("grad_norm: tensors must be contiguous (or channels_last)")
+    if dev < 0 or len(devices) != 1:
+        raise _lib.GeodiffError(f"grad_norm: expected GPU tensors of one device (the HIP path has no CPU fallback), got {sorted({str(t.device) for t in grads})}")
+    dense = all(map(torch.Tensor.is_contiguous, grads))
+    if not dense and not all(t.is_contiguous() or (t.dim() == 4 and t.is_contiguous(memory_format=torch.channels_last)) for t in grads):
+        raise _lib.GeodiffError("grad_norm: tensors must be contiguous (or channels_last)")
+    dtypes = list(map(_tensor_dtype, grads))
+    codes = list(map(_DT.get, dtypes))
+    if None in codes:
+        raise _lib.GeodiffError(f"grad_norm: expected float16/bfloat16/float32, got {dtypes[codes.index(None)]}")
     n = len(grads)
-    src = (ctypes.c_void_p * n)(*[t.data_ptr() for t in grads])
-    numel = (ctypes.c_int64 * n)(*[t.numel() for t in grads])
-    dts = (ctypes.c_int32 * n)(*[_DT.get(t.dtype, -1) for t in grads])
+    src = (ctypes.c_void_p * n)(*map(torch.Tensor.data_ptr, grads))
+    numel = (ctypes.c_int64 * n)(*map(torch.Tensor.numel, grads))
+    dts = (ctypes.c_int32 * n)(*codes)
     dst = None
     if max_norm is not None:
         max_norm = float(max_norm)
@@ -1329,12 +1339,15 @@ def _grad_norm(grads, norm_type, max_norm, out):
         dst = src
         if out is not None:
             out = list(out)
-            if len(out) != n or any(o.shape != t.shape or o.dtype != t.dtype or o.get_device() != dev or o.stride() != t.stride() for o, t in zip(out, grads)):
+            if (list(map(_tensor_shape, out)) != list(map(_tensor_shape, grads)) or list(map(_tensor_dtype, out)) != dtypes or set(map(torch.Tensor.get_device, out)) != devices
+                    or not (dense and all(map(torch.Tensor.is_contiguous, out)) or all(o.stride() == t.stride() for o, t in zip(out, grads)))):
                 raise _lib.GeodiffError("clip_grad_norm: out needs a tensor of the same shape, strides, dtype and device for each gradient")
-            dst = (ctypes.c_void_p * n)(*[t.data_ptr() for t in out])
+            dst = (ctypes.c_void_p * n)(*map(torch.Tensor.data_ptr, out))
+        torch._C._increment_version(grads if out is None else out)       # what autograd saved of them is no longer what it was
+    where = grads[0].device
     nbytes = lib.gd_grad_norm_workspace_bytes()
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=grads[0].device)
-    norm = torch.empty((), dtype=torch.float32, device=grads[0].device)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=where)
+    norm = torch.empty((), dtype=torch.float32, device=where)
     _launch(lib.gd_grad_norm, "gd_grad_norm", dev, src, dst, numel, dts, n, int(norm_type != 2.0), max_norm or 0.0, ws.data_ptr(), nbytes, norm.data_ptr())
     return norm
 

@@ -354,7 +354,8 @@ class BasicTransformerBlock(nn.Module):
             return False
         norms = (self.norm1, self.norm2, self.norm3)
         return (any(p.requires_grad for n_ in norms for p in n_.parameters())
-                and all(type(n_) is nn.LayerNorm and not (n_._forward_hooks or n_._forward_pre_hooks or n_._backward_hooks) for n_ in norms)
+                and all(type(n_) is nn.LayerNorm and "forward" not in n_.__dict__
+                        and not (n_._forward_hooks or n_._forward_pre_hooks or n_._backward_hooks or n_._backward_pre_hooks) for n_ in norms)
                 and all(p.dtype == x.dtype and p.device == x.device and p.is_contiguous() for n_ in norms for p in n_.parameters()))
 
 

@@ -146,6 +146,18 @@ def test_embedding_gradient_of_every_run_length(ops, n, seed):
 
 
 @gpu
+@pytest.mark.parametrize("n,V", [(900, 1 << 21), (2000, (1 << 20) + 7), (2000, (1 << 20) - 1), (4097, 255), (4096, 256), (5000, 65535), (5000, 65536), (30000, 3000001), (3000, (1 << 24) + 3)])
+def test_embedding_gradient_of_large_vocabularies(ops, n, V):
+    """Tokens of one to four bytes: as many passes of the sort, and the one-launch sort's limit on either side."""
+    g = _gen(n)
+    ids = torch.randint(0, V, (n,), generator=g)
+    ids[::3] = V - 1
+    ids[1::7] = ids[0]
+    _check_embed_bwd(ops, ids.to(DEV), _randn(g, n, 8), V)
+    _check_embed_bwd(ops, ids.to(DEV), _randn(g, n, 3, dtype=torch.float16), V, padding_idx=V - 1)
+
+
+@gpu
 @pytest.mark.parametrize("n", [6, 300, 9000])
 def test_embedding_gradient_skips_padding_and_foreign_ids(ops, n):
     g = _gen(n)
@@ -642,6 +654,39 @@ def test_clipping_refusals(ops):
             call()
             pytest.fail(str(i))
     assert float(t.sum()) == 24
+
+
+@gpu
+def test_calls_larger_than_the_cache(ops):
+    """Calls whose tensors exceed the memory-side cache store past it: the same bits as their rows give in a small call, or as torch's."""
+    g = torch.Generator(device=DEV).manual_seed(8)
+    r = lambda *s: torch.randn(*s, generator=g, device=DEV).bfloat16()
+    table = r(50000, 1024)
+    ids = torch.randint(0, 50000, (1700, 77), generator=g, device=DEV)
+    y = ops.embed_tokens(ids, table)
+    assert (y.numel() + table.numel()) * 2 > 1 << 28 and bool((y == table[ids]).all())
+    del y, table
+    ids = torch.randint(0, 300000, (2500,), generator=g, device=DEV)
+    _check_embed_bwd(ops, ids, r(2500, 512), 300000)
+    x, res, gy, gs = (r(2, 20000, 1280) for _ in range(4))
+    gate, pre, post = r(2, 1280), ops.Norm("layer", r(1280), r(1280)), ops.Norm("rms", r(1280))
+    s, y, st = ops.block_norm(x, res, pre, post, gate, 0.5)
+    d = ops.block_norm_bwd(x, res, gy, gs, st, pre, post, gate, 0.5)
+    cut = lambda t: t[:, 300:420].contiguous()
+    s2, y2, st2 = ops.block_norm(cut(x), cut(res), pre, post, gate, 0.5)
+    d2 = ops.block_norm_bwd(cut(x), cut(res), cut(gy), cut(gs), st2, pre, post, gate, 0.5)
+    assert torch.equal(cut(s), s2) and torch.equal(cut(y), y2) and torch.equal(cut(d["dx"]), d2["dx"]) and torch.equal(cut(d["dres"]), d2["dres"])
+    del x, res, gy, gs, s, y, d
+    grads = [r(9000, 9000), r(77), r(8191 * 8191)]
+    out = [torch.zeros_like(t) for t in grads]
+    n = ops.clip_grad_norm(grads, 2.0, out=out)
+    total = float(_norm_ref(grads))
+    assert abs(float(n) - total) <= 2 * U32 * total
+    for t, o in zip(grads, out):
+        _close(o, t.double() * (2.0 / (total + 1e-6)), 2, t.double().abs() * (2.0 / total))
+    v = grads[0]._version
+    ops.clip_grad_norm(grads, 2.0)
+    assert all(torch.equal(t, o) for t, o in zip(grads, out)) and grads[0]._version > v
 
 
 # ------------------------------------------------------------------------------------------------ streams, graphs
