@@ -526,26 +526,37 @@ __global__ void __launch_bounds__(256) k_embed_bwd_sum(const em_sum a, const T* 
 // tail).  The second launch adds those, one for each group.  All rows are read whole: a CU has a bounded number of cache lines on their way.
 #define EM_GROUP 64
 
-// rows [lo, hi) of `rows`, channel c: 16 at a time (behind the last: the first again, adding nothing)
-__device__ __forceinline__ float em_rows(const float* __restrict__ rows, long long lo, long long hi, long long step, int C, int c) {
-    float s = 0.f;
-    for (long long k = lo; k < hi; k += 16 * step) {
-        float v[16];
+template <int W> struct alignas(4 * W) em_sums { float v[W]; };
+
+// sum of rows lo, lo + step, .. below hi of `rows`, channels c .. c + W - 1, added to s: 8 rows at a time (behind the last: the first again,
+// adding nothing)
+template <int W>
+__device__ __forceinline__ void em_rows(em_sums<W>& s, const float* __restrict__ rows, long long lo, long long hi, long long step, int C, int c) {
+    for (long long k = lo; k < hi; k += 8 * step) {
+        em_sums<W> v[8];
 #pragma unroll
-        for (int j = 0; j < 16; ++j) v[j] = rows[(k + j * step < hi ? k + j * step : lo) * C + c];
+        for (int j = 0; j < 8; ++j) v[j] = *(const em_sums<W>*)(rows + (k + j * step < hi ? k + j * step : lo) * C + c);
 #pragma unroll
-        for (int j = 0; j < 16; ++j) s += k + j * step < hi ? v[j] : 0.f;
+        for (int j = 0; j < 8; ++j)
+#pragma unroll
+            for (int i = 0; i < W; ++i) s.v[i] += k + j * step < hi ? v[j].v[i] : 0.f;
     }
-    return s;
+}
+
+template <typename T, int W>
+__device__ __forceinline__ void em_write_row(T* __restrict__ p, const em_sums<W>& s, float scale) {
+#pragma unroll
+    for (int i = 0; i < W; ++i) p[i] = to_storage<T>(s.v[i] * scale);
 }
 
 // whether the run of `key` has begun before tile u and goes on into it (the entries are sorted; u in range)
 __device__ __forceinline__ bool em_into(const em_sum& a, long long u, uint32_t key) { return u > 0 && a.key[u * a.tile - 1] == key && a.key[u * a.tile] == key; }
 
-template <typename T>
+// W: channels a thread (4 where C is a multiple of 4, else 1)
+template <typename T, int W>
 __global__ void __launch_bounds__(256) k_embed_bwd_join(const em_sum a, T* __restrict__ dtable) {
     const int lane = threadIdx.x & 63, C = a.C;
-    const int wide = (C + 255) / 256, groups = a.tiles > EM_GROUP ? (a.tiles + EM_GROUP - 1) / EM_GROUP : 0;
+    const int wide = (C + 256 * W - 1) / (256 * W), groups = a.tiles > EM_GROUP ? (a.tiles + EM_GROUP - 1) / EM_GROUP : 0;
     if ((int)blockIdx.x >= groups * wide) {
         const int t = blockIdx.x - groups * wide;            // (a run of three tiles begins in front of the last two)
         const long long e1 = (long long)(t + 1) * a.tile, q = (t / EM_GROUP + 1) * EM_GROUP;
@@ -554,28 +565,40 @@ __global__ void __launch_bounds__(256) k_embed_bwd_join(const em_sum a, T* __res
         if (key >= a.vocab || in_tile != key || behind != key || before == key || crosses) return;
         const long long u = (long long)t + 1 + lane;
         const int more = __builtin_ctzll(~__ballot(u < a.tiles && u < q && a.key[u * a.tile] == key));
-        for (int c = threadIdx.x; c < C; c += 256)
-            dtable[(long long)key * C + c] = to_storage<T>((a.tail[(long long)t * C + c] + em_rows(a.head, t + 1, t + 1 + more, 1, C, c)) * a.scale);
+        for (int c = threadIdx.x * W; c < C; c += 256 * W) {
+            em_sums<W> s = *(const em_sums<W>*)(a.tail + (long long)t * C + c);
+            em_rows<W>(s, a.head, t + 1, t + 1 + more, 1, C, c);
+            em_write_row<T, W>(dtable + (long long)key * C + c, s, a.scale);
+        }
         return;
     }
-    const int c = blockIdx.x / groups * 256 + threadIdx.x;
+    const int c = (blockIdx.x / groups * 256 + threadIdx.x) * W;
     const long long q = (long long)(blockIdx.x % groups) * EM_GROUP, q2 = q + EM_GROUP, u = q + lane;
     const uint32_t key = a.key[q * a.tile];
     if (q > 0 && key < a.vocab && a.key[q * a.tile - 1] == key) {
         const unsigned long long on = __ballot(u < a.tiles && a.key[u * a.tile] == key);
         const int m = ~on ? __builtin_ctzll(~on) : 64;
-        if (m > 1 && c < C) a.head[q * C + c] = em_rows(a.head, q, q + m, 1, C, c);
+        if (m > 1 && c < C) {
+            em_sums<W> s = {};
+            em_rows<W>(s, a.head, q, q + m, 1, C, c);
+            *(em_sums<W>*)(a.head + q * C + c) = s;
+        }
     }
     if (q2 >= a.tiles) return;
     const uint32_t key2 = a.key[q2 * a.tile];
     if (key2 >= a.vocab || a.key[q2 * a.tile - 1] != key2 || (q > 0 && a.key[q * a.tile - 1] == key2)) return;
     const int m = __popcll(__ballot(em_into(a, u, key2)));  // the group's last m tiles (not its first: the run begins behind that one's start)
-    if (m > 0 && c < C) a.tail[(q2 - 1 - m) * C + c] += em_rows(a.head, q2 - m, q2, 1, C, c);
+    if (m > 0 && c < C) {
+        float* const tail = a.tail + (q2 - 1 - m) * C + c;
+        em_sums<W> s = *(const em_sums<W>*)tail;
+        em_rows<W>(s, a.head, q2 - m, q2, 1, C, c);
+        *(em_sums<W>*)tail = s;
+    }
 }
 
-template <typename T>
+template <typename T, int W>
 __global__ void __launch_bounds__(256) k_embed_bwd_join_groups(const em_sum a, T* __restrict__ dtable) {
-    const int lane = threadIdx.x & 63, C = a.C, c = blockIdx.y * 256 + threadIdx.x;
+    const int lane = threadIdx.x & 63, C = a.C, c = (blockIdx.y * 256 + threadIdx.x) * W;
     const long long q = (long long)(blockIdx.x + 1) * EM_GROUP, g = q - EM_GROUP;
     const uint32_t key = a.key[q * a.tile], behind = q + 1 < a.tiles ? a.key[(q + 1) * a.tile] : 0xffffffffu;
     if (key >= a.vocab || a.key[q * a.tile - 1] != key || (g > 0 && a.key[g * a.tile - 1] == key)) return;
@@ -590,7 +613,18 @@ __global__ void __launch_bounds__(256) k_embed_bwd_join_groups(const em_sum a, T
             break;
         }
     }
-    if (c < C) dtable[(long long)key * C + c] = to_storage<T>((a.tail[(q - 1 - m) * C + c] + em_rows(a.head, q, q + groups * EM_GROUP, EM_GROUP, C, c)) * a.scale);
+    if (c < C) {
+        em_sums<W> s = *(const em_sums<W>*)(a.tail + (q - 1 - m) * C + c);
+        em_rows<W>(s, a.head, q, q + groups * EM_GROUP, EM_GROUP, C, c);
+        em_write_row<T, W>(dtable + (long long)key * C + c, s, a.scale);
+    }
+}
+
+template <typename T, int W>
+static void em_join(const em_sum& a, T* dtable, hipStream_t st) {
+    const unsigned wide = (unsigned)((a.C + 256 * W - 1) / (256 * W)), groups = (unsigned)((a.tiles + EM_GROUP - 1) / EM_GROUP);
+    if (a.tiles > 2) k_embed_bwd_join<T, W><<<(a.tiles - 2) + (groups > 1 ? groups * wide : 0), 256, 0, st>>>(a, dtable);
+    if (groups > 1) k_embed_bwd_join_groups<T, W><<<dim3(groups - 1, wide), 256, 0, st>>>(a, dtable);
 }
 
 // dP is the column sum of dy as a [B, L * C] matrix.  A thread has one word (16 bytes; VEC) or element of a row and adds EM_POS_ROWS sequences
@@ -755,19 +789,7 @@ extern "C" int gd_embed_bwd(const void* ids, int ids64, int64_t n, const void* d
         }
         const em_sum a = {k.key, k.pos, (const unsigned char*)(ws + p.there), (float*)(ws + p.head), (float*)(ws + p.tail), n, p.tile, p.tiles, slices, C, (unsigned)vocab, scale, past, zero_rows, shift};
         EM_LAUNCH(dtype, vec, (k_embed_bwd_sum<T, VEC><<<(unsigned)grid, 256, 0, st>>>(a, (const T*)dy, (T*)dtable)));
-        const unsigned wide = (unsigned)((C + 255) / 256), groups = (unsigned)((p.tiles + EM_GROUP - 1) / EM_GROUP);
-        if (p.tiles > 2) {
-            const unsigned joins = (p.tiles - 2) + (groups > 1 ? groups * wide : 0);
-            if (dtype == GD_F32) k_embed_bwd_join<float><<<joins, 256, 0, st>>>(a, (float*)dtable);
-            else if (dtype == GD_F16) k_embed_bwd_join<f16_t><<<joins, 256, 0, st>>>(a, (f16_t*)dtable);
-            else k_embed_bwd_join<bf16_t><<<joins, 256, 0, st>>>(a, (bf16_t*)dtable);
-        }
-        if (groups > 1) {
-            const dim3 joins(groups - 1, wide);
-            if (dtype == GD_F32) k_embed_bwd_join_groups<float><<<joins, 256, 0, st>>>(a, (float*)dtable);
-            else if (dtype == GD_F16) k_embed_bwd_join_groups<f16_t><<<joins, 256, 0, st>>>(a, (f16_t*)dtable);
-            else k_embed_bwd_join_groups<bf16_t><<<joins, 256, 0, st>>>(a, (bf16_t*)dtable);
-        }
+        EM_LAUNCH(dtype, C % 4 == 0, (em_join<T, VEC ? 4 : 1>(a, (T*)dtable, st)));
     }
     GD_CHECK_LAUNCH("gd_embed_bwd");
     return GD_OK;
