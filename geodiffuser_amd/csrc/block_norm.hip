@@ -153,13 +153,12 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) k_block_norm(const gd_b
     if (a.gate) gate.load((const T*)a.gate + (a.rows_per_gate == a.rows ? 0 : row / a.rows_per_gate) * a.gate_ld, t, C);
     if (a.pre_gamma) eg.load((const T*)a.pre_gamma, t, C);
     if (a.pre_beta) eb.load((const T*)a.pre_beta, t, C);
-    float h[N];
+    float h[N], mean = 0.f, r = 1.f;
 #pragma unroll
     for (int i = 0; i < N; ++i) h[i] = x[i];
+    if (a.post_kind) bn_stats<PART, TPR, N>(h, t, C, a.post_kind, a.post_eps, lds, turn, mean, r);
+    if (a.stats && t == 0) { a.stats[row * 4] = mean; a.stats[row * 4 + 1] = r; }
     if (a.post_kind) {
-        float mean, r;
-        bn_stats<PART, TPR, N>(h, t, C, a.post_kind, a.post_eps, lds, turn, mean, r);
-        if (a.stats && t == 0) { a.stats[row * 4] = mean; a.stats[row * 4 + 1] = r; }
 #pragma unroll
         for (int i = 0; i < N; ++i) h[i] = PART::col(t, i) < C ? (h[i] - mean) * r : 0.f;
         if (a.post_gamma) {
@@ -180,10 +179,11 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) k_block_norm(const gd_b
         for (int i = 0; i < N; ++i) h[i] = __builtin_fmaf(a.res_scale, res[i], h[i]);
     }
     if (a.s) PART::store((T*)a.s + row * C, t, C, h, stream);
-    if (!a.pre_kind) return;
-    float mean, r;
-    bn_stats<PART, TPR, N>(h, t, C, a.pre_kind, a.pre_eps, lds, turn, mean, r);
+    mean = 0.f;
+    r = 1.f;
+    if (a.pre_kind) bn_stats<PART, TPR, N>(h, t, C, a.pre_kind, a.pre_eps, lds, turn, mean, r);
     if (a.stats && t == 0) { a.stats[row * 4 + 2] = mean; a.stats[row * 4 + 3] = r; }
+    if (!a.pre_kind) return;
 #pragma unroll
     for (int i = 0; i < N; ++i) h[i] = (h[i] - mean) * r;
     if (a.pre_gamma) {

@@ -49,6 +49,10 @@ class _TextLayer(nn.Module):
         self.fc1, self.fc2 = nn.Linear(d, 4 * d), nn.Linear(4 * d, d)
 
     def forward(self, x, mask):
+        if training.fuses_norms(x, (self.ln1, self.ln2)):    # a pass that learns them: residual add and norms fused, with their gradients
+            x, h = training.block_norm(x, None, training.layer_norm_of(self.ln1))
+            x, h = training.block_norm(self.attn(h, h, h, attn_mask=mask, need_weights=False)[0].contiguous(), x, training.layer_norm_of(self.ln2))
+            return x + self.fc2(F.gelu(self.fc1(h)))
         h = self.ln1(x)
         x = x + self.attn(h, h, h, attn_mask=mask, need_weights=False)[0]
         return x + self.fc2(F.gelu(self.fc1(self.ln2(x))))

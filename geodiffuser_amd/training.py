@@ -68,6 +68,22 @@ def block_norm(x, res, pre: Optional[Norm], post: Optional[Norm] = None, gate=No
                               pre and (pre.kind, pre.eps), post and (post.kind, post.eps), res_scale)
 
 
+def fuses_norms(x, norms) -> bool:
+    """Whether a pass over x differentiates w.r.t. the weights of these norms and ``block_norm`` takes them: affine nn.LayerNorms of x's dtype and
+    device that nothing (a hook, a replaced ``forward``, autocast) makes into something else.  Norms that do not learn keep their path."""
+    if not (torch.is_grad_enabled() and x.is_cuda and x.is_contiguous() and x.shape[-1] <= 16384 and x.numel() > 0
+            and x.dtype in (torch.float16, torch.bfloat16, torch.float32) and not torch.is_autocast_enabled()):
+        return False
+    return (any(p.requires_grad for n in norms for p in n.parameters())
+            and all(type(n) is torch.nn.LayerNorm and "forward" not in n.__dict__
+                    and not (n._forward_hooks or n._forward_pre_hooks or n._backward_hooks or n._backward_pre_hooks) for n in norms)
+            and all(p.dtype == x.dtype and p.device == x.device and p.is_contiguous() for n in norms for p in n.parameters()))
+
+
+def layer_norm_of(module: torch.nn.LayerNorm) -> Norm:
+    return Norm("layer", module.weight, module.bias, module.eps)
+
+
 def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: float, norm_type: float = 2.0):
     """torch.nn.utils.clip_grad_norm_ on ``ops.clip_grad_norm``: scales the parameters' gradients in place so that their joint norm is at most
     ``max_norm`` -> the norm before (0-d tensor on the device, nothing is synchronised; 0 if no parameter has a gradient)."""

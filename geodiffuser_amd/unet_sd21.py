@@ -334,29 +334,18 @@ class BasicTransformerBlock(nn.Module):
             a = self.attn2(h, encoder_hidden_states=ctx)
             x, h = _AddLayerNormFn.apply(a.contiguous(), x, self.norm3.weight, self.norm3.bias, self.norm3.eps)
             return self.ff(h) + x
-        if self._learning_norms(x):
-            # norms that learn: the same fusion with gradients for gamma / beta too
-            from . import training
-            norm = [training.Norm("layer", n_.weight, n_.bias, n_.eps) for n_ in (self.norm1, self.norm2, self.norm3)]
-            x, h = training.block_norm(x, None, norm[0])
-            x, h = training.block_norm(self.attn1(h).contiguous(), x, norm[1])
-            x, h = training.block_norm(self.attn2(h, encoder_hidden_states=ctx).contiguous(), x, norm[2])
-            return self.ff(h) + x
+        if FUSED and _DBG["GD_FUSE_TF"] and torch.is_grad_enabled():
+            from . import training as tr
+            if tr.fuses_norms(x, (self.norm1, self.norm2, self.norm3)):
+                # norms that learn: the same fusion with gradients for gamma / beta too
+                x, h = tr.block_norm(x, None, tr.layer_norm_of(self.norm1))
+                x, h = tr.block_norm(self.attn1(h).contiguous(), x, tr.layer_norm_of(self.norm2))
+                x, h = tr.block_norm(self.attn2(h, encoder_hidden_states=ctx).contiguous(), x, tr.layer_norm_of(self.norm3))
+                return self.ff(h) + x
         x = self.attn1(self.norm1(x)) + x
         x = self.attn2(self.norm2(x), encoder_hidden_states=ctx) + x
         x = self.ff(self.norm3(x)) + x
         return x
-
-    def _learning_norms(self, x):
-        """Whether a pass differentiates w.r.t. norm weights that gd_block_norm takes: affine nn.LayerNorms of x's dtype and device, no hooks."""
-        if not (FUSED and _DBG["GD_FUSE_TF"] and torch.is_grad_enabled() and x.is_cuda and x.is_contiguous() and x.shape[-1] <= 16384
-                and x.dtype in (torch.float16, torch.bfloat16, torch.float32) and not torch.is_autocast_enabled()):
-            return False
-        norms = (self.norm1, self.norm2, self.norm3)
-        return (any(p.requires_grad for n_ in norms for p in n_.parameters())
-                and all(type(n_) is nn.LayerNorm and "forward" not in n_.__dict__
-                        and not (n_._forward_hooks or n_._forward_pre_hooks or n_._backward_hooks or n_._backward_pre_hooks) for n_ in norms)
-                and all(p.dtype == x.dtype and p.device == x.device and p.is_contiguous() for n_ in norms for p in n_.parameters()))
 
 
 class Transformer2DModel(nn.Module):

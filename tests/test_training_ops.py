@@ -432,6 +432,25 @@ def test_block_norm_hard_values(ops, kind, C):
 
 
 @gpu
+def test_block_norm_beyond_32_bits(ops):
+    """Tensors of more than 2^31 elements: the rows behind that border have the bits that a call on them alone gives."""
+    R, C = (1 << 21) + 40, 1024
+    x = torch.zeros(R, C, dtype=torch.bfloat16, device=DEV)
+    tail = _randn(_gen(1), 50, C, dtype=torch.bfloat16)
+    x[-50:] = tail
+    n = ops.Norm("layer", _randn(_gen(2), C, dtype=torch.bfloat16), None)
+    s, y, st = ops.block_norm(x, x, n)
+    s2, y2, st2 = ops.block_norm(tail, tail, n)
+    assert torch.equal(s[-50:], s2) and torch.equal(y[-50:], y2) and torch.equal(st[-50:], st2) and not bool(y[:50].any())
+    del s, y
+    d = ops.block_norm_bwd(x, x, x, None, st, n, need=["dx", "dpre_gamma"])
+    d2 = ops.block_norm_bwd(tail, tail, tail, None, st2, n, need=["dx", "dpre_gamma"])
+    assert torch.equal(d["dx"][-50:], d2["dx"])
+    m = (tail.double().abs() * (y2.double().abs() + 1)).sum(0)
+    _close(d["dpre_gamma"], d2["dpre_gamma"].double(), 2 * (2 * K_ROW + 50) + 2 ** 17, m)      # each rounds to bf16 once: 2^17 2^-24 = one step of bf16
+
+
+@gpu
 def test_block_norm_need_and_empty(ops):
     x, r, pre, po, gt, gy, gs = _block_case(ops, (2, 33, 64), torch.float32, "layer", "sample", True, True, 5)
     _, _, stats = ops.block_norm(x, r, pre, po, gt)
@@ -479,6 +498,35 @@ def test_block_norm_against_differences(ops):
     noise = float((gs.double().abs() * mf["s"]).sum() + (gy.double().abs() * mf["y"]).sum())
     # (x + h d rounds too, by one step: 2 K_ROW covers it; 4: the magnitudes at the moved points)
     assert abs((loss(h, False) - loss(-h, False)) - (loss(h, True) - loss(-h, True))) <= 2 * 4 * 2 * K_ROW * U32 * noise
+
+
+def test_norm_and_embedding_refusals_on_the_host():
+    """The library's own checks, with addresses that are never followed."""
+    from geodiffuser_amd import _lib
+    lib = _lib.load()
+    A = 1 << 20
+    ok = dict(x=A, res=A, gate=0, y=A, s=A, stats=A, rows=8, rows_per_gate=8, gate_ld=64, C=64, pre_kind=1, res_scale=1.0)
+    bad = [dict(x=0), dict(rows=0), dict(C=0), dict(C=16385), dict(pre_kind=3), dict(post_kind=-1), dict(gate=A, rows_per_gate=3), dict(gate=A, gate_ld=8), dict(gate=A, rows_per_gate=0),
+           dict(s=0, y=0, pre_kind=0), dict(pre_kind=0), dict(y=0), dict(rows=1 << 31), dict(gate=A, rows=1 << 17, rows_per_gate=1)]
+    for b in bad:
+        assert lib.gd_block_norm(ctypes.byref(_lib.GdBlockNorm(**{**ok, **b})), 2, None) < 0, b
+    assert lib.gd_block_norm(ctypes.byref(_lib.GdBlockNorm(**ok)), 3, None) == -1 and lib.gd_block_norm(None, 2, None) == -1
+
+    def bwd(f=None, ws=1 << 24, **k):
+        return lib.gd_block_norm_bwd(ctypes.byref(_lib.GdBlockNormBwd(f=_lib.GdBlockNorm(**{**ok, **(f or {})}), **k)), ctypes.c_void_p(A), ws, 2, None)
+
+    for k in (dict(), dict(gy=A, f=dict(stats=0)), dict(gy=A, f=dict(pre_kind=0)), dict(gs=A, dpre_gamma=A), dict(gy=A, dpost_gamma=A), dict(gy=A, dgate=A), dict(gy=A, dres=A, f=dict(res=0)),
+              dict(gs=A, f=dict(post_kind=2, stats=0))):
+        assert bwd(**k) == -1, k
+    assert bwd(gy=A, dpre_gamma=A, ws=8) == -2
+    nb = lib.gd_embed_bwd_workspace_bytes(5000, 100, 64)
+    assert lib.gd_embed_bwd_workspace_bytes(1024, 100, 64) == 0 and nb > 5000 * 16
+    E = lambda n=5000, vocab=100, C=64, ids=A, ws=nb, dt=2: lib.gd_embed_bwd(ctypes.c_void_p(ids), 1, n, ctypes.c_void_p(A), vocab, C, -1, 1.0, ctypes.c_void_p(A), ctypes.c_void_p(A), ws, dt, None)
+    assert E(n=-1) == -4 and E(n=1 << 30) == -4 and E(vocab=0) == -4 and E(C=0) == -4 and E(ids=0) == -1 and E(ws=nb - 1) == -2 and E(dt=5) == -1
+    assert lib.gd_embed(ctypes.c_void_p(A), 1, 0, ctypes.c_void_p(A), 10, None, 1, 8, 1.0, ctypes.c_void_p(A), 2, None) == -1
+    assert lib.gd_embed(ctypes.c_void_p(A), 1, 4, ctypes.c_void_p(A), 10, ctypes.c_void_p(A), 0, 8, 1.0, ctypes.c_void_p(A), 2, None) == -1
+    assert lib.gd_embed_pos_bwd(ctypes.c_void_p(A), 4, 8, 8, 7, ctypes.c_void_p(A), None, 0, 2, None) == -1
+    assert lib.gd_embed_pos_bwd(ctypes.c_void_p(A), 4096, 8, 8, 8, ctypes.c_void_p(A), None, 0, 2, None) == -2
 
 
 def test_block_norm_refuses_cpu_tensors():
@@ -808,6 +856,51 @@ def test_transformer_block_with_trainable_norms(ops, dtype):
             assert rel(p.grad, q.grad) < u, (n, rel(p.grad, q.grad), u)
         else:
             assert p.grad is None
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_text_tower_learns_end_to_end(ops, dtype):
+    """Every gradient of a two-layer tower (embedding, positions, norms on the operators; attention and projections on torch) against the same
+    tower on the CPU in 64 bits, in relative 2-norm, and clipping of all of them.  Both sides round every intermediate tensor; fewer than 60
+    such roundings of u relative lie on a path through two layers forward and back (bf16; each of torch's f32 products adds at most a few
+    2^-24 sqrt(256) of its own, so that f32 gets 60 * 16 of them)."""
+    import copy
+    from geodiffuser_amd import training as T
+    from geodiffuser_amd.pipeline import TextEncoder
+    torch.manual_seed(5)
+    te = TextEncoder(width=64, layers=2, heads=2, vocab=120, max_len=20).to(DEV, dtype)
+    for n, p in te.named_parameters():
+        if "ln" in n:
+            p.data.add_(_randn(_gen(len(n)), *p.shape, std=0.2).to(dtype))
+    ids = torch.randint(0, 120, (3, 17), generator=_gen(2))
+    ids[:, 9:] = 0
+    w = _randn(_gen(3), 3, 17, 64, dtype=dtype)
+    calls = []
+    saved = ops.block_norm, ops.embed_tokens
+    ops.block_norm = lambda *a, **k: calls.append("norm") or saved[0](*a, **k)
+    ops.embed_tokens = lambda *a, **k: calls.append("embed") or saved[1](*a, **k)
+    try:
+        y = te(ids.to(DEV))[0]
+        (y.float() * w.float()).sum().backward()
+    finally:
+        ops.block_norm, ops.embed_tokens = saved
+    assert calls == ["embed"] + ["norm"] * 4
+    ref = copy.deepcopy(te).cpu().double()
+    ref.zero_grad()
+    yr = ref(ids)[0]
+    (yr * w.cpu().double()).sum().backward()
+    u = 60 * (16 * U32 if dtype == torch.float32 else torch.finfo(dtype).eps / 2)
+    rel = lambda a, b: float((a.detach().cpu().double() - b.detach()).norm() / b.detach().norm())
+    assert rel(y, yr) < u
+    for (n, p), q in zip(te.named_parameters(), ref.parameters()):
+        # (the key's bias has no gradient: softmax does not see it, so that only rounding is left there)
+        a, b = (p.grad[:64], q.grad[:64]) if n.endswith("in_proj_bias") else (p.grad, q.grad)
+        assert rel(a, b) < u, (n, rel(a, b), u)
+    total = math.sqrt(sum(float(p.grad.double().square().sum()) for p in te.parameters()))
+    norm = T.clip_grad_norm_(te.parameters(), total / 3)
+    after = math.sqrt(sum(float(p.grad.double().square().sum()) for p in te.parameters()))
+    assert abs(float(norm) - total) <= 2 * U32 * total and abs(after - total / 3) <= (4 * U32 + (0 if dtype == torch.float32 else torch.finfo(dtype).eps / 2)) * total / 3
 
 
 @gpu
