@@ -632,25 +632,36 @@ static void em_join(const em_sum& a, T* dtable, hipStream_t st) {
 // more than one.
 #define EM_POS_ROWS 64
 
+template <typename T, int N, bool NT>
+__device__ __forceinline__ void em_column(const T* p, long long width, long long b0, long long b1, float* acc) {
+    for (long long b = b0; b < b1; b += 8) {
+        em_piece<T, N> w[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const T* at = p + (b + j < b1 ? b + j : b0) * width;
+            if constexpr (NT) w[j] = __builtin_bit_cast(em_piece<T, N>, __builtin_nontemporal_load((const u32x4*)at));
+            else w[j] = *(const em_piece<T, N>*)at;
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+#pragma unroll
+            for (int i = 0; i < N; ++i) acc[i] += b + j < b1 ? (float)w[j].v[i] : 0.f;
+    }
+}
+
+// stream: dy is larger than the memory-side cache: it is read past it, so that the part which the table's gradient has left there is
+// still there when its turn comes
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(256) k_embed_pos_bwd(const T* __restrict__ dy, long long B, long long width, long long out_width, long long per, float* __restrict__ part,
-                                                       T* __restrict__ dpos) {
+__global__ void __launch_bounds__(256) k_embed_pos_bwd(const T* __restrict__ dy, long long B, long long width, long long out_width, long long per, bool stream,
+                                                       float* __restrict__ part, T* __restrict__ dpos) {
     constexpr int N = VEC ? word16<T>::N : 1;
     const long long at = ((long long)blockIdx.x * 256 + threadIdx.x) * N;
     if (at >= out_width) return;
     float acc[N] = {};
     if (at < width) {
         const long long b0 = (long long)blockIdx.y * per, b1 = b0 + per < B ? b0 + per : B;
-        const T* p = dy + at;
-        for (long long b = b0; b < b1; b += 8) {
-            em_piece<T, N> w[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) w[j] = *(const em_piece<T, N>*)(p + (b + j < b1 ? b + j : b0) * width);
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-#pragma unroll
-                for (int i = 0; i < N; ++i) acc[i] += b + j < b1 ? (float)w[j].v[i] : 0.f;
-        }
+        if (VEC && stream) em_column<T, N, VEC>(dy + at, width, b0, b1, acc);
+        else em_column<T, N, false>(dy + at, width, b0, b1, acc);
     }
     if (part) {
         if (at < width) {
@@ -825,7 +836,8 @@ extern "C" int gd_embed_pos_bwd(const void* dy, int64_t B, int L, int C, int pos
     GD_REQUIRE((out_width + 255) / 256 < (1ll << 31), GD_EUNSUPPORTED, "gd_embed_pos_bwd: too many positions for this width");
     float* const part = parts > 1 ? (float*)workspace : nullptr;
     hipStream_t st = as_stream(stream);
-    EM_LAUNCH(dtype, vec, (k_embed_pos_bwd<T, VEC><<<dim3((unsigned)grid, parts), 256, 0, st>>>((const T*)dy, B, width, out_width, per, part, (T*)dpos)));
+    EM_LAUNCH(dtype, vec, (k_embed_pos_bwd<T, VEC><<<dim3((unsigned)grid, parts), 256, 0, st>>>((const T*)dy, B, width, out_width, per,
+                      streams_past_cache((double)B * width * EM_ELEM(dtype)), part, (T*)dpos)));
     if (parts > 1) {
         const unsigned g = (unsigned)((out_width + 255) / 256);
         if (dtype == GD_F32) k_embed_pos_join<float><<<g, 256, 0, st>>>(part, parts, width, out_width, (float*)dpos);
