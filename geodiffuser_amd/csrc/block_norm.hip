@@ -16,6 +16,10 @@
 // both norms cost no second read.  Everything between the loads and the one rounding of each result is binary32; y comes from the sum s
 // BEFORE its rounding, and the backward recomputes that sum from x and res instead of reading the rounded s: the gradients are those of
 // the function that the forward computed, at the same traffic.
+//
+// Measured (MI355X; a large copy moves 4.9 TB/s): 32768 x 1280 f32, rms norms on both sides, a gate for each sample: forward 125 us
+// (671 MB, 5.4 TB/s), backward 194 us (1.0 GB, 5.2 TB/s) + 7 us for the column sums.  4096 x 640 bf16, one layer norm, one gate: 7.8, 14.6 and
+// 3.9 us (the data lie in the caches: the chain of loads and sums of a few rows a wave).  77 x 1024 bf16, forward: 3.9 us.
 #include "train_common.hpp"
 
 template <typename T> __device__ __forceinline__ uint32_t bits16(float x) {
@@ -198,6 +202,8 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) k_block_norm(const gd_b
 }
 
 // ---- backward -------------------------------------------------------------------------------------------------------------------------
+// Bound by HBM like the forward; a row's four loads are issued while the row before is worked on (without that, and with the parameters
+// loaded inside the loop, the f32 case above took 417 us: one row's latency after the other).
 // Workgroup w takes the rows [w * R, (w + 1) * R) in order; its threads keep the column sums of their channels in registers and leave
 // them in the workspace, one row of C floats for each sum: four sums over all rows (slot w) and the gate's, which ends wherever the rows
 // of one gate end.  Going through (w, gate row) in order, each step raises w or the gate row by one, so that slot w + gate row is
