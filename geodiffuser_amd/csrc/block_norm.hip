@@ -250,11 +250,17 @@ template <typename PART> struct bn_row {
     float stats[4];
 };
 
-// WRAP: there is a gate or a norm on x (their registers otherwise serve occupancy)
-template <typename T, int TPR, int N, bool VEC, bool WRAP>
+// WRAP: there is a gate or a norm on x (their registers otherwise serve occupancy).  SUMS: BN_ALL, or the two halves of a launch whose
+// column sums together do not fit the registers (WRAP above 4096 channels): BN_OUT writes dx, dres and sums for the norm in front of the
+// next block, BN_WRAP sums for the gate and the norm on x.  (2048 x 8192 bf16 with both: one launch 213 us, spilling, two 110.)
+enum { BN_ALL, BN_OUT, BN_WRAP };
+template <typename T, int TPR, int N, bool VEC, bool WRAP, int SUMS>
 __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) k_block_norm_bwd(const bn_bwd_args b) {
     using PART = bn_part<T, TPR, N, VEC>;
     constexpr int RPB = TPR < 256 ? 256 / TPR : 1;
+    // the next row's data beside this one's and the parameters over all rows, where the registers hold them: 8 waves and 16 channels a
+    // thread leave none
+    constexpr bool AHEAD = TPR * N < 8192;
     __shared__ float lds[TPR < 256 ? 4 * 64 * N : 64];
     int turn = 0;
     const gd_block_norm_bwd_t& a = b.a;
@@ -262,12 +268,15 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) k_block_norm_bwd(const 
     const long long r0 = (long long)blockIdx.x * b.rows_per_wg, r1 = r0 + b.rows_per_wg < a.f.rows ? r0 + b.rows_per_wg : a.f.rows;
     float pre_g[N] = {}, pre_b[N] = {}, post_g[N] = {}, post_b[N] = {}, dgate[N] = {};
     PART og, ob, eg, gate;
-    if (a.f.pre_gamma) eg.load((const T*)a.f.pre_gamma, t, C); else eg.fill(1.f);
-    if constexpr (WRAP) {
-        if (a.f.post_gamma) og.load((const T*)a.f.post_gamma, t, C); else og.fill(1.f);
-        if (a.f.post_beta) ob.load((const T*)a.f.post_beta, t, C); else ob.fill(0.f);
-        gate.fill(1.f);
-    }
+    const auto params = [&](long long gate_row) {
+        if (a.f.pre_gamma) eg.load((const T*)a.f.pre_gamma, t, C); else eg.fill(1.f);
+        if constexpr (WRAP) {
+            if (a.f.post_gamma) og.load((const T*)a.f.post_gamma, t, C); else og.fill(1.f);
+            if (a.f.post_beta) ob.load((const T*)a.f.post_beta, t, C); else ob.fill(0.f);
+            if (a.f.gate) gate.load((const T*)a.f.gate + gate_row * a.f.gate_ld, t, C); else gate.fill(1.f);
+        }
+    };
+    if (AHEAD) params(0);
     bn_row<PART> cur, next;
     long long held = -1;                                     // the row in `next`
     const auto fetch = [&](long long row) {
@@ -282,19 +291,25 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) k_block_norm_bwd(const 
         }
     };
     const long long per = WRAP && a.f.gate ? a.f.rows_per_gate : a.f.rows;
-    if (r0 + wave < r1) fetch(r0 + wave);
+    if (AHEAD && r0 + wave < r1) fetch(r0 + wave);
     for (long long g0 = r0; g0 < r1;) {
         const long long gate_row = per == a.f.rows ? 0 : g0 / per;
         const long long g1 = (gate_row + 1) * per < r1 ? (gate_row + 1) * per : r1;
-        if constexpr (WRAP) {
+        if constexpr (WRAP && AHEAD) {
             if (a.f.gate) gate.load((const T*)a.f.gate + gate_row * a.f.gate_ld, t, C);
         }
         for (long long row = g0 + wave; row < g1; row += RPB) {        // (TPR >= 256: the same rows for the whole workgroup)
-            if (held != row) fetch(row);                     // (a wave that had no row of the gate before)
+            if constexpr (!AHEAD) {
+                asm volatile("" ::: "memory");               // (else the parameters are held in registers over all rows, as floats)
+                params(gate_row);
+            }
+            if (!AHEAD || held != row) fetch(row);           // (held: not so for a wave that had no row of the gate before)
             cur = next;
-            // the row behind this one: of this gate, or the first of the next gate's rows
-            const long long then = row + RPB < g1 ? row + RPB : g1 + wave;
-            if (then < r1) fetch(then);
+            if constexpr (AHEAD) {
+                // the row behind this one: of this gate, or the first of the next gate's rows
+                const long long then = row + RPB < g1 ? row + RPB : g1 + wave;
+                if (then < r1) fetch(then);
+            }
             float d[N], sv[N], xh[N];
             // forward again: xh = normalised x, h = post(x), sv = the sum
             const float post_mean = WRAP && a.f.post_kind ? cur.stats[0] : 0.f, post_r = WRAP && a.f.post_kind ? cur.stats[1] : 1.f;
@@ -313,8 +328,10 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) k_block_norm_bwd(const 
                 for (int i = 0; i < N; ++i) {
                     sv[i] = PART::col(t, i) < C ? (sv[i] - mean) * r : 0.f;
                     const float g = cur.gy[i];
-                    pre_g[i] = __builtin_fmaf(g, sv[i], pre_g[i]);
-                    pre_b[i] += g;
+                    if constexpr (SUMS != BN_WRAP) {
+                        pre_g[i] = __builtin_fmaf(g, sv[i], pre_g[i]);
+                        pre_b[i] += g;
+                    }
                     d[i] = g * eg[i];
                     m[0] += d[i];
                     m[1] = __builtin_fmaf(d[i], sv[i], m[1]);
@@ -327,7 +344,7 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) k_block_norm_bwd(const 
 #pragma unroll
                 for (int i = 0; i < N; ++i) d[i] = cur.gs[i];
             }
-            if (a.dres) {
+            if (SUMS != BN_WRAP && a.dres) {
                 float w[N];
 #pragma unroll
                 for (int i = 0; i < N; ++i) w[i] = a.f.res_scale * d[i];
@@ -337,33 +354,37 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) k_block_norm_bwd(const 
                 float m[2] = {0.f, 0.f};
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
-                    dgate[i] = __builtin_fmaf(d[i], __builtin_fmaf(xh[i], og[i], ob[i]), dgate[i]);
+                    if constexpr (SUMS != BN_OUT) dgate[i] = __builtin_fmaf(d[i], __builtin_fmaf(xh[i], og[i], ob[i]), dgate[i]);
                     d[i] *= gate[i];
-                    post_g[i] = __builtin_fmaf(d[i], xh[i], post_g[i]);
-                    post_b[i] += d[i];
+                    if constexpr (SUMS != BN_OUT) {
+                        post_g[i] = __builtin_fmaf(d[i], xh[i], post_g[i]);
+                        post_b[i] += d[i];
+                    }
                     if (a.f.post_kind) {
                         d[i] *= og[i];
                         m[0] += d[i];
                         m[1] = __builtin_fmaf(d[i], xh[i], m[1]);
                     }
                 }
-                if (a.f.post_kind) {
+                if (SUMS != BN_WRAP && a.f.post_kind) {
                     bn_row_sum<TPR, 2>(m, lds, turn);
                     const float m0 = a.f.post_kind == GD_NORM_LAYER ? m[0] / (float)C : 0.f, m1 = m[1] / (float)C;
 #pragma unroll
                     for (int i = 0; i < N; ++i) d[i] = post_r * (d[i] - m0 - xh[i] * m1);
                 }
             }
-            if (a.dx) PART::store((T*)a.dx + row * C, t, C, d, b.stream);
+            if (SUMS != BN_WRAP && a.dx) PART::store((T*)a.dx + row * C, t, C, d, b.stream);
         }
-        if constexpr (WRAP) {
+        if constexpr (WRAP && SUMS != BN_OUT) {
             if (b.gate_sums) bn_flush<PART, TPR, N>(dgate, b.gate_sums + ((long long)blockIdx.x + gate_row) * C, C, lds);
         }
         g0 = g1;
     }
-    if (b.sums[BN_PRE_G]) bn_flush<PART, TPR, N>(pre_g, b.sums[BN_PRE_G] + (long long)blockIdx.x * C, C, lds);
-    if (b.sums[BN_PRE_B]) bn_flush<PART, TPR, N>(pre_b, b.sums[BN_PRE_B] + (long long)blockIdx.x * C, C, lds);
-    if constexpr (WRAP) {
+    if constexpr (SUMS != BN_WRAP) {
+        if (b.sums[BN_PRE_G]) bn_flush<PART, TPR, N>(pre_g, b.sums[BN_PRE_G] + (long long)blockIdx.x * C, C, lds);
+        if (b.sums[BN_PRE_B]) bn_flush<PART, TPR, N>(pre_b, b.sums[BN_PRE_B] + (long long)blockIdx.x * C, C, lds);
+    }
+    if constexpr (WRAP && SUMS != BN_OUT) {
         if (b.sums[BN_POST_G]) bn_flush<PART, TPR, N>(post_g, b.sums[BN_POST_G] + (long long)blockIdx.x * C, C, lds);
         if (b.sums[BN_POST_B]) bn_flush<PART, TPR, N>(post_b, b.sums[BN_POST_B] + (long long)blockIdx.x * C, C, lds);
     }
@@ -418,7 +439,7 @@ static bool bn_vec(const gd_block_norm_t& f, int elem) {
         else if ((C) <= 1024) X(64, 16);                                                                      \
         else if ((C) <= 2048) X(256, 8);                                                                      \
         else if ((C) <= 4096) X(512, 8);                                                                      \
-        else if ((C) <= 8192) X(512, 16);                                                                     \
+        else if ((C) <= 8192) X(1024, 8);                                                                     \
         else X(1024, 16);                                                                                     \
     } while (0)
 
@@ -490,14 +511,23 @@ static void bn_launch_bwd(const gd_block_norm_bwd_t& a, float* ws, hipStream_t s
         any |= dst[k] != nullptr;
     }
     b.gate_sums = a.dgate ? ws + (size_t)BN_SUMS * wg0 * a.f.C : nullptr;
-    const bool wrap = a.f.gate || a.f.post_kind;
+    const bool wrap = a.f.gate || a.f.post_kind, wrap_sums = a.dgate || a.dpost_gamma || a.dpost_beta;
     const bool vec = bn_vec(a.f, sizeof(T)) && bn_aligned(a.gy) && bn_aligned(a.gs) && bn_aligned(a.dx) && bn_aligned(a.dres);
 #define BN_GO(TPR, N)                                                                                         \
     do {                                                                                                      \
         constexpr int threads = TPR < 256 ? 256 : TPR;                                                        \
-        if (!vec) k_block_norm_bwd<T, TPR, N, false, true><<<wg, threads, 0, st>>>(b);                        \
-        else if (wrap) k_block_norm_bwd<T, TPR, N, true, true><<<wg, threads, 0, st>>>(b);                    \
-        else k_block_norm_bwd<T, TPR, N, true, false><<<wg, threads, 0, st>>>(b);                             \
+        if constexpr (TPR * N >= 8192) {                                                                      \
+            if (!vec) k_block_norm_bwd<T, TPR, N, false, true, BN_OUT><<<wg, threads, 0, st>>>(b);            \
+            else if (wrap) k_block_norm_bwd<T, TPR, N, true, true, BN_OUT><<<wg, threads, 0, st>>>(b);        \
+            else k_block_norm_bwd<T, TPR, N, true, false, BN_ALL><<<wg, threads, 0, st>>>(b);                 \
+            if (!wrap_sums) break;                                                                            \
+            if (!vec) k_block_norm_bwd<T, TPR, N, false, true, BN_WRAP><<<wg, threads, 0, st>>>(b);           \
+            else k_block_norm_bwd<T, TPR, N, true, true, BN_WRAP><<<wg, threads, 0, st>>>(b);                 \
+        } else {                                                                                              \
+            if (!vec) k_block_norm_bwd<T, TPR, N, false, true, BN_ALL><<<wg, threads, 0, st>>>(b);            \
+            else if (wrap) k_block_norm_bwd<T, TPR, N, true, true, BN_ALL><<<wg, threads, 0, st>>>(b);        \
+            else k_block_norm_bwd<T, TPR, N, true, false, BN_ALL><<<wg, threads, 0, st>>>(b);                 \
+        }                                                                                                     \
     } while (0)
     BN_SHAPE(a.f.C, BN_GO);
 #undef BN_GO
