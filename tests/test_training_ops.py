@@ -784,6 +784,92 @@ def test_training_ops_on_another_stream_and_replayed_in_graphs(ops):
             want = all_ops()
 
 
+@gpu
+def test_a_captured_training_step(ops):
+    """Forward, backward and clipping of embedding and block norm as one graph, replayed on new data between eager steps on leaves of their own."""
+    from geodiffuser_amd import training as T
+    g = _gen(21)
+    V, C = 400, 72
+    ids = torch.randint(0, V, (6, 77), generator=g).to(DEV)
+    data = dict(table=_randn(g, V, C), pos=_randn(g, 77, C), gate=_randn(g, 6, C), g1=_randn(g, C), b1=_randn(g, C), g2=_randn(g, C), w=_randn(g, 6, 77, C))
+
+    def step(d):
+        p = {k: d[k].detach().requires_grad_() for k in ("table", "pos", "gate", "g1", "b1", "g2")}
+        x = T.embed_tokens(ids, p["table"], p["pos"], 2.0)
+        s, y = T.block_norm(x, x, T.Norm("layer", p["g1"], p["b1"]), post=T.Norm("rms", p["g2"]), gate=p["gate"], res_scale=0.5)
+        grads = [t.contiguous() for t in torch.autograd.grad([s, y], list(p.values()), [d["w"], d["w"]])]
+        return [y.detach(), ops.clip_grad_norm(grads, 3.0), *grads]
+
+    static = {k: v.clone() for k, v in data.items()}
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(static)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(static)
+    for k in range(4):
+        ids.copy_(torch.randint(0, V, ids.shape, generator=g))
+        for t in static.values():
+            t.copy_(_randn(g, *t.shape))
+        want = step({k_: v.clone() for k_, v in static.items()})
+        graph.replay()
+        torch.cuda.synchronize()
+        assert float(want[1]) > 3.0 and all(torch.equal(a, b) for a, b in zip(out, want)), k
+
+
+@gpu
+def test_training_ops_from_two_threads_at_once(ops):
+    """Nothing is shared between calls: two threads on two streams, each over its own sizes, against the same calls one after the other."""
+    import threading
+
+    def work(seed, n, C, out):
+        g = torch.Generator(device=DEV).manual_seed(seed)
+        r = lambda *s: torch.randn(*s, generator=g, device=DEV)
+        ids = torch.randint(0, 777, (n,), generator=g, device=DEV)
+        dy, x, res, gate = r(n, C), r(3, 60, C), r(3, 60, C), r(3, C)
+        norm, grads = ops.Norm("layer", r(C), r(C)), [r(k) for k in (9, 70000, 3)]
+        for _ in range(20):
+            s, y, st = ops.block_norm(x, res, norm, gate=gate)
+            d = ops.block_norm_bwd(x, res, y, s, st, norm, gate=gate)
+            buf = [torch.empty_like(t) for t in grads]
+            got = [ops.embed_tokens_bwd(ids, dy, 777), ops.embed_positions_bwd(dy.view(-1, 5, C), 6), y, d["dgate"], d["dpre_gamma"], ops.clip_grad_norm(grads, 1.0, out=buf), *buf]
+        out.extend(got)
+
+    args = [(1, 5000, 64), (2, 900, 200)]
+    want = [[], []]
+    for a, w in zip(args, want):
+        work(*a, w)
+    torch.cuda.synchronize()
+    got = [[], []]
+
+    def on_stream(a, o):
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            work(*a, o)
+        s.synchronize()
+
+    threads = [threading.Thread(target=on_stream, args=(a, o)) for a, o in zip(args, got)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert all(len(g_) == len(w) and all(torch.equal(a, b) for a, b in zip(g_, w)) for g_, w in zip(got, want))
+
+
+@gpu
+def test_training_ops_while_another_device_is_current(ops, monkeypatch):
+    """A call makes its tensors' device current for its launches (here: the one there is, behind a runtime that names another)."""
+    x = torch.randn(5, 64, device=DEV)
+    want = ops.block_norm(x, x, ops.Norm("rms"))[1]
+    seen = []
+    real = torch.cuda.device
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 5)
+    monkeypatch.setattr(torch.cuda, "device", lambda d: seen.append(d) or real(d))
+    y = ops.block_norm(x, x, ops.Norm("rms"))[1]
+    monkeypatch.undo()
+    assert seen == [0] and torch.equal(y, want)
+
+
 # ------------------------------------------------------------------------------------------------ as the framework uses them
 @gpu
 @pytest.mark.parametrize("dtype", DTYPES)
