@@ -27,11 +27,14 @@ template <typename T> __device__ __forceinline__ uint32_t bits16(float x) {
     else return 0;
 }
 
-// How a thread's N channels lie in a row.  VEC: words of 16 bytes (8 or 4 channels), neighbouring threads on neighbouring words - needs
-// C * sizeof(T) and every pointer to be multiples of 16; otherwise element by element, neighbouring threads on neighbouring elements.
-// An object holds them as they are stored (words: packed, half the registers for 16-bit types), so that a load is under way until a value
-// is asked for.
-template <typename T, int TPR, int N, bool VEC> struct bn_part {
+// How a thread's N channels lie in a row: words of 16 bytes (8 or 4 channels), neighbouring threads on neighbouring words (BN_WORDS: C and
+// every address are multiples of a word; BN_ODD: rows of any length and address); rows shorter than a word element by element (BN_ELEMENTS).
+// An object holds them as they are stored (words: packed, half the registers for 16-bit types), so that a load is under way until
+// settle() or a value asks for it.  (4096 x 4001 bf16 with a gate, forward and backward: element by element 47 and 113 us, odd words 36 and
+// 67; the aligned words of 4096 x 4096 27 and 59.)
+enum { BN_ELEMENTS, BN_WORDS, BN_ODD };
+template <typename T, int TPR, int N, int MODE> struct bn_part {
+    static constexpr bool VEC = MODE != BN_ELEMENTS;
     static constexpr int W = VEC ? word16<T>::N : 1;
     static __device__ __forceinline__ int col(int t, int i) { return ((i / W) * TPR + t) * W + i % W; }
     u32x4 word[VEC ? N / word16<T>::N : 1];
@@ -42,7 +45,10 @@ template <typename T, int TPR, int N, bool VEC> struct bn_part {
             for (int i = 0; i < N; i += W) {
                 const int c = col(t, i);
                 word[i / W] = u32x4{0, 0, 0, 0};
-                if (c < C) word[i / W] = *(const u32x4*)(p + c);
+                if (c < C) {
+                    if constexpr (MODE == BN_ODD) word[i / W] = row_word_load<T>(p, c, C);
+                    else word[i / W] = *(const u32x4*)(p + c);
+                }
             }
         } else {
 #pragma unroll
@@ -51,6 +57,14 @@ template <typename T, int TPR, int N, bool VEC> struct bn_part {
                 one[i] = (T)0.f;
                 if (c < C) one[i] = p[c];
             }
+        }
+    }
+    // before the first value after a load
+    __device__ __forceinline__ void settle(int t, int C) {
+        if constexpr (MODE == BN_ODD) {
+#pragma unroll
+            for (int i = 0; i < N; i += W)
+                if (col(t, i) < C) word[i / W] = row_word_shift<T>(word[i / W], col(t, i), C);
         }
     }
     __device__ __forceinline__ void fill(float x) {
@@ -83,7 +97,8 @@ template <typename T, int TPR, int N, bool VEC> struct bn_part {
                     word16<T> a;
 #pragma unroll
                     for (int j = 0; j < W; ++j) a.v[j] = to_storage<T>(v[i + j]);
-                    store16(p + c, a, stream);
+                    if constexpr (MODE == BN_ODD) store_row_word(p, c, C, a, stream);
+                    else store16(p + c, a, stream);
                 } else {
                     p[c] = to_storage<T>(v[i]);
                 }
@@ -139,9 +154,9 @@ __device__ __forceinline__ void bn_stats(const float* v, int t, int C, int kind,
     r = rsqrtf(q / (float)C + eps);
 }
 
-template <typename T, int TPR, int N, bool VEC>
+template <typename T, int TPR, int N, int MODE>
 __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) k_block_norm(const gd_block_norm_t a, bool stream) {
-    using PART = bn_part<T, TPR, N, VEC>;
+    using PART = bn_part<T, TPR, N, MODE>;
     constexpr int RPB = TPR < 256 ? 256 / TPR : 1;           // rows a workgroup
     __shared__ float lds[64];
     int turn = 0;
@@ -158,6 +173,7 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) k_block_norm(const gd_b
     if (a.pre_gamma) eg.load((const T*)a.pre_gamma, t, C);
     if (a.pre_beta) eb.load((const T*)a.pre_beta, t, C);
     float h[N], mean = 0.f, r = 1.f;
+    x.settle(t, C);
 #pragma unroll
     for (int i = 0; i < N; ++i) h[i] = x[i];
     if (a.post_kind) bn_stats<PART, TPR, N>(h, t, C, a.post_kind, a.post_eps, lds, turn, mean, r);
@@ -166,19 +182,23 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) k_block_norm(const gd_b
 #pragma unroll
         for (int i = 0; i < N; ++i) h[i] = PART::col(t, i) < C ? (h[i] - mean) * r : 0.f;
         if (a.post_gamma) {
+            og.settle(t, C);
 #pragma unroll
             for (int i = 0; i < N; ++i) h[i] *= og[i];
         }
         if (a.post_beta) {
+            ob.settle(t, C);
 #pragma unroll
             for (int i = 0; i < N; ++i) h[i] += ob[i];
         }
     }
     if (a.gate) {
+        gate.settle(t, C);
 #pragma unroll
         for (int i = 0; i < N; ++i) h[i] *= gate[i];
     }
     if (a.res) {
+        res.settle(t, C);
 #pragma unroll
         for (int i = 0; i < N; ++i) h[i] = __builtin_fmaf(a.res_scale, res[i], h[i]);
     }
@@ -191,10 +211,12 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) k_block_norm(const gd_b
 #pragma unroll
     for (int i = 0; i < N; ++i) h[i] = (h[i] - mean) * r;
     if (a.pre_gamma) {
+        eg.settle(t, C);
 #pragma unroll
         for (int i = 0; i < N; ++i) h[i] *= eg[i];
     }
     if (a.pre_beta) {
+        eb.settle(t, C);
 #pragma unroll
         for (int i = 0; i < N; ++i) h[i] += eb[i];
     }
@@ -254,9 +276,9 @@ template <typename PART> struct bn_row {
 // column sums together do not fit the registers (WRAP above 4096 channels): BN_OUT writes dx, dres and sums for the norm in front of the
 // next block, BN_WRAP sums for the gate and the norm on x.  (2048 x 8192 bf16 with both: one launch 213 us, spilling, two 110.)
 enum { BN_ALL, BN_OUT, BN_WRAP };
-template <typename T, int TPR, int N, bool VEC, bool WRAP, int SUMS>
+template <typename T, int TPR, int N, int MODE, bool WRAP, int SUMS>
 __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) k_block_norm_bwd(const bn_bwd_args b) {
-    using PART = bn_part<T, TPR, N, VEC>;
+    using PART = bn_part<T, TPR, N, MODE>;
     constexpr int RPB = TPR < 256 ? 256 / TPR : 1;
     // the next row's data beside this one's and the parameters over all rows, where the registers hold them: 8 waves and 16 channels a
     // thread leave none
@@ -269,11 +291,11 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) k_block_norm_bwd(const 
     float pre_g[N] = {}, pre_b[N] = {}, post_g[N] = {}, post_b[N] = {}, dgate[N] = {};
     PART og, ob, eg, gate;
     const auto params = [&](long long gate_row) {
-        if (a.f.pre_gamma) eg.load((const T*)a.f.pre_gamma, t, C); else eg.fill(1.f);
+        if (a.f.pre_gamma) eg.load((const T*)a.f.pre_gamma, t, C), eg.settle(t, C); else eg.fill(1.f);
         if constexpr (WRAP) {
-            if (a.f.post_gamma) og.load((const T*)a.f.post_gamma, t, C); else og.fill(1.f);
-            if (a.f.post_beta) ob.load((const T*)a.f.post_beta, t, C); else ob.fill(0.f);
-            if (a.f.gate) gate.load((const T*)a.f.gate + gate_row * a.f.gate_ld, t, C); else gate.fill(1.f);
+            if (a.f.post_gamma) og.load((const T*)a.f.post_gamma, t, C), og.settle(t, C); else og.fill(1.f);
+            if (a.f.post_beta) ob.load((const T*)a.f.post_beta, t, C), ob.settle(t, C); else ob.fill(0.f);
+            if (a.f.gate) gate.load((const T*)a.f.gate + gate_row * a.f.gate_ld, t, C), gate.settle(t, C); else gate.fill(1.f);
         }
     };
     if (AHEAD) params(0);
@@ -296,7 +318,7 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) k_block_norm_bwd(const 
         const long long gate_row = per == a.f.rows ? 0 : g0 / per;
         const long long g1 = (gate_row + 1) * per < r1 ? (gate_row + 1) * per : r1;
         if constexpr (WRAP && AHEAD) {
-            if (a.f.gate) gate.load((const T*)a.f.gate + gate_row * a.f.gate_ld, t, C);
+            if (a.f.gate) gate.load((const T*)a.f.gate + gate_row * a.f.gate_ld, t, C), gate.settle(t, C);
         }
         for (long long row = g0 + wave; row < g1; row += RPB) {        // (TPR >= 256: the same rows for the whole workgroup)
             if constexpr (!AHEAD) {
@@ -310,6 +332,10 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) k_block_norm_bwd(const 
                 const long long then = row + RPB < g1 ? row + RPB : g1 + wave;
                 if (then < r1) fetch(then);
             }
+            cur.x.settle(t, C);
+            if (a.f.res) cur.res.settle(t, C);
+            if (a.gy) cur.gy.settle(t, C);
+            if (a.gs) cur.gs.settle(t, C);
             float d[N], sv[N], xh[N];
             // forward again: xh = normalised x, h = post(x), sv = the sum
             const float post_mean = WRAP && a.f.post_kind ? cur.stats[0] : 0.f, post_r = WRAP && a.f.post_kind ? cur.stats[1] : 1.f;
@@ -425,7 +451,7 @@ __global__ void __launch_bounds__(1024) k_block_norm_cols(const bn_bwd_args b, i
 
 static bool bn_aligned(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
-static bool bn_vec(const gd_block_norm_t& f, int elem) {
+static bool bn_words(const gd_block_norm_t& f, int elem) {
     return f.C * elem % 16 == 0 && bn_aligned(f.x) && bn_aligned(f.res) && bn_aligned(f.gate) && (!f.gate || f.gate_ld * elem % 16 == 0) &&
            bn_aligned(f.post_gamma) && bn_aligned(f.post_beta) && bn_aligned(f.pre_gamma) && bn_aligned(f.pre_beta) && bn_aligned(f.s) && bn_aligned(f.y);
 }
@@ -458,13 +484,18 @@ static int bn_check(const gd_block_norm_t* f, int dtype, const char* who) {
 
 template <typename T>
 static void bn_launch(const gd_block_norm_t& a, hipStream_t st) {
-    const bool vec = bn_vec(a, sizeof(T)), stream = streams_past_cache((double)a.rows * a.C * sizeof(T) * (1 + !!a.res + !!a.s + !!a.y));
+    const bool stream = streams_past_cache((double)a.rows * a.C * sizeof(T) * (1 + !!a.res + !!a.s + !!a.y));
+    const bool words = bn_words(a, sizeof(T));
+    if (a.C < word16<T>::N) {
+        k_block_norm<T, 64, 8, BN_ELEMENTS><<<(unsigned)((a.rows + 3) / 4), 256, 0, st>>>(a, stream);
+        return;
+    }
 #define BN_GO(TPR, N)                                                                                         \
     do {                                                                                                      \
         constexpr int rpb = TPR < 256 ? 256 / TPR : 1;                                                        \
         const unsigned grid = (unsigned)((a.rows + rpb - 1) / rpb);                                           \
-        if (vec) k_block_norm<T, TPR, N, true><<<grid, rpb * TPR, 0, st>>>(a, stream);                                \
-        else k_block_norm<T, TPR, N, false><<<grid, rpb * TPR, 0, st>>>(a, stream);                                   \
+        if (words) k_block_norm<T, TPR, N, BN_WORDS><<<grid, rpb * TPR, 0, st>>>(a, stream);                  \
+        else k_block_norm<T, TPR, N, BN_ODD><<<grid, rpb * TPR, 0, st>>>(a, stream);                          \
     } while (0)
     BN_SHAPE(a.C, BN_GO);
 #undef BN_GO
@@ -496,6 +527,19 @@ extern "C" size_t gd_block_norm_bwd_workspace_bytes(int64_t rows, int C, int64_t
     return sizeof(float) * (size_t)C * (size_t)(BN_SUMS * wg + (gate_rows > 0 ? wg + gate_rows - 1 : 0));
 }
 
+template <typename T, int TPR, int N, int MODE>
+static void bn_go_bwd(const bn_bwd_args& b, int wg, bool wrap, bool wrap_sums, hipStream_t st) {
+    constexpr int threads = TPR < 256 ? 256 : TPR;
+    if (!wrap) {
+        k_block_norm_bwd<T, TPR, N, MODE, false, BN_ALL><<<wg, threads, 0, st>>>(b);
+    } else if constexpr (TPR * N >= 8192) {
+        k_block_norm_bwd<T, TPR, N, MODE, true, BN_OUT><<<wg, threads, 0, st>>>(b);
+        if (wrap_sums) k_block_norm_bwd<T, TPR, N, MODE, true, BN_WRAP><<<wg, threads, 0, st>>>(b);
+    } else {
+        k_block_norm_bwd<T, TPR, N, MODE, true, BN_ALL><<<wg, threads, 0, st>>>(b);
+    }
+}
+
 template <typename T>
 static void bn_launch_bwd(const gd_block_norm_bwd_t& a, float* ws, hipStream_t st) {
     bn_bwd_args b;
@@ -512,24 +556,14 @@ static void bn_launch_bwd(const gd_block_norm_bwd_t& a, float* ws, hipStream_t s
     }
     b.gate_sums = a.dgate ? ws + (size_t)BN_SUMS * wg0 * a.f.C : nullptr;
     const bool wrap = a.f.gate || a.f.post_kind, wrap_sums = a.dgate || a.dpost_gamma || a.dpost_beta;
-    const bool vec = bn_vec(a.f, sizeof(T)) && bn_aligned(a.gy) && bn_aligned(a.gs) && bn_aligned(a.dx) && bn_aligned(a.dres);
+    const bool words = bn_words(a.f, sizeof(T)) && bn_aligned(a.gy) && bn_aligned(a.gs) && bn_aligned(a.dx) && bn_aligned(a.dres);
 #define BN_GO(TPR, N)                                                                                         \
     do {                                                                                                      \
-        constexpr int threads = TPR < 256 ? 256 : TPR;                                                        \
-        if constexpr (TPR * N >= 8192) {                                                                      \
-            if (!vec) k_block_norm_bwd<T, TPR, N, false, true, BN_OUT><<<wg, threads, 0, st>>>(b);            \
-            else if (wrap) k_block_norm_bwd<T, TPR, N, true, true, BN_OUT><<<wg, threads, 0, st>>>(b);        \
-            else k_block_norm_bwd<T, TPR, N, true, false, BN_ALL><<<wg, threads, 0, st>>>(b);                 \
-            if (!wrap_sums) break;                                                                            \
-            if (!vec) k_block_norm_bwd<T, TPR, N, false, true, BN_WRAP><<<wg, threads, 0, st>>>(b);           \
-            else k_block_norm_bwd<T, TPR, N, true, true, BN_WRAP><<<wg, threads, 0, st>>>(b);                 \
-        } else {                                                                                              \
-            if (!vec) k_block_norm_bwd<T, TPR, N, false, true, BN_ALL><<<wg, threads, 0, st>>>(b);            \
-            else if (wrap) k_block_norm_bwd<T, TPR, N, true, true, BN_ALL><<<wg, threads, 0, st>>>(b);        \
-            else k_block_norm_bwd<T, TPR, N, true, false, BN_ALL><<<wg, threads, 0, st>>>(b);                 \
-        }                                                                                                     \
+        if (words) bn_go_bwd<T, TPR, N, BN_WORDS>(b, wg, wrap, wrap_sums, st);                                \
+        else bn_go_bwd<T, TPR, N, BN_ODD>(b, wg, wrap, wrap_sums, st);                                        \
     } while (0)
-    BN_SHAPE(a.f.C, BN_GO);
+    if (a.f.C < word16<T>::N) k_block_norm_bwd<T, 64, 8, BN_ELEMENTS, true, BN_ALL><<<wg, 256, 0, st>>>(b);
+    else BN_SHAPE(a.f.C, BN_GO);
 #undef BN_GO
     const int gates = a.dgate ? (int)(a.f.rows / a.f.rows_per_gate) : 0;
     if (any || gates) k_block_norm_cols<T><<<dim3((a.f.C + 15) / 16, BN_SUMS + gates), 1024, 0, st>>>(b, wg);

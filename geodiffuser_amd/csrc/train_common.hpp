@@ -8,6 +8,19 @@ template <typename T> struct alignas(16) word16 {
     T v[16 / sizeof(T)];
 };
 
+// The same at any address of a 16-bit element: global memory takes unaligned vector accesses, so that rows of odd length and views into a
+// buffer are loaded and stored as wide as others.
+typedef u32x4 u32x4_any __attribute__((aligned(2), may_alias));
+
+// A row of C elements as words of W = 16 / sizeof(T) where C is no multiple of W (but at least W), and at any address.  The word at
+// element c is loaded as it stands; the last one, of which the row has less, where it is whole, and shifted when it is needed: zeros
+// behind the row's end.
+template <typename T> __device__ __forceinline__ int row_word_start(int c, int C) { return c + word16<T>::N <= C ? c : C - word16<T>::N; }
+template <typename T> __device__ __forceinline__ u32x4 row_word_load(const T* p, int c, int C) { return *(const u32x4_any*)(p + row_word_start<T>(c, C)); }
+template <typename T> __device__ __forceinline__ u32x4 row_word_shift(u32x4 w, int c, int C) {
+    return __builtin_bit_cast(u32x4, __builtin_bit_cast(unsigned __int128, w) >> ((c - row_word_start<T>(c, C)) * 8 * (int)sizeof(T)));
+}
+
 // The one rounding of a result to its storage type.  f16: the binary32 value is kept out of the compiler's sight, which otherwise folds
 // the last multiplication and the conversion of SINGLE elements into v_fma_mixlo_f16 (rounding once from the exact product) but not
 // those of pairs: a result's bits would depend on whether its tensor is aligned.
@@ -22,14 +35,24 @@ template <typename T> __device__ __forceinline__ T to_storage(float x) {
 // against it 152 MB of zero rows (inside the cache) 22 -> 28 us.
 static inline bool streams_past_cache(double bytes) { return bytes > 256.0 * 1024 * 1024; }
 
-template <typename T> __device__ __forceinline__ void store16(T* p, const word16<T>& w, bool stream) {
+template <typename T, typename WORD = u32x4> __device__ __forceinline__ void store16(T* p, const word16<T>& w, bool stream) {
     const u32x4 bits = __builtin_bit_cast(u32x4, w);
     if (stream) {                   // (the empty statements keep the compiler from merging the two stores into one ordinary one)
         asm volatile("" ::: "memory");
-        __builtin_nontemporal_store(bits, (u32x4*)p);
+        __builtin_nontemporal_store(bits, (WORD*)p);
         asm volatile("" ::: "memory");
     } else {
-        *(u32x4*)p = bits;
+        *(WORD*)p = bits;
+    }
+}
+// the word at p[c] of a row of C elements: what lies behind the row's end is not written
+template <typename T> __device__ __forceinline__ void store_row_word(T* p, int c, int C, const word16<T>& w, bool stream) {
+    if (c + word16<T>::N <= C) {
+        store16<T, u32x4_any>(p + c, w, stream);
+    } else {
+#pragma unroll
+        for (int j = 0; j < word16<T>::N; ++j)
+            if (c + j < C) p[c + j] = w.v[j];
     }
 }
 

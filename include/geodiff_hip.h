@@ -558,7 +558,8 @@ int gd_embed_pos_bwd(const void* dy, int64_t B, int L, int C, int pos_rows, void
  *   kinds: GD_NORM_NONE, GD_NORM_LAYER (xh = (v - mean) / sqrt(var + eps)), GD_NORM_RMS (xh = v / sqrt(mean v^2 + eps)), then
  *   xh * gamma + beta; gamma, beta [C] or NULL (1, 0).  gate: one row of C for every rows_per_gate rows, gate_ld elements apart, or
  *   NULL (1).  res NULL: s = gate * h.  s may be NULL; y goes with pre_kind.  stats [rows, 4] f32 (mean, 1 / deviation of x, then of
- *   s; 0, 1 for a norm that is not there; NULL: not kept) is what the backward needs.  y is computed from the unrounded s. */
+ *   s; 0, 1 for a norm that is not there; NULL: not kept) is what the backward needs.  y is computed from the unrounded s.
+ *   No output may overlap an input. */
 enum { GD_NORM_NONE = 0, GD_NORM_LAYER = 1, GD_NORM_RMS = 2 };
 typedef struct gd_block_norm {
     const void *x, *res, *gate, *post_gamma, *post_beta, *pre_gamma, *pre_beta;
