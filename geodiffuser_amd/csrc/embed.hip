@@ -12,40 +12,55 @@
 //   position gradient of the same                                    50 + 5 us (323 MB, a part of it still in the cache)
 #include "train_common.hpp"
 
-// A lane's N channels of a slice of 64 * N: one word of 16 bytes (VEC: C * sizeof(T) and all pointers are multiples of 16), or N single
-// elements, neighbouring lanes on neighbouring elements.
+// A lane's N channels of a slice of 64 * N: one word of 16 bytes at any address (VEC), or, of rows shorter than a word, N single elements,
+// neighbouring lanes on neighbouring elements.  Where C is no multiple of the word, a row's last word lies over the one before it: both
+// lanes compute and store the same bits for the channels that they share.  (Gradient of 1024 x 77 rows of 1279 f16 channels: element by
+// element 197 us, so 84; 1280 channels 80.  Lookup of the same: 127, 65 and 59.)
 template <typename T, bool VEC>
 struct em_cols {
     static constexpr int N = VEC ? (int)(16 / sizeof(T)) : 8, SLICE = 64 * N;
-    static __device__ __forceinline__ int col(int slice, int lane, int i) { return slice * SLICE + (VEC ? lane * N + i : i * 64 + lane); }
+    // the lane's first channel (C and above: none) and the distance to its next ones
+    static constexpr int STEP = VEC ? 1 : 64;
+    static __device__ __forceinline__ int col(int slice, int lane, int C) {
+        const int c = slice * SLICE + lane * (VEC ? N : 1);
+        return VEC && c < C ? row_word_start<T>(c, C) : c;
+    }
     static __device__ __forceinline__ void load(const T* __restrict__ p, int slice, int lane, int C, float* v) {
         if constexpr (VEC) {
-            const int c = col(slice, lane, 0);
+            const int c = col(slice, lane, C);
             word16<T> a = {};
-            if (c < C) a = *(const word16<T>*)(p + c);
+            if (c < C) a = __builtin_bit_cast(word16<T>, *(const u32x4_any*)(p + c));
 #pragma unroll
             for (int i = 0; i < N; ++i) v[i] = (float)a.v[i];
         } else {
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                const int c = col(slice, lane, i);
+                const int c = col(slice, lane, C) + i * STEP;
                 v[i] = c < C ? (float)p[c] : 0.f;
             }
         }
     }
     static __device__ __forceinline__ void store(T* p, int slice, int lane, int C, const float* v, bool stream) {
         if constexpr (VEC) {
-            const int c = col(slice, lane, 0);
+            const int c = col(slice, lane, C);
             word16<T> a;
 #pragma unroll
             for (int i = 0; i < N; ++i) a.v[i] = to_storage<T>(v[i]);
-            if (c < C) store16(p + c, a, stream);
+            if (c < C) store16<T, u32x4_any>(p + c, a, stream);
         } else {
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                const int c = col(slice, lane, i);
+                const int c = col(slice, lane, C) + i * STEP;
                 if (c < C) p[c] = to_storage<T>(v[i]);
             }
+        }
+    }
+    static __device__ __forceinline__ void store_sums(float* p, int slice, int lane, int C, const float* v) {
+        const int c = col(slice, lane, C);
+        if (c < C) {
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                if (VEC || c + i * STEP < C) p[c + i * STEP] = v[i];
         }
     }
 };
@@ -56,7 +71,19 @@ struct em_ids {
     __device__ __forceinline__ long long operator[](long long i) const { return wide ? ((const long long*)p)[i] : (long long)((const int*)p)[i]; }
 };
 
-template <typename T, int N> struct alignas(N * sizeof(T)) em_piece { T v[N]; };
+// one word (VEC) or element of a row
+template <typename T, bool VEC> struct em_piece { T v[VEC ? word16<T>::N : 1]; };
+template <typename T, bool VEC> __device__ __forceinline__ em_piece<T, VEC> em_load(const T* p) {
+    if constexpr (VEC) return __builtin_bit_cast(em_piece<T, VEC>, *(const u32x4_any*)p);
+    else return em_piece<T, VEC>{{*p}};
+}
+template <typename T, bool VEC> __device__ __forceinline__ void em_store(T* p, const em_piece<T, VEC>& v, bool stream) {
+    if constexpr (VEC) store16<T, u32x4_any>(p, __builtin_bit_cast(word16<T>, v), stream);
+    else *p = v.v[0];
+}
+// words or elements of a row of C, and where unit u of it begins
+template <typename T, bool VEC> __device__ __forceinline__ int em_units(int C) { return VEC ? (C + word16<T>::N - 1) / word16<T>::N : C; }
+template <typename T, bool VEC> __device__ __forceinline__ int em_start(int u, int C) { return VEC ? row_word_start<T>(u * word16<T>::N, C) : u; }
 
 // How a wave covers rows of `units` words (VEC) or elements: 2^shift lanes a row, 64 >> shift rows at a time
 static int em_lane_shift(int units) {
@@ -70,32 +97,31 @@ template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) k_embed(const em_ids ids, long long n, const T* __restrict__ table, const T* __restrict__ pos, int L, int V, int C,
                                                float scale, bool stream, int shift, T* y) {
     constexpr int W = VEC ? word16<T>::N : 1, BATCH = VEC && sizeof(T) == 2 ? 2 : 4;       // (f16, 1280 channels: 2 words 43.5 us, 4 47.6; f32: 43 and 41)
-    const int lane = threadIdx.x & 63, units = C / W, lanes = 1 << shift;
+    const int lane = threadIdx.x & 63, units = em_units<T, VEC>(C), lanes = 1 << shift;
     const long long row = (((long long)blockIdx.x * 4 + (threadIdx.x >> 6)) << (6 - shift)) + (lane >> shift);
     if (row >= n) return;
     const long long id = ids[row];
     const bool in = id >= 0 && id < V;
-    const em_piece<T, W>* src = (const em_piece<T, W>*)(table + (in ? id : 0) * C);
-    const em_piece<T, W>* ps = pos ? (const em_piece<T, W>*)(pos + (long long)((unsigned)row % (unsigned)L) * C) : nullptr;
-    em_piece<T, W>* out = (em_piece<T, W>*)(y + row * C);
+    const T* src = table + (in ? id : 0) * C;
+    const T* ps = pos ? pos + (long long)((unsigned)row % (unsigned)L) * C : nullptr;
+    T* out = y + row * C;
     for (int u0 = 0; u0 < units; u0 += BATCH * lanes) {
-        em_piece<T, W> w[BATCH], q[BATCH];
+        em_piece<T, VEC> w[BATCH], q[BATCH];
         const int u = u0 + (lane & (lanes - 1));
 #pragma unroll
         for (int j = 0; j < BATCH; ++j)
             if (u0 + j * lanes < units) {                    // (the same for the whole wave)
-                const int at = u + j * lanes < units ? u + j * lanes : 0;
-                w[j] = src[at];
-                if (ps) q[j] = ps[at];
+                const int at = u + j * lanes < units ? em_start<T, VEC>(u + j * lanes, C) : 0;
+                w[j] = em_load<T, VEC>(src + at);
+                if (ps) q[j] = em_load<T, VEC>(ps + at);
             }
 #pragma unroll
         for (int j = 0; j < BATCH; ++j)
             if (u + j * lanes < units) {
-                em_piece<T, W> o;
+                em_piece<T, VEC> o;
 #pragma unroll
                 for (int i = 0; i < W; ++i) o.v[i] = to_storage<T>(in ? __builtin_fmaf(scale, (float)w[j].v[i], ps ? (float)q[j].v[i] : 0.f) : __builtin_nanf(""));
-                if constexpr (VEC) store16(&out[u + j * lanes].v[0], __builtin_bit_cast(word16<T>, o), stream);
-                else out[u + j * lanes] = o;
+                em_store<T, VEC>(out + em_start<T, VEC>(u + j * lanes, C), o, stream);
             }
     }
 }
@@ -103,15 +129,11 @@ __global__ void __launch_bounds__(256) k_embed(const em_ids ids, long long n, co
 // Zeros in those of the rows [v0, v0 + rows) of the table that `there` (of the row's offset) does not name.
 template <typename T, bool VEC, typename THERE>
 __device__ __forceinline__ void em_zero_rows(T* dtable, long long v0, int rows, int C, int shift, bool stream, THERE&& there) {
-    constexpr int W = VEC ? word16<T>::N : 1;
-    const int lane = threadIdx.x & 63, units = C / W, lanes = 1 << shift;
+    const int lane = threadIdx.x & 63, units = em_units<T, VEC>(C), lanes = 1 << shift;
     for (int r = ((threadIdx.x >> 6) << (6 - shift)) + (lane >> shift); r < rows; r += (blockDim.x >> 6) << (6 - shift)) {
         if (there(r)) continue;
         T* p = dtable + (v0 + r) * C;
-        for (int u = lane & (lanes - 1); u < units; u += lanes) {
-            if constexpr (VEC) store16(p + (long long)u * W, word16<T>{}, stream);
-            else p[u] = (T)0.f;
-        }
+        for (int u = lane & (lanes - 1); u < units; u += lanes) em_store<T, VEC>(p + em_start<T, VEC>(u, C), em_piece<T, VEC>{}, stream);
     }
 }
 
@@ -498,8 +520,7 @@ __global__ void __launch_bounds__(256) k_embed_bwd_sum(const em_sum a, const T* 
                 for (int i = 0; i < N; ++i) acc[i] += v[j][i];
                 if (stop > live ? k == stop - 1 || (k < live && ((ends >> k) & 1)) : (ends >> k) & 1) {
                     if (partial) {
-#pragma unroll
-                        for (int i = 0; i < N; ++i) if (COLS::col(sl, lane, i) < C) a.head[(long long)t * C + COLS::col(sl, lane, i)] = acc[i];
+                        COLS::store_sums(a.head + (long long)t * C, sl, lane, C, acc);
                     } else {
 #pragma unroll
                         for (int i = 0; i < N; ++i) acc[i] *= a.scale;
@@ -513,9 +534,7 @@ __global__ void __launch_bounds__(256) k_embed_bwd_sum(const em_sum a, const T* 
             }
         }
         if (goes && stop == live) {
-            float* part = partial ? a.head : a.tail;
-#pragma unroll
-            for (int i = 0; i < N; ++i) if (COLS::col(sl, lane, i) < C) part[(long long)t * C + COLS::col(sl, lane, i)] = acc[i];
+            COLS::store_sums((partial ? a.head : a.tail) + (long long)t * C, sl, lane, C, acc);
         }
         return;
     }
@@ -636,21 +655,31 @@ static void em_join(const em_sum& a, T* dtable, hipStream_t st) {
 // more than one.
 #define EM_POS_ROWS 64
 
-template <typename T, int N, bool NT>
+template <typename T, bool VEC, bool NT>
 __device__ __forceinline__ void em_column(const T* p, long long width, long long b0, long long b1, float* acc) {
     for (long long b = b0; b < b1; b += 8) {
-        em_piece<T, N> w[8];
+        em_piece<T, VEC> w[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const T* at = p + (b + j < b1 ? b + j : b0) * width;
-            if constexpr (NT) w[j] = __builtin_bit_cast(em_piece<T, N>, __builtin_nontemporal_load((const u32x4*)at));
-            else w[j] = *(const em_piece<T, N>*)at;
+            if constexpr (NT) w[j] = __builtin_bit_cast(em_piece<T, VEC>, __builtin_nontemporal_load((const u32x4_any*)at));
+            else w[j] = em_load<T, VEC>(at);
         }
 #pragma unroll
         for (int j = 0; j < 8; ++j)
 #pragma unroll
-            for (int i = 0; i < N; ++i) acc[i] += b + j < b1 ? (float)w[j].v[i] : 0.f;
+            for (int i = 0; i < (VEC ? word16<T>::N : 1); ++i) acc[i] += b + j < b1 ? (float)w[j].v[i] : 0.f;
     }
+}
+
+// where a thread of k_embed_pos_bwd has its word: those of the sums, then those of the zeros behind them, the last of each moved back to
+// end where they end (the zeros are rows of C, which is a word at least)
+template <typename T, bool VEC> __device__ __forceinline__ long long em_pos_start(long long u, long long width, long long out_width) {
+    constexpr int N = VEC ? word16<T>::N : 1;
+    const long long sums = (width + N - 1) / N;
+    if (u < sums) return u * N + N <= width ? u * N : width - N;
+    const long long at = width + (u - sums) * N;
+    return at + N <= out_width || at >= out_width ? at : out_width - N;
 }
 
 // stream: dy is larger than the memory-side cache: it is read past it, so that the part which the table's gradient has left there is
@@ -659,26 +688,24 @@ template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) k_embed_pos_bwd(const T* __restrict__ dy, long long B, long long width, long long out_width, long long per, bool stream,
                                                        float* __restrict__ part, T* __restrict__ dpos) {
     constexpr int N = VEC ? word16<T>::N : 1;
-    const long long at = ((long long)blockIdx.x * 256 + threadIdx.x) * N;
+    const long long at = em_pos_start<T, VEC>((long long)blockIdx.x * 256 + threadIdx.x, width, out_width);
     if (at >= out_width) return;
     float acc[N] = {};
     if (at < width) {
         const long long b0 = (long long)blockIdx.y * per, b1 = b0 + per < B ? b0 + per : B;
-        if (VEC && stream) em_column<T, N, VEC>(dy + at, width, b0, b1, acc);
-        else em_column<T, N, false>(dy + at, width, b0, b1, acc);
+        if (VEC && stream) em_column<T, VEC, VEC>(dy + at, width, b0, b1, acc);
+        else em_column<T, VEC, false>(dy + at, width, b0, b1, acc);
     }
     if (part) {
         if (at < width) {
 #pragma unroll
             for (int i = 0; i < N; ++i) part[(long long)blockIdx.y * width + at + i] = acc[i];
         }
-    } else if constexpr (VEC) {
-        word16<T> w;
+    } else {
+        em_piece<T, VEC> w;
 #pragma unroll
         for (int i = 0; i < N; ++i) w.v[i] = to_storage<T>(acc[i]);
-        *(word16<T>*)(dpos + at) = w;
-    } else {
-        dpos[at] = to_storage<T>(acc[0]);
+        em_store<T, VEC>(dpos + at, w, false);
     }
 }
 
@@ -689,9 +716,8 @@ __global__ void __launch_bounds__(256) k_embed_pos_join(const float* __restrict_
     dpos[at] = to_storage<T>(at < width ? sum_strided(part + at, width, 0, parts, 1) : 0.f);
 }
 
-static bool em_vec(int C, int elem, const void* a, const void* b, const void* c = nullptr) {
-    return C * elem % 16 == 0 && (((uintptr_t)a | (uintptr_t)b | (uintptr_t)c) & 15) == 0;
-}
+// a row has a word at least
+static bool em_vec(int C, int elem) { return C * elem >= 16; }
 
 // picks T and VEC for a launch expression
 #define EM_LAUNCH(dtype, vec, CALL)                                                                           \
@@ -717,9 +743,9 @@ extern "C" int gd_embed(const void* ids, int ids64, int64_t n, const void* table
     if (rc != GD_OK) return rc;
     GD_REQUIRE(n > 0 && ids && table && y, GD_EINVAL, "gd_embed: null pointer or no positions");
     GD_REQUIRE(!pos || L > 0, GD_EINVAL, "gd_embed: position rows need the sequence length");
-    const bool vec = em_vec(C, EM_ELEM(dtype), table, y, pos);
+    const bool vec = em_vec(C, EM_ELEM(dtype));
     hipStream_t st = as_stream(stream);
-    const int shift = em_lane_shift(vec ? C * EM_ELEM(dtype) / 16 : C);
+    const int shift = em_lane_shift(vec ? (C * EM_ELEM(dtype) + 15) / 16 : C);
     const long long waves = (n + (64 >> shift) - 1) >> (6 - shift);
     const bool past = streams_past_cache((double)EM_ELEM(dtype) * C * ((double)n + (n < vocab ? n : vocab)));
     EM_LAUNCH(dtype, vec, (k_embed<T, VEC><<<(unsigned)((waves + 3) / 4), 256, 0, st>>>(em_ids{ids, ids64}, n, (const T*)table, (const T*)pos, L, (int)vocab, C, scale, past, shift, (T*)y)));
@@ -768,9 +794,9 @@ extern "C" int gd_embed_bwd(const void* ids, int ids64, int64_t n, const void* d
     const int rc = em_check(n, vocab, C, dtype, "gd_embed_bwd");
     if (rc != GD_OK) return rc;
     GD_REQUIRE(dtable && (n == 0 || (ids && dy)), GD_EINVAL, "gd_embed_bwd: null pointer");
-    const bool vec = em_vec(C, EM_ELEM(dtype), dy, dtable);
+    const bool vec = em_vec(C, EM_ELEM(dtype));
     const int slice = vec ? 64 * (16 / EM_ELEM(dtype)) : 512, slices = (C + slice - 1) / slice;
-    const int zero_rows = em_zero_rows_of(C, EM_ELEM(dtype)), shift = em_lane_shift(vec ? C * EM_ELEM(dtype) / 16 : C);
+    const int zero_rows = em_zero_rows_of(C, EM_ELEM(dtype)), shift = em_lane_shift(vec ? (C * EM_ELEM(dtype) + 15) / 16 : C);
     const long long zeros = (vocab + zero_rows - 1) / zero_rows;
     const bool past = streams_past_cache((double)EM_ELEM(dtype) * C * ((double)n + vocab));
     const em_plan p = em_plan_of(n, vocab, C);
@@ -810,10 +836,15 @@ extern "C" int gd_embed_bwd(const void* ids, int ids64, int64_t n, const void* d
     return GD_OK;
 }
 
-// sequences a workgroup adds, and how many workgroups share a column: as many as give each EM_POS_ROWS, at most 32 (every further one is
-// another row of sums to write and read)
-static int em_pos_parts(long long B, long long* per) {
-    long long parts = B / EM_POS_ROWS;
+// sequences a workgroup adds, and how many workgroups share a column: as many as give each EM_POS_ROWS, or fewer rows, down to 8, where
+// that leaves most CUs without a wave; from 64 sequences on (below, one workgroup and no second launch) and at most 32 (every further one
+// is another row of sums to write and read).  (f16, 77 positions, 8 to 32 rows against 64: 256 x 64 channels 6.3 and 9.3 us, 100 x 768 8.5
+// and 10.4; 256 x 768, beyond the bound, 11.7 and 10.7; 32 sequences of 768 channels in 4 workgroups 5.5, in one 4.8.)
+static int em_pos_parts(long long B, long long width, long long* per) {
+    long long rows = EM_POS_ROWS;
+    if (B >= 64)
+        while (rows > 8 && B / rows * width < 400 * 64 * 8) rows /= 2;
+    long long parts = B / rows;
     parts = parts < 1 ? 1 : parts > 32 ? 32 : parts;
     *per = (B + parts - 1) / parts;
     return *per > 0 ? (int)((B + *per - 1) / *per) : 1;
@@ -822,7 +853,7 @@ static int em_pos_parts(long long B, long long* per) {
 extern "C" size_t gd_embed_pos_bwd_workspace_bytes(int64_t B, int L, int C) {
     long long per;
     if (B < 0 || L <= 0 || C <= 0) return 0;
-    const int parts = em_pos_parts(B, &per);
+    const int parts = em_pos_parts(B, (long long)L * C, &per);
     return parts > 1 ? sizeof(float) * (size_t)parts * L * C : 0;
 }
 
@@ -833,10 +864,11 @@ extern "C" int gd_embed_pos_bwd(const void* dy, int64_t B, int L, int C, int pos
     const size_t need = gd_embed_pos_bwd_workspace_bytes(B, L, C);
     GD_REQUIRE(!need || (workspace && workspace_bytes >= need), GD_EWORKSPACE, "gd_embed_pos_bwd: workspace of %zu bytes needed", need);
     long long per;
-    const int parts = em_pos_parts(B, &per);
+    const int parts = em_pos_parts(B, (long long)L * C, &per);
     const long long width = (long long)L * C, out_width = (long long)pos_rows * C;
-    const bool vec = width * EM_ELEM(dtype) % 16 == 0 && out_width * EM_ELEM(dtype) % 16 == 0 && (((uintptr_t)dy | (uintptr_t)dpos) & 15) == 0;
-    const long long words = (out_width + (vec ? 16 / EM_ELEM(dtype) : 1) - 1) / (vec ? 16 / EM_ELEM(dtype) : 1), grid = (words + 255) / 256;
+    const bool vec = em_vec(C, EM_ELEM(dtype));
+    const int word = vec ? 16 / EM_ELEM(dtype) : 1;
+    const long long words = (width + word - 1) / word + (out_width - width + word - 1) / word, grid = (words + 255) / 256;
     GD_REQUIRE((out_width + 255) / 256 < (1ll << 31), GD_EUNSUPPORTED, "gd_embed_pos_bwd: too many positions for this width");
     float* const part = parts > 1 ? (float*)workspace : nullptr;
     hipStream_t st = as_stream(stream);

@@ -1091,3 +1091,43 @@ def test_null_text_optimisation_with_clipped_gradients(ops):
     free, loose, tight = run(None), run(1e9), run(1e-12)
     assert torch.isfinite(tight).all() and float(loose.norm()) > 0.5 * float(free.norm()) > 0
     assert float(tight.norm()) < 0.05 * float(free.norm())
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("C", [1, 2, 3, 4, 5, 7, 8, 9, 11, 15, 16, 17, 31, 33, 63, 65, 129, 513, 514, 517, 1023, 1027, 4097])
+def test_rows_of_every_width_stay_in_their_place(ops, monkeypatch, dtype, C):
+    """Every result lies inside a larger buffer, at an address that is a multiple of the element only: nothing around it is written, and the
+    results are those of the ordinary call."""
+    g = _gen(C)
+    V, B, L, P = 23, 5, 4, 7
+    ids, table, pos, dy = torch.randint(0, V, (B, L), generator=g).to(DEV), _randn(g, V, C, dtype=dtype), _randn(g, P, C, dtype=dtype), _randn(g, B, L, C, dtype=dtype)
+    many, dmany = torch.randint(0, V, (1100,), generator=g).to(DEV), _randn(g, 1100, C, dtype=dtype)
+    x, res, gy, gs = (_randn(g, B, L, C, dtype=dtype) for _ in range(4))
+    pre, post = (ops.Norm(k, _randn(g, C, dtype=dtype), _randn(g, C, dtype=dtype), 1e-5) for k in ("layer", "rms"))
+    gate = _randn(g, B, C, dtype=dtype)
+
+    def results():
+        s, y, stats = ops.block_norm(x, res, pre, post=post, gate=gate)
+        d = ops.block_norm_bwd(x, res, gy, gs, stats, pre, post=post, gate=gate)
+        return [ops.embed_tokens(ids, table, pos), ops.embed_tokens_bwd(ids, dy, V), ops.embed_tokens_bwd(many, dmany, V), ops.embed_positions_bwd(dy, P), s, y, stats,
+                *(d[k] for k in sorted(d))]
+    plain = results()
+    empty, like, around = torch.empty, torch.empty_like, []
+
+    def inside(*shape, dtype=torch.float32, device=None):
+        shape = torch.Size(shape[0] if len(shape) == 1 and not isinstance(shape[0], int) else shape)
+        front, n = 64 if dtype == torch.uint8 else 33, shape.numel()          # (workspaces keep their alignment)
+        buf = empty(front + n + 40, dtype=dtype, device=device).fill_(7)
+        around.extend((buf[:front], buf[front + n:]))
+        return buf[front:front + n].view(shape)
+    monkeypatch.setattr(torch, "empty", inside)
+    monkeypatch.setattr(torch, "empty_like", lambda t: inside(*t.shape, dtype=t.dtype, device=t.device))
+    moved = results()
+    monkeypatch.undo()
+    assert torch.empty is empty and torch.empty_like is like and len(around) >= 2 * len(plain)
+    assert all(bool((a == 7).all()) for a in around)
+    fi = torch.finfo(dtype)
+    for a, b in zip(plain, moved):
+        # (the column sums and row sums may be dealt out otherwise; values of ~1 and sums of at most 1100 of them)
+        assert a.shape == b.shape and bool(((a.double() - b.double()).abs() <= fi.eps * b.double().abs() + 1100 * 64 * U32 * 8 + fi.smallest_normal).all())
