@@ -249,17 +249,27 @@ struct em_keys {                // a pass's input: the ids themselves, or the la
 
 // lanes of the wave whose digit is this lane's (0 for lanes without a key)
 __device__ __forceinline__ unsigned long long em_match(int digit, bool live) {
-    unsigned long long m = __ballot(live);
+    const unsigned long long all = __ballot(live);
+    uint32_t lo = (uint32_t)all, hi = (uint32_t)(all >> 32);
 #pragma unroll
     for (int b = 0; b < 8; ++b) {
-        const unsigned long long s = __ballot((digit >> b) & 1);
-        m &= (digit >> b) & 1 ? s : ~s;
+        const int bit = (int)((unsigned)digit << (31 - b)) >> 31;    // 0 or ~0
+        const unsigned long long s = __ballot(bit);
+        lo &= ~((uint32_t)s ^ (uint32_t)bit);
+        hi &= ~((uint32_t)(s >> 32) ^ (uint32_t)bit);
     }
-    return live ? m : 0;
+    return live ? (unsigned long long)hi << 32 | lo : 0;
+}
+
+// What this wave's lanes wrote to LDS is what its lanes read from here on (a wave's LDS instructions stay in order; volatile accesses would
+// go through the flat path, waiting for each: 24 us instead of 21 for 20000 positions in one launch).
+__device__ __forceinline__ void em_wave_order() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
+    __builtin_amdgcn_wave_barrier();
 }
 
 // counts[digit] += occurrences in the wave's entries [lo, hi)
-__device__ __forceinline__ void em_count(const em_keys& k, long long lo, long long hi, int shift, volatile int* counts) {
+__device__ __forceinline__ void em_count(const em_keys& k, long long lo, long long hi, int shift, int* counts) {
     const int lane = threadIdx.x & 63;
     for (long long base = lo; base < hi; base += 64) {
         const long long i = base + lane;
@@ -267,7 +277,7 @@ __device__ __forceinline__ void em_count(const em_keys& k, long long lo, long lo
         const int d = live ? (int)(k(i) >> shift) & 255 : 0;
         const unsigned long long m = em_match(d, live);
         if (live && (m & ((1ull << lane) - 1)) == 0) counts[d] += __popcll(m);
-        __builtin_amdgcn_wave_barrier();
+        em_wave_order();
     }
 }
 
@@ -340,14 +350,14 @@ __global__ void __launch_bounds__(1024) k_embed_sort_move(const em_keys k, const
     part[q][0][d0] = before;
     part[q][1][d0] = all;
     __syncthreads();
-    volatile int* place = counts[wave];
+    int* place = counts[wave];
     int round = 0;
     for (long long base = lo; base < hi; base += 64, ++round) {
         const bool live = base + lane < hi;
         const int d = live ? (int)((few ? key_of[round & 1] : k(base + lane)) >> shift) & 255 : 0;
         const unsigned long long m = em_match(d, live);
         if (live && (m & ((1ull << lane) - 1)) == 0) place[d] += __popcll(m);
-        __builtin_amdgcn_wave_barrier();
+        em_wave_order();
     }
     before = part[0][0][d0] + part[1][0][d0] + part[2][0][d0] + part[3][0][d0];
     all = part[0][1][d0] + part[1][1][d0] + part[2][1][d0] + part[3][1][d0];
@@ -370,9 +380,9 @@ __global__ void __launch_bounds__(1024) k_embed_sort_move(const em_keys k, const
         const unsigned long long m = em_match(d, live);
         const int rank = __popcll(m & ((1ull << lane) - 1));
         const int first = live ? place[d] : 0;
-        __builtin_amdgcn_wave_barrier();
+        em_wave_order();
         if (live && rank == 0) place[d] = first + __popcll(m);
-        __builtin_amdgcn_wave_barrier();
+        em_wave_order();
         if (live) {
             key_out[first + rank] = key;
             pos_out[first + rank] = few ? pos_of[round & 1] : k.key ? k.pos[i] : (uint32_t)i;
@@ -381,73 +391,81 @@ __global__ void __launch_bounds__(1024) k_embed_sort_move(const em_keys k, const
     }
 }
 
-// Up to EM_LDS_MAX positions and vocabularies below 2^20: the same sort by one workgroup in LDS, an entry in 32 bits (token above, position
-// below), one launch for all passes.  (The gradient of 4000 positions takes 31 us so and 36 us by the launches above, of 8000 42 and 37.)
-#define EM_LDS_MAX 4096
-#define EM_LDS_POS_BITS 12
+// Fewer positions, in one launch: every workgroup looks through all ids and puts those of its own 256 tokens in their places, behind the
+// number of smaller ones, which it has counted on the way.  A thread keeps its ids in registers from the one look on, and one digit is left
+// to rank by.  (Bound by the workgroup with the padding and the most frequent words, which ranks most of the positions the others
+// find that they have none among 64, and in large tables by the looks.  The gradient (bf16, by this sort and by the passes above): 5400
+// positions and 12000 rows of 64 channels 25 and 36 us, 8192 26 and 37, 16384 35 and 39, 24000 44 and 40; 8192 positions and 300000 rows 30
+// and 46, 1000000 rows 52 and 50.)
+#define EM_RANGE_MAX 16384
+static bool em_by_ranges(long long n, long long vocab) { return n <= EM_RANGE_MAX && vocab < (1 << 20) && n * vocab <= 1ll << 32; }
 
-__global__ void __launch_bounds__(1024) k_embed_sort_lds(const em_keys k, int n, int passes, uint32_t* __restrict__ key_out, uint32_t* __restrict__ pos_out,
-                                                         unsigned char* __restrict__ there, int there_words) {
-    __shared__ uint32_t entry[2][EM_LDS_MAX];
-    __shared__ int counts[16][256], sums[4];
-    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
-    for (int i = tid; i < there_words; i += 1024) ((uint32_t*)there)[i] = 0;
+template <int CHUNKS>
+__global__ void __launch_bounds__(1024) k_embed_sort_ranges(const em_ids ids, int n, unsigned vocab, long long padding, uint32_t* __restrict__ key_out,
+                                                            uint32_t* __restrict__ pos_out, unsigned char* __restrict__ there) {
+    __shared__ int counts[16][256], sums[4], smaller[16];
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+    const int chunks = (n + 1023) / 1024, lo = wave * chunks * 64 + lane;
+    const uint32_t from = blockIdx.x * 256;
+    uint32_t e[CHUNKS];                                      // the key (vocab: no row of the table; ~0: no position), then rank << 9 | 256 | digit, or 0
+    const auto look = [&](auto* p) {
+        decltype(*p + 0) id[CHUNKS];
 #pragma unroll
-    for (int r = 0; r < EM_LDS_MAX / 1024; ++r) {
-        const int i = r * 1024 + tid;
-        if (i < n) entry[0][i] = k(i) << EM_LDS_POS_BITS | (uint32_t)i;
-    }
-    const int run = (n + 1023) / 1024 * 64, lo = wave * run, hi = lo + run < n ? lo + run : n;
-    for (int p = 0; p < passes; ++p) {
-        const uint32_t* from = entry[p & 1];
-        uint32_t* to = entry[(p + 1) & 1];
-        const int shift = EM_LDS_POS_BITS + 8 * p;
-        for (int i = tid; i < 16 * 256; i += 1024) counts[0][i] = 0;
-        __syncthreads();
-        volatile int* place = counts[wave];
-        for (int base = lo; base < hi; base += 64) {
-            const bool live = base + lane < hi;
-            const int d = live ? (int)(from[base + lane] >> shift) & 255 : 0;
-            const unsigned long long m = em_match(d, live);
-            if (live && (m & ((1ull << lane) - 1)) == 0) place[d] += __popcll(m);
-            __builtin_amdgcn_wave_barrier();
-        }
-        __syncthreads();
-        int all = 0;
-        if (tid < 256) {
+        for (int c = 0; c < CHUNKS; ++c)
+            if (c < chunks) id[c] = p[lo + c * 64 < n ? lo + c * 64 : n - 1];
 #pragma unroll
-            for (int w = 0; w < 16; ++w) all += counts[w][tid];
-        }
-        int at = em_below(all, sums);
-        if (tid < 256) {
+        for (int c = 0; c < CHUNKS; ++c)
+            if (c < chunks) e[c] = lo + c * 64 >= n ? ~0u : id[c] >= 0 && (long long)id[c] < (long long)vocab && (long long)id[c] != padding ? (uint32_t)id[c] : vocab;
+    };
+    if (ids.wide) look((const long long*)ids.p);
+    else look((const int*)ids.p);
+    for (int i = tid; i < 16 * 256; i += 1024) counts[0][i] = 0;
+    __syncthreads();
+    int* count = counts[wave];
+    int less = 0;
 #pragma unroll
-            for (int w = 0; w < 16; ++w) {
-                const int c = counts[w][tid];
-                counts[w][tid] = at;
-                at += c;
+    for (int c = 0; c < CHUNKS; ++c)
+        if (c < chunks) {
+            const uint32_t d = e[c] - from;
+            const bool live = d < 256 && e[c] != ~0u;
+            less += __popcll(__ballot(e[c] < from));
+            e[c] = 0;
+            if (__ballot(live)) {
+                const unsigned long long m = em_match((int)d & 255, live);
+                const int rank = __popcll(m & ((1ull << lane) - 1)), first = live ? count[d] : 0;
+                em_wave_order();
+                if (live && rank == 0) count[d] = first + __popcll(m);
+                em_wave_order();
+                if (live) e[c] = (uint32_t)(first + rank) << 9 | 256 | d;
             }
         }
-        __syncthreads();
-        for (int base = lo; base < hi; base += 64) {
-            const bool live = base + lane < hi;
-            const uint32_t e = live ? from[base + lane] : 0;
-            const int d = (int)(e >> shift) & 255;
-            const unsigned long long m = em_match(d, live);
-            const int rank = __popcll(m & ((1ull << lane) - 1));
-            const int first = live ? place[d] : 0;
-            __builtin_amdgcn_wave_barrier();
-            if (live && rank == 0) place[d] = first + __popcll(m);
-            __builtin_amdgcn_wave_barrier();
-            if (live) to[first + rank] = e;
+    if (lane == 0) smaller[wave] = less;
+    __syncthreads();
+    int all = 0;
+    if (tid < 256) {
+#pragma unroll
+        for (int w = 0; w < 16; ++w) all += counts[w][tid];
+        if (from + tid < vocab) there[from + tid] = all != 0;
+    }
+    int at = em_below(all, sums);
+#pragma unroll
+    for (int w = 0; w < 16; ++w) at += smaller[w];
+    if (tid < 256) {
+#pragma unroll
+        for (int w = 0; w < 16; ++w) {
+            const int c = counts[w][tid];
+            counts[w][tid] = at;
+            at += c;
         }
-        __syncthreads();
     }
-    for (int i = tid; i < n; i += 1024) {
-        const uint32_t e = entry[passes & 1][i], key = e >> EM_LDS_POS_BITS;
-        key_out[i] = key;
-        pos_out[i] = e & (EM_LDS_MAX - 1);
-        if (key < k.vocab) there[key] = 1;
-    }
+    __syncthreads();
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c)
+        if (c < chunks && e[c]) {
+            const int d = e[c] & 255, to = counts[wave][d] + (int)(e[c] >> 9);
+            key_out[to] = from + d;
+            pos_out[to] = (uint32_t)(lo + c * 64);
+        }
 }
 
 // Sums over the sorted entries: a wave takes a tile of them (at most 64) and one slice of channels, and writes the tokens that begin in its
@@ -551,16 +569,16 @@ __global__ void __launch_bounds__(256) k_embed_bwd_sum(const em_sum a, const T* 
 
 template <int W> struct alignas(4 * W) em_sums { float v[W]; };
 
-// sum of rows lo, lo + step, .. below hi of `rows`, channels c .. c + W - 1, added to s: 8 rows at a time (behind the last: the first again,
-// adding nothing)
+// sum of rows lo, lo + step, .. below hi of `rows`, channels c .. c + W - 1, added to s: 16 rows at a time (8: a join of 64 takes 0.8 us
+// more; behind the last: the first again, adding nothing)
 template <int W>
 __device__ __forceinline__ void em_rows(em_sums<W>& s, const float* __restrict__ rows, long long lo, long long hi, long long step, int C, int c) {
-    for (long long k = lo; k < hi; k += 8 * step) {
-        em_sums<W> v[8];
+    for (long long k = lo; k < hi; k += 16 * step) {
+        em_sums<W> v[16];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = *(const em_sums<W>*)(rows + (k + j * step < hi ? k + j * step : lo) * C + c);
+        for (int j = 0; j < 16; ++j) v[j] = *(const em_sums<W>*)(rows + (k + j * step < hi ? k + j * step : lo) * C + c);
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
+        for (int j = 0; j < 16; ++j)
 #pragma unroll
             for (int i = 0; i < W; ++i) s.v[i] += k + j * step < hi ? v[j].v[i] : 0.f;
     }
@@ -755,7 +773,7 @@ extern "C" int gd_embed(const void* ids, int ids64, int64_t n, const void* table
 
 struct em_plan {
     em_sort sort;
-    bool in_lds;
+    bool ranges;
     int passes, tile, tiles;
     size_t key[2], pos[2], table, there, head, tail, bytes;
 };
@@ -764,7 +782,7 @@ static em_plan em_plan_of(long long n, long long vocab, int C) {
     em_plan p = {};
     if (n <= EM_SCAN_MAX) return p;
     p.sort = em_sort_of(n);
-    p.in_lds = n <= EM_LDS_MAX && vocab < (1 << (32 - EM_LDS_POS_BITS));
+    p.ranges = em_by_ranges(n, vocab);
     p.passes = 1;
     while (p.passes < 4 && ((unsigned long long)vocab >> (8 * p.passes))) ++p.passes;
     // 64 entries a tile where they give each CU 32 waves (times the slices of 512 channels): a partial sum costs two entries' traffic.  With
@@ -813,9 +831,11 @@ extern "C" int gd_embed_bwd(const void* ids, int ids64, int64_t n, const void* d
         char* const ws = (char*)workspace;
         em_keys k = {in, nullptr, nullptr, (unsigned)vocab, padding};
         const int there_words = (int)((vocab + 3) / 4);
-        if (p.in_lds) {
+        if (p.ranges) {
             uint32_t *const key = (uint32_t*)(ws + p.key[0]), *const pos = (uint32_t*)(ws + p.pos[0]);
-            k_embed_sort_lds<<<1, 1024, 0, st>>>(k, (int)n, p.passes, key, pos, (unsigned char*)(ws + p.there), there_words);
+            const unsigned ranges = (unsigned)(vocab / 256 + 1);    // (with the key `vocab`)
+            if (n <= 8192) k_embed_sort_ranges<8><<<ranges, 1024, 0, st>>>(in, (int)n, (unsigned)vocab, padding, key, pos, (unsigned char*)(ws + p.there));
+            else k_embed_sort_ranges<EM_RANGE_MAX / 1024><<<ranges, 1024, 0, st>>>(in, (int)n, (unsigned)vocab, padding, key, pos, (unsigned char*)(ws + p.there));
             k.key = key;
             k.pos = pos;
         } else {
