@@ -515,10 +515,15 @@ extern "C" int gd_block_norm(const gd_block_norm_t* f, int dtype, void* stream) 
 }
 
 // As many workgroups as are resident at once: one a CU for the kernels with 16 channels or 512 threads a row and more (their registers leave
-// one wave a SIMD), two for the others.  Every further one is another row of partial sums to write and add.  At least 4 rows each.
-// (16384 x 1024 bf16 with gate and both norms: 256 workgroups 46 us, 512 53, 1024 69; 4096 x 4096 bf16: 41, 47, 59; 16384 x 1280 f32: 119, 109, 116.)
+// one wave a SIMD), two for the others.  Every further one is another row of partial sums to write and add.  At least 4 rows
+// each, but for the first ones: the 64 slots that k_block_norm_cols reads side by side cost no more than one (with four waves a row; where
+// one wave has a row and a workgroup four, 16: the rows of a gate each are worked on one after the other).
+// (16384 x 1024 bf16 with gate and both norms: 256 workgroups 46 us, 512 53, 1024 69; 4096 x 4096 bf16: 41, 47, 59; 16384 x 1280 f32: 119, 109, 116.
+// 4 samples of one row of 1280 with a gate each: in one workgroup 19 us, in four 11.5; 64 rows: 16 and 64 workgroups 15.4 and 12.2, of 1000
+// channels 11.8 and 12.7.)
 static long long bn_workgroups(long long rows, int C) {
-    const long long n = (rows + 3) / 4, most = (C > 512 && C <= 1024) || C > 2048 ? 256 : 512;
+    const long long first = C > 1024 ? 64 : 16, n = rows < first ? rows : rows < 4 * first ? first : (rows + 3) / 4;
+    const long long most = (C > 512 && C <= 1024) || C > 2048 ? 256 : 512;
     return n < most ? n : most;
 }
 

@@ -393,7 +393,7 @@ __global__ void __launch_bounds__(1024) k_embed_sort_move(const em_keys k, const
 
 // Fewer positions, in one launch: every workgroup looks through all ids and puts those of its own 256 tokens in their places, behind the
 // number of smaller ones, which it has counted on the way.  A thread keeps its ids in registers from the one look on, and one digit is left
-// to rank by.  (Bound by the workgroup with the padding and the most frequent words, which ranks most of the positions the others
+// to rank by.  (Bound by the workgroup with the padding and the most frequent words, which ranks most of the positions, where the others
 // find that they have none among 64, and in large tables by the looks.  The gradient (bf16, by this sort and by the passes above): 5400
 // positions and 12000 rows of 64 channels 25 and 36 us, 8192 26 and 37, 16384 35 and 39, 24000 44 and 40; 8192 positions and 300000 rows 30
 // and 46, 1000000 rows 52 and 50.)
