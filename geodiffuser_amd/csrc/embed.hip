@@ -8,8 +8,8 @@
 // Bound by HBM (dy once, the table's gradient once); for a few prompts by the launch.  Measured (MI355X; a large copy moves 4.9 TB/s):
 //   lookup, 1024 x 77 rows of 1280 f16 from a table of 126 MB       41 us: the 202 MB that it writes at 4.9 TB/s, the table out of the cache
 //   gradient, 4 x 77 rows into 49408 x 768 f32                       25 us: 152 MB of zeros at 6.1 TB/s, one launch
-//   gradient, 2048 x 77 rows of 1024 bf16 into 49408 rows            98 us for the sums (438 MB, 4.5 TB/s), 28 for the sort, 15 for the joins
-//   position gradient of the same                                    50 + 5 us (323 MB, a part of it still in the cache)
+//   gradient, 2048 x 77 rows of 1024 bf16 into 49408 rows            96 us for the sums (438 MB, 4.5 TB/s), 27 for the sort, 14 for the joins
+//   position gradient of the same                                    49 + 5 us (323 MB, a part of it still in the cache)
 #include "train_common.hpp"
 
 // A lane's N channels of a slice of 64 * N: one word of 16 bytes at any address (VEC), or, of rows shorter than a word, N single elements,
