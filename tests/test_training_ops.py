@@ -1131,3 +1131,21 @@ def test_rows_of_every_width_stay_in_their_place(ops, monkeypatch, dtype, C):
     for a, b in zip(plain, moved):
         # (the column sums and row sums may be dealt out otherwise; values of ~1 and sums of at most 1100 of them)
         assert a.shape == b.shape and bool(((a.double() - b.double()).abs() <= fi.eps * b.double().abs() + 1100 * 64 * U32 * 8 + fi.smallest_normal).all())
+
+
+@gpu
+@pytest.mark.parametrize("n,V", [(1025, 1), (1025, 255), (1025, 256), (1025, 257), (4096, (1 << 20) - 1), (8192, 1 << 19), (8192, (1 << 19) + 1), (8193, 5000), (16384, 1 << 18), (16384, 300), (16385, 300)])
+@pytest.mark.parametrize("wide", [False, True])
+def test_embedding_gradient_at_the_borders_of_its_sorts(ops, n, V, wide):
+    """Sizes beside each choice of sort, 32- and 64-bit ids; frequent tokens, all of one block of 256, ids outside the table and a padding row."""
+    g = _gen(n + V)
+    dy = _randn(g, n, 3)
+    for kind in range(4):
+        ids = (V * torch.rand(n, generator=g, dtype=torch.float64) ** (1, 6, 1, 1)[kind]).long().clamp(0, V - 1)
+        if kind == 1:
+            ids[torch.rand(n, generator=g) < 0.5] = V // 2
+        elif kind == 2:
+            ids = V - 1 - ids % min(V, 200)
+        elif kind == 3:
+            ids[::3] = torch.tensor([-1, V, -(1 << 31), (1 << 31) - 1])[torch.arange(0, n, 3) // 3 % 4]
+        _check_embed_bwd(ops, (ids if wide else ids.int()).to(DEV), dy, V, scale=0.5, padding_idx=None if kind == 0 else V // 2)
