@@ -1123,6 +1123,15 @@ def _like(t: Optional[torch.Tensor], name: str, dtype, dev: int, shape) -> int:
     return t.data_ptr()
 
 
+def _at_most(value: int, most: int, what: str) -> None:
+    """Sizes that the library takes as 32-bit numbers are checked here: ctypes cuts larger ones off without a word."""
+    if value > most:
+        raise _lib.GeodiffError(f"{what}={value}: at most {most}")
+
+
+_EMBED_MAX_C, _INT32_MAX = 1 << 20, (1 << 31) - 1
+
+
 def _token_ids(ids: torch.Tensor, ref: torch.Tensor) -> int:
     _need(ids, "ids")
     if ids.dtype not in (torch.int64, torch.int32) or ids.device != ref.device or ids.dim() < 1:
@@ -1142,6 +1151,7 @@ def embed_tokens(ids, table, pos=None, scale: float = 1.0):
     if table.dim() != 2 or (pos is not None and (pos.dim() != 2 or pos.shape[0] < L)):
         raise _lib.GeodiffError("embed_tokens: table is [V, C], pos is [>= L, C]")
     V, C = table.shape
+    _at_most(C, _EMBED_MAX_C, "embed_tokens: C")
     pp = 0 if pos is None else _like(pos, "pos", table.dtype, table.get_device(), (pos.shape[0], C))
     y = torch.empty(*shape, C, dtype=table.dtype, device=table.device)
     n = ids.numel()
@@ -1163,6 +1173,7 @@ def embed_tokens_bwd(ids, dy, vocab: int, scale: float = 1.0, padding_idx: Optio
     if padding_idx is not None and not 0 <= padding_idx < vocab:
         raise _lib.GeodiffError("embed_tokens_bwd: padding_idx must be a row of the table")
     C, n = dy.shape[-1], ids.numel()
+    _at_most(C, _EMBED_MAX_C, "embed_tokens_bwd: C")
     d = torch.empty(vocab, C, dtype=dy.dtype, device=dy.device)
     if vocab and C:
         nbytes = lib.gd_embed_bwd_workspace_bytes(n, vocab, C)
@@ -1181,6 +1192,8 @@ def embed_positions_bwd(dy, pos_rows: int):
     if dy.dim() < 2 or pos_rows < dy.shape[-2]:
         raise _lib.GeodiffError("embed_positions_bwd: dy is [..., L, C] with L <= pos_rows")
     L, C = dy.shape[-2:]
+    _at_most(C, _EMBED_MAX_C, "embed_positions_bwd: C")
+    _at_most(pos_rows, _INT32_MAX, "embed_positions_bwd: pos_rows")
     d = torch.empty(pos_rows, C, dtype=dy.dtype, device=dy.device)
     if pos_rows and C:
         B = dy.numel() // (L * C) if L else 0
@@ -1201,6 +1214,9 @@ class Norm(NamedTuple):
 _NORM_KINDS = {"layer": _lib.GD_NORM_LAYER, "rms": _lib.GD_NORM_RMS}
 
 
+_BLOCK_NORM_MAX_C = 16384
+
+
 def _block_norm_x(x):
     """-> dtype code, shape, C, rows, GPU of block_norm's x"""
     _need(x, "x")
@@ -1208,6 +1224,7 @@ def _block_norm_x(x):
     C = shape[-1] if shape else 0
     if C == 0:
         raise _lib.GeodiffError("block_norm: x is [..., C]")
+    _at_most(C, _BLOCK_NORM_MAX_C, "block_norm: C")
     return _dt(x, "x"), shape, C, x.numel() // C, x.get_device()
 
 
