@@ -1149,3 +1149,16 @@ def test_embedding_gradient_at_the_borders_of_its_sorts(ops, n, V, wide):
         elif kind == 3:
             ids[::3] = torch.tensor([-1, V, -(1 << 31), (1 << 31) - 1])[torch.arange(0, n, 3) // 3 % 4]
         _check_embed_bwd(ops, (ids if wide else ids.int()).to(DEV), dy, V, scale=0.5, padding_idx=None if kind == 0 else V // 2)
+
+
+@gpu
+def test_sizes_beyond_32_bits_are_refused(ops):
+    """Widths and row counts that the library takes as 32-bit numbers: 2^32 + 8 channels must not be taken for 8."""
+    big = torch.empty((1 << 32) + 8, dtype=torch.float16, device=DEV)
+    one, ids = big.view(1, -1), torch.zeros(1, dtype=torch.long, device=DEV)
+    few = torch.zeros(1, 1, 1, dtype=torch.float16, device=DEV)
+    for call in (lambda: ops.block_norm(one, None, ops.Norm("layer")), lambda: ops.block_norm_bwd(one, None, one, None, torch.zeros(1, 4, device=DEV), ops.Norm("layer")),
+                 lambda: ops.embed_tokens(ids, one), lambda: ops.embed_tokens_bwd(ids, one, 1), lambda: ops.embed_positions_bwd(big.view(1, -1, 1), (1 << 32) + 8),
+                 lambda: ops.embed_positions_bwd(big.view(1, 1, -1), 1), lambda: ops.embed_positions_bwd(few, (1 << 32) + 8)):
+        with pytest.raises(GeodiffError, match="at most"):
+            call()
