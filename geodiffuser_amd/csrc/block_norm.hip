@@ -161,7 +161,7 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) k_block_norm(const gd_b
     __shared__ float lds[64];
     int turn = 0;
     const int t = threadIdx.x % TPR, C = a.C;
-    const long long row = (long long)blockIdx.x * RPB + (TPR < 256 ? __builtin_amdgcn_readfirstlane(threadIdx.x / TPR) : 0);
+    const long long row = workgroup() * RPB + (TPR < 256 ? __builtin_amdgcn_readfirstlane(threadIdx.x / TPR) : 0);
     if (row >= a.rows) return;                               // TPR >= 256: the whole workgroup has one row
     // everything that the row needs is on its way before the first sum waits for x
     PART x, res, gate, og, ob, eg, eb;
@@ -487,13 +487,13 @@ static void bn_launch(const gd_block_norm_t& a, hipStream_t st) {
     const bool stream = streams_past_cache((double)a.rows * a.C * sizeof(T) * (1 + !!a.res + !!a.s + !!a.y));
     const bool words = bn_words(a, sizeof(T));
     if (a.C < word16<T>::N) {
-        k_block_norm<T, 64, 8, BN_ELEMENTS><<<(unsigned)((a.rows + 3) / 4), 256, 0, st>>>(a, stream);
+        k_block_norm<T, 64, 8, BN_ELEMENTS><<<grid_of((a.rows + 3) / 4), 256, 0, st>>>(a, stream);
         return;
     }
 #define BN_GO(TPR, N)                                                                                         \
     do {                                                                                                      \
         constexpr int rpb = TPR < 256 ? 256 / TPR : 1;                                                        \
-        const unsigned grid = (unsigned)((a.rows + rpb - 1) / rpb);                                           \
+        const dim3 grid = grid_of((a.rows + rpb - 1) / rpb);                                                  \
         if (words) k_block_norm<T, TPR, N, BN_WORDS><<<grid, rpb * TPR, 0, st>>>(a, stream);                  \
         else k_block_norm<T, TPR, N, BN_ODD><<<grid, rpb * TPR, 0, st>>>(a, stream);                          \
     } while (0)

@@ -98,7 +98,7 @@ __global__ void __launch_bounds__(256) k_embed(const em_ids ids, long long n, co
                                                float scale, bool stream, int shift, T* y) {
     constexpr int W = VEC ? word16<T>::N : 1, BATCH = VEC && sizeof(T) == 2 ? 2 : 4;       // (f16, 1280 channels: 2 words 43.5 us, 4 47.6; f32: 43 and 41)
     const int lane = threadIdx.x & 63, units = em_units<T, VEC>(C), lanes = 1 << shift;
-    const long long row = (((long long)blockIdx.x * 4 + (threadIdx.x >> 6)) << (6 - shift)) + (lane >> shift);
+    const long long row = ((workgroup() * 4 + (threadIdx.x >> 6)) << (6 - shift)) + (lane >> shift);
     if (row >= n) return;
     const long long id = ids[row];
     const bool in = id >= 0 && id < V;
@@ -157,10 +157,10 @@ __global__ void __launch_bounds__(EM_SCAN_MAX) k_embed_bwd_scan(const em_ids ids
     __shared__ int list[EM_SCAN_MAX], count[WAVES];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int slices = (C + COLS::SLICE - 1) / COLS::SLICE;
-    const long long owners = (long long)n * slices;
+    const long long owners = (long long)n * slices, wg = workgroup();
     const long long mine = tid < n ? ids[tid] : -1;
-    if (blockIdx.x < owners) {
-        const int first = (int)(blockIdx.x / slices), sl = (int)(blockIdx.x % slices);
+    if (wg < owners) {                                       // (at most 1024 positions of 2^14 slices)
+        const int first = (int)((unsigned)wg / slices), sl = (int)((unsigned)wg % slices);
         const long long id = ids[first];
         if (id < 0 || id >= V || id == padding) return;
         const bool same = tid < n && mine == id;
@@ -204,7 +204,8 @@ __global__ void __launch_bounds__(EM_SCAN_MAX) k_embed_bwd_scan(const em_ids ids
         }
         return;
     }
-    const long long v0 = ((long long)blockIdx.x - owners) * zero_rows;
+    const long long v0 = (wg - owners) * zero_rows;
+    if (v0 >= V) return;
     const int rows = v0 + zero_rows < V ? zero_rows : (int)(V - v0);
     if (tid < rows) list[tid] = 0;
     __syncthreads();
@@ -706,7 +707,7 @@ template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) k_embed_pos_bwd(const T* __restrict__ dy, long long B, long long width, long long out_width, long long per, bool stream,
                                                        float* __restrict__ part, T* __restrict__ dpos) {
     constexpr int N = VEC ? word16<T>::N : 1;
-    const long long at = em_pos_start<T, VEC>((long long)blockIdx.x * 256 + threadIdx.x, width, out_width);
+    const long long at = em_pos_start<T, VEC>((((long long)blockIdx.z << 20) + blockIdx.x) * 256 + threadIdx.x, width, out_width);
     if (at >= out_width) return;
     float acc[N] = {};
     if (at < width) {
@@ -729,7 +730,7 @@ __global__ void __launch_bounds__(256) k_embed_pos_bwd(const T* __restrict__ dy,
 
 template <typename T>
 __global__ void __launch_bounds__(256) k_embed_pos_join(const float* __restrict__ part, int parts, long long width, long long out_width, T* __restrict__ dpos) {
-    const long long at = (long long)blockIdx.x * 256 + threadIdx.x;
+    const long long at = workgroup() * 256 + threadIdx.x;
     if (at >= out_width) return;
     dpos[at] = to_storage<T>(at < width ? sum_strided(part + at, width, 0, parts, 1) : 0.f);
 }
@@ -766,7 +767,7 @@ extern "C" int gd_embed(const void* ids, int ids64, int64_t n, const void* table
     const int shift = em_lane_shift(vec ? (C * EM_ELEM(dtype) + 15) / 16 : C);
     const long long waves = (n + (64 >> shift) - 1) >> (6 - shift);
     const bool past = streams_past_cache((double)EM_ELEM(dtype) * C * ((double)n + (n < vocab ? n : vocab)));
-    EM_LAUNCH(dtype, vec, (k_embed<T, VEC><<<(unsigned)((waves + 3) / 4), 256, 0, st>>>(em_ids{ids, ids64}, n, (const T*)table, (const T*)pos, L, (int)vocab, C, scale, past, shift, (T*)y)));
+    EM_LAUNCH(dtype, vec, (k_embed<T, VEC><<<grid_of((waves + 3) / 4), 256, 0, st>>>(em_ids{ids, ids64}, n, (const T*)table, (const T*)pos, L, (int)vocab, C, scale, past, shift, (T*)y)));
     GD_CHECK_LAUNCH("gd_embed");
     return GD_OK;
 }
@@ -824,10 +825,12 @@ extern "C" int gd_embed_bwd(const void* ids, int ids64, int64_t n, const void* d
     if (!p.bytes) {
         const long long grid = n * slices + zeros;
         GD_REQUIRE(grid < (1ll << 31), GD_EUNSUPPORTED, "gd_embed_bwd: table too large");
-        EM_LAUNCH(dtype, vec, (k_embed_bwd_scan<T, VEC><<<(unsigned)grid, EM_SCAN_MAX, 0, st>>>(in, (int)n, (const T*)dy, (int)vocab, C, padding, scale, past, zero_rows, shift, (T*)dtable)));
+        EM_LAUNCH(dtype, vec, (k_embed_bwd_scan<T, VEC><<<grid_of(grid), EM_SCAN_MAX, 0, st>>>(in, (int)n, (const T*)dy, (int)vocab, C, padding, scale, past, zero_rows, shift, (T*)dtable)));
     } else {
         const long long grid = ((long long)p.tiles * slices + 3) / 4 + zeros;
-        GD_REQUIRE(grid < (1ll << 31) && (long long)p.tiles * ((C + 255) / 256) < (1ll << 30), GD_EUNSUPPORTED, "gd_embed_bwd: too many positions for this width");
+        // (the launches of 256 threads below: each less than 2^32)
+        GD_REQUIRE(grid < (1ll << 24) && p.tiles + (p.tiles + EM_GROUP - 1ll) / EM_GROUP * ((C + 255) / 256) < (1ll << 24), GD_EUNSUPPORTED,
+                   "gd_embed_bwd: too many positions for this width");
         char* const ws = (char*)workspace;
         em_keys k = {in, nullptr, nullptr, (unsigned)vocab, padding};
         const int there_words = (int)((vocab + 3) / 4);
@@ -890,12 +893,13 @@ extern "C" int gd_embed_pos_bwd(const void* dy, int64_t B, int L, int C, int pos
     const int word = vec ? 16 / EM_ELEM(dtype) : 1;
     const long long words = (width + word - 1) / word + (out_width - width + word - 1) / word, grid = (words + 255) / 256;
     GD_REQUIRE((out_width + 255) / 256 < (1ll << 31), GD_EUNSUPPORTED, "gd_embed_pos_bwd: too many positions for this width");
+    const dim3 g1 = grid_of(grid);
     float* const part = parts > 1 ? (float*)workspace : nullptr;
     hipStream_t st = as_stream(stream);
-    EM_LAUNCH(dtype, vec, (k_embed_pos_bwd<T, VEC><<<dim3((unsigned)grid, parts), 256, 0, st>>>((const T*)dy, B, width, out_width, per,
+    EM_LAUNCH(dtype, vec, (k_embed_pos_bwd<T, VEC><<<dim3(g1.x, parts, g1.y), 256, 0, st>>>((const T*)dy, B, width, out_width, per,
                       streams_past_cache((double)B * width * EM_ELEM(dtype)), part, (T*)dpos)));
     if (parts > 1) {
-        const unsigned g = (unsigned)((out_width + 255) / 256);
+        const dim3 g = grid_of((out_width + 255) / 256);
         if (dtype == GD_F32) k_embed_pos_join<float><<<g, 256, 0, st>>>(part, parts, width, out_width, (float*)dpos);
         else if (dtype == GD_F16) k_embed_pos_join<f16_t><<<g, 256, 0, st>>>(part, parts, width, out_width, (f16_t*)dpos);
         else k_embed_pos_join<bf16_t><<<g, 256, 0, st>>>(part, parts, width, out_width, (bf16_t*)dpos);

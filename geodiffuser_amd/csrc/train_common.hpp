@@ -21,6 +21,13 @@ template <typename T> __device__ __forceinline__ u32x4 row_word_shift(u32x4 w, i
     return __builtin_bit_cast(u32x4, __builtin_bit_cast(unsigned __int128, w) >> ((c - row_word_start<T>(c, C)) * 8 * (int)sizeof(T)));
 }
 
+// A launch has fewer than 2^32 threads along an axis: more are cut off without an error (67 million rows of 8 channels, a wave each, are as
+// many).  Launches whose number of workgroups grows with the call lie in two axes from 2^20 on; workgroups behind the last one end at once.
+static inline dim3 grid_of(long long workgroups) {
+    return dim3((unsigned)(workgroups < (1 << 20) ? workgroups : 1 << 20), (unsigned)((workgroups + (1 << 20) - 1) >> 20));
+}
+__device__ __forceinline__ long long workgroup() { return ((long long)blockIdx.y << 20) + blockIdx.x; }
+
 // The one rounding of a result to its storage type.  f16: the binary32 value is kept out of the compiler's sight, which otherwise folds
 // the last multiplication and the conversion of SINGLE elements into v_fma_mixlo_f16 (rounding once from the exact product) but not
 // those of pairs: a result's bits would depend on whether its tensor is aligned.

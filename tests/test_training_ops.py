@@ -1162,3 +1162,48 @@ def test_sizes_beyond_32_bits_are_refused(ops):
                  lambda: ops.embed_positions_bwd(big.view(1, 1, -1), 1), lambda: ops.embed_positions_bwd(few, (1 << 32) + 8)):
         with pytest.raises(GeodiffError, match="at most"):
             call()
+
+
+@gpu
+def test_launches_of_more_than_2_32_threads(ops):
+    """A launch has fewer than 2^32 threads along an axis: 2^26 rows of a wave each, and 2^29 of eight lanes, reach that."""
+    R = (1 << 26) + 5
+    g = _gen(3)
+    x = torch.zeros(R, 8, dtype=torch.float16, device=DEV)
+    x[-9:] = x[:9] = tail = _randn(g, 9, 8, dtype=torch.float16)
+    n = ops.Norm("layer", _randn(g, 8, dtype=torch.float16), None)
+    _, y, st = ops.block_norm(x, None, n)
+    _, y2, st2 = ops.block_norm(tail, None, n)
+    for at in (slice(0, 9), slice(R - 9, R)):
+        assert torch.equal(y[at], y2) and torch.equal(st[at], st2)
+    assert not bool(y[9:-9].any())
+    dx = ops.block_norm_bwd(x, None, x, None, st, n, need=["dx"])["dx"]
+    assert torch.equal(dx[-9:], ops.block_norm_bwd(tail, None, tail, None, st2, n, need=["dx"])["dx"])
+    del x, y, st, dx
+    N = (1 << 29) + 3
+    table = _randn(g, 5, 7, dtype=torch.float16)
+    ids = torch.zeros(N, dtype=torch.int32, device=DEV)
+    ids[-1], ids[-2], ids[1] = 4, 3, 2
+    y = ops.embed_tokens(ids, table)
+    assert torch.equal(y[-2:], table[[3, 4]]) and torch.equal(y[:2], table[[0, 2]])
+    del ids
+    for part in y[2:-2].split(1 << 26):
+        assert bool((part == table[0]).all())
+    del y, part
+    V = (1 << 30) + 7                                        # zero rows: 2^22 workgroups of 1024 threads and more
+    torch.full((V, 1), 7.0, dtype=torch.float16, device=DEV)  # (what the gradient's memory holds before)
+    d = ops.embed_tokens_bwd(torch.tensor([V - 1, 3, V - 1], device=DEV), torch.ones(3, 1, dtype=torch.float16, device=DEV), V)
+    assert float(d[-1]) == 2.0 and float(d[3]) == 1.0 and int((d != 0).sum()) == 2
+    P = (1 << 31) - 1                                        # position rows: 6 billion single elements, summed by one workgroup a column and by several
+    for B in (1, 100):
+        torch.full((P, 3), 7.0, dtype=torch.float16, device=DEV)
+        d = ops.embed_positions_bwd(torch.ones(B, 2, 3, dtype=torch.float16, device=DEV), P)
+        assert bool((d[:2] == B).all()) and int((d[2:] != 0).sum()) == 0
+
+
+def test_gradient_launches_beyond_2_32_threads_are_refused():
+    """(on the host, with addresses that are never followed) 2^30 - 1 positions need 2^24 workgroups of 256 threads for the joins."""
+    from geodiffuser_amd import _lib
+    lib = _lib.load()
+    A, n = 1 << 20, (1 << 30) - 1
+    assert lib.gd_embed_bwd(ctypes.c_void_p(A), 1, n, ctypes.c_void_p(A), 100, 1, -1, 1.0, ctypes.c_void_p(A), ctypes.c_void_p(A), lib.gd_embed_bwd_workspace_bytes(n, 100, 1), 2, None) == -4
