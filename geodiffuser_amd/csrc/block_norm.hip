@@ -475,6 +475,8 @@ static int bn_check(const gd_block_norm_t* f, int dtype, const char* who) {
     GD_REQUIRE(f->C <= BN_MAX_C, GD_EUNSUPPORTED, "%s: at most %d channels (C=%d)", who, BN_MAX_C, f->C);
     GD_REQUIRE(f->rows < (1ll << 31), GD_EUNSUPPORTED, "%s: too many rows", who);
     GD_REQUIRE(f->post_kind >= 0 && f->post_kind <= GD_NORM_RMS && f->pre_kind >= 0 && f->pre_kind <= GD_NORM_RMS, GD_EINVAL, "%s: bad norm kind", who);
+    // (the forward would not apply them, the backward would)
+    GD_REQUIRE((f->post_kind || (!f->post_gamma && !f->post_beta)) && (f->pre_kind || (!f->pre_gamma && !f->pre_beta)), GD_EINVAL, "%s: gamma or beta without its norm", who);
     GD_REQUIRE(!f->gate || (f->rows_per_gate > 0 && f->rows % f->rows_per_gate == 0 && f->gate_ld >= f->C), GD_EINVAL,
                "%s: gate rows must divide the rows and be at least C apart", who);
     GD_REQUIRE(!f->gate || f->rows / f->rows_per_gate <= 65535 - BN_SUMS, GD_EUNSUPPORTED, "%s: at most %d gate rows", who, 65535 - BN_SUMS);

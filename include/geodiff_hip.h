@@ -556,7 +556,7 @@ int gd_embed_pos_bwd(const void* dy, int64_t B, int L, int C, int pos_rows, void
 
 /* h = post(x);  s = res_scale * res + gate * h;  y = pre(s) for rows of C <= 16384 channels.
  *   kinds: GD_NORM_NONE, GD_NORM_LAYER (xh = (v - mean) / sqrt(var + eps)), GD_NORM_RMS (xh = v / sqrt(mean v^2 + eps)), then
- *   xh * gamma + beta; gamma, beta [C] or NULL (1, 0).  gate: one row of C for every rows_per_gate rows, gate_ld elements apart, or
+ *   xh * gamma + beta; gamma, beta [C] or NULL (1, 0), NULL without the norm.  gate: one row of C for every rows_per_gate rows, gate_ld elements apart, or
  *   NULL (1).  res NULL: s = gate * h.  s may be NULL; y goes with pre_kind.  stats [rows, 4] f32 (mean, 1 / deviation of x, then of
  *   s; 0, 1 for a norm that is not there; NULL: not kept) is what the backward needs.  y is computed from the unrounded s.
  *   No output may overlap an input. */

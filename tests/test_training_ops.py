@@ -1207,3 +1207,15 @@ def test_gradient_launches_beyond_2_32_threads_are_refused():
     lib = _lib.load()
     A, n = 1 << 20, (1 << 30) - 1
     assert lib.gd_embed_bwd(ctypes.c_void_p(A), 1, n, ctypes.c_void_p(A), 100, 1, -1, 1.0, ctypes.c_void_p(A), ctypes.c_void_p(A), lib.gd_embed_bwd_workspace_bytes(n, 100, 1), 2, None) == -4
+
+
+def test_block_norm_refuses_parameters_of_a_norm_that_is_not_there():
+    """(on the host, with addresses that are never followed) the forward would leave them out and the backward apply them."""
+    from geodiffuser_amd import _lib
+    lib = _lib.load()
+    A = 1 << 20
+    ok = dict(x=A, res=A, gate=A, y=A, s=A, stats=A, rows=8, rows_per_gate=8, gate_ld=64, C=64, pre_kind=1, res_scale=1.0)
+    for bad in (dict(post_gamma=A), dict(post_beta=A), dict(pre_kind=0, y=0, pre_gamma=A), dict(pre_kind=0, y=0, pre_beta=A)):
+        f = _lib.GdBlockNorm(**{**ok, **bad})
+        assert lib.gd_block_norm(ctypes.byref(f), 2, None) == -1, bad
+        assert lib.gd_block_norm_bwd(ctypes.byref(_lib.GdBlockNormBwd(f=f, gs=A, dx=A)), None, 0, 2, None) == -1, bad
