@@ -69,11 +69,12 @@ class TextEncoder(nn.Module):
         self.ln_f = nn.LayerNorm(width)
 
     def _embed(self, input_ids):
-        """Token + position embedding: one launch on the GPU (gd_embed, the same rounding), with its gradient where table or positions learn."""
+        """Token + position embedding: one launch on the GPU (gd_embed, the same rounding), with its gradient where table or positions learn.  An id
+        outside the table gives a row of NaN there."""
         w, pos = self.tok.weight, self.pos.to(self.tok.weight.dtype)
         tok = self.tok                                       # anything that changes what the module does keeps its own call
-        stock = (type(tok) is nn.Embedding and "forward" not in tok.__dict__ and tok.padding_idx is None and tok.max_norm is None and not tok.sparse
-                 and not tok.scale_grad_by_freq and not (tok._forward_hooks or tok._forward_pre_hooks or tok._backward_hooks or tok._backward_pre_hooks))
+        stock = (training.in_plain_torch(input_ids, w, pos) and training.is_stock(tok, nn.Embedding) and tok.padding_idx is None and tok.max_norm is None
+                 and not tok.sparse and not tok.scale_grad_by_freq)
         if stock and w.is_cuda and input_ids.device == pos.device == w.device and w.dtype in (torch.float16, torch.bfloat16, torch.float32) and w.is_contiguous():
             return training.embed_tokens(input_ids.contiguous(), w, pos.contiguous())
         return self.tok(input_ids) + pos[: input_ids.shape[1]]

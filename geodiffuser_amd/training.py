@@ -9,9 +9,29 @@ from __future__ import annotations
 from typing import Iterable, Optional, Union
 
 import torch
+from torch.autograd import forward_ad
+from torch.nn.modules import module as _module
 
 from . import ops
 from .ops import Norm  # noqa: F401 - part of this module's interface
+
+_PLAIN_TYPES = (torch.Tensor, torch.nn.Parameter)
+
+
+def in_plain_torch(*tensors: torch.Tensor) -> bool:
+    """Whether these are ordinary tensors of an ordinary eager pass, which is what a kernel that is handed addresses can serve.  Where not - under
+    torch.func.grad / vmap / jvp, forward-mode differentiation, a dispatch mode (fake tensors, make_fx, counters), a jit or compiler trace,
+    for tensor subclasses - the framework's modules keep to torch's own operations."""
+    if (torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack() or torch._C._functorch.peek_interpreter_stack() is not None
+            or forward_ad._current_level >= 0 or torch._C._get_tracing_state() is not None):
+        return False
+    return all(type(t) in _PLAIN_TYPES and not torch._C._functorch.is_legacy_batchedtensor(t) for t in tensors)
+
+
+def is_stock(module: torch.nn.Module, kind: type) -> bool:
+    """Whether calling the module runs kind.forward and nothing else: no subclass, replaced ``forward``, or hook of its own or of all modules."""
+    return (type(module) is kind and "forward" not in module.__dict__ and not _module._has_any_global_hook()
+            and not (module._forward_hooks or module._forward_pre_hooks or module._backward_hooks or module._backward_pre_hooks))
 
 
 class _EmbedFn(torch.autograd.Function):
@@ -70,14 +90,16 @@ def block_norm(x, res, pre: Optional[Norm], post: Optional[Norm] = None, gate=No
 
 def fuses_norms(x, norms) -> bool:
     """Whether a pass over x differentiates w.r.t. the weights of these norms and ``block_norm`` takes them: affine nn.LayerNorms of x's dtype and
-    device that nothing (a hook, a replaced ``forward``, autocast) makes into something else.  Norms that do not learn keep their path."""
+    device that nothing (a hook, a replaced ``forward``, autocast, a transform) makes into something else.  Norms that do not learn keep
+    their path."""
+    if not in_plain_torch(x):
+        return False
     if not (torch.is_grad_enabled() and x.is_cuda and x.is_contiguous() and x.shape[-1] <= 16384 and x.numel() > 0
             and x.dtype in (torch.float16, torch.bfloat16, torch.float32) and not torch.is_autocast_enabled()):
         return False
     return (any(p.requires_grad for n in norms for p in n.parameters())
-            and all(type(n) is torch.nn.LayerNorm and "forward" not in n.__dict__
-                    and not (n._forward_hooks or n._forward_pre_hooks or n._backward_hooks or n._backward_pre_hooks) for n in norms)
-            and all(p.dtype == x.dtype and p.device == x.device and p.is_contiguous() for n in norms for p in n.parameters()))
+            and all(is_stock(n, torch.nn.LayerNorm) for n in norms)
+            and all(in_plain_torch(p) and p.dtype == x.dtype and p.device == x.device and p.is_contiguous() for n in norms for p in n.parameters()))
 
 
 def layer_norm_of(module: torch.nn.LayerNorm) -> Norm:

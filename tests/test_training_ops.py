@@ -1219,3 +1219,119 @@ def test_block_norm_refuses_parameters_of_a_norm_that_is_not_there():
         f = _lib.GdBlockNorm(**{**ok, **bad})
         assert lib.gd_block_norm(ctypes.byref(f), 2, None) == -1, bad
         assert lib.gd_block_norm_bwd(ctypes.byref(_lib.GdBlockNormBwd(f=f, gs=A, dx=A)), None, 0, 2, None) == -1, bad
+
+
+class _NoAttention(torch.nn.Module):
+    """Stands where a text layer has its attention: one product, which every transform of torch can follow."""
+
+    def __init__(self, d):
+        super().__init__()
+        self.lin = torch.nn.Linear(d, d)
+
+    def forward(self, q, k, v, attn_mask=None, need_weights=False):
+        return torch.tanh(self.lin(q)), None
+
+
+def _small_tower(dev, dtype=torch.float32):
+    from geodiffuser_amd.pipeline import TextEncoder
+    torch.manual_seed(7)
+    te = TextEncoder(width=32, layers=1, heads=2, vocab=50, max_len=12)
+    te.layers[0].attn = _NoAttention(32)
+    return te.to(dev, dtype)
+
+
+def _tower_views(te, ids):
+    """What torch's transforms say of the tower: name -> a list of tensors."""
+    from torch.autograd import forward_ad
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    params = {k: p.detach() for k, p in te.named_parameters()}
+    call = lambda p, i: torch.func.functional_call(te, p, (i,))[0]
+    loss = lambda p, i: call(p, i).square().sum()
+    t = {k: torch.sin(torch.arange(p.numel(), device=p.device, dtype=p.dtype)).view(p.shape) for k, p in params.items()}
+
+    def dual():
+        with forward_ad.dual_level():
+            return [forward_ad.unpack_dual(call({k: forward_ad.make_dual(p, t[k]) for k, p in params.items()}, ids)).tangent.clone()]
+
+    def fake():
+        with FakeTensorMode(allow_non_fake_inputs=True) as mode:
+            y = te(mode.from_tensor(ids))[0]
+        assert type(y).__name__ == "FakeTensor"
+        return [torch.zeros(y.shape)]
+
+    def second(keys=("tok.weight", "pos", "layers.0.ln1.weight", "ln_f.bias", "layers.0.fc1.weight")):
+        """gradient of the gradient's inner product with t"""
+        p = {k: v.clone().requires_grad_() for k, v in params.items()}
+        g = torch.autograd.grad(loss(p, ids), [p[k] for k in keys], create_graph=True)
+        return list(torch.autograd.grad(sum((a * t[k]).sum() for a, k in zip(g, keys)), [p[k] for k in keys]))
+
+    def batched():
+        p = {k: v.clone().requires_grad_() for k, v in params.items()}
+        y = call(p, ids)
+        return list(torch.autograd.grad(y, list(p.values()), torch.stack([y.detach().cos(), y.detach().sin()]), is_grads_batched=True))
+
+    return {
+        "grad": lambda: list(torch.func.grad(loss)(params, ids).values()),
+        "vmap": lambda: [torch.func.vmap(call, in_dims=(None, 0))(params, ids[:, None])],
+        "vmap of grad": lambda: list(torch.func.vmap(torch.func.grad(loss), in_dims=(None, 0))(params, ids[:, None]).values()),
+        "jvp": lambda: [torch.func.jvp(lambda p: call(p, ids), (params,), (t,))[1]],
+        "dual": dual, "fake": fake, "second": second, "batched": batched,
+        "traced": lambda: [torch.jit.trace(te, (ids,), strict=False, check_trace=False)(ids.flip(0))[0]],
+        "compiled": lambda: [torch.compile(te, backend="eager", fullgraph=True)(ids)[0]],
+    }
+
+
+_VIEWS = ["grad", "vmap", "vmap of grad", "jvp", "dual", "fake", "traced", "compiled"]
+
+
+@gpu
+@pytest.mark.parametrize("view", _VIEWS)
+def test_text_tower_under_transforms(ops, view):
+    """torch's transforms reach through the tower on the GPU as they do on the CPU in 64 bits.  f32: fewer than 60 roundings lie on a path forward
+    and back, each product adding at most a few 2^-24 sqrt(32), and as many again for a second derivative: 60 * 16 * 2 of 2^-24 in relative
+    2-norm, over all results of a view together."""
+    torch._dynamo.reset()
+    ids = torch.randint(0, 50, (3, 9), generator=_gen(2))
+    ids[:, 5:] = 0
+    te = _small_tower(DEV)
+    got = _tower_views(te, ids.to(DEV))[view]()
+    want = _tower_views(_small_tower("cpu").double(), ids)[view]()
+    assert len(got) == len(want) and all(a.shape == b.shape for a, b in zip(got, want))
+    flat = lambda ts: torch.cat([t.detach().cpu().double().flatten() for t in ts])
+    a, b = flat(got), flat(want)
+    assert float((a - b).norm()) <= 2 * 60 * 16 * U32 * float(b.norm())
+
+
+def test_what_is_taken_for_an_ordinary_pass():
+    from torch.autograd import forward_ad
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from geodiffuser_amd import training as T
+    x, p = torch.ones(3), torch.nn.Parameter(torch.ones(3))
+    seen = []
+    look = lambda t: seen.append(T.in_plain_torch(t)) or t.sum()
+    assert T.in_plain_torch(x, p) and T.in_plain_torch()
+    with torch.no_grad(), torch.device("cpu"):
+        assert T.in_plain_torch(x)
+    torch.func.grad(look)(x), torch.func.vmap(look)(x), torch.func.jvp(look, (x,), (x,)), torch.jit.trace(look, (x,), check_trace=False)
+    with forward_ad.dual_level():
+        look(forward_ad.make_dual(x, x))
+    with FakeTensorMode() as mode:
+        look(mode.from_tensor(x))
+    fake = mode.from_tensor(x)
+
+    class Sub(torch.Tensor):
+        pass
+    seen += [T.in_plain_torch(x, fake), T.in_plain_torch(x.as_subclass(Sub))]
+    assert len(seen) == 8 and not any(seen) and T.in_plain_torch(x)
+    ln = torch.nn.LayerNorm(3)
+    assert T.is_stock(ln, torch.nn.LayerNorm) and not T.is_stock(ln, torch.nn.Embedding)
+    h = torch.nn.modules.module.register_module_forward_hook(lambda *a: None)
+    assert not T.is_stock(ln, torch.nn.LayerNorm)
+    h.remove()
+    for register in (ln.register_forward_hook, ln.register_forward_pre_hook, ln.register_full_backward_hook):
+        h = register(lambda *a: None)
+        assert not T.is_stock(ln, torch.nn.LayerNorm)
+        h.remove()
+    assert T.is_stock(ln, torch.nn.LayerNorm)
+    ln.forward = lambda t: t
+    assert not T.is_stock(ln, torch.nn.LayerNorm)
