@@ -1281,7 +1281,7 @@ def _tower_views(te, ids):
     }
 
 
-_VIEWS = ["grad", "vmap", "vmap of grad", "jvp", "dual", "fake", "traced", "compiled"]
+_VIEWS = ["grad", "vmap", "vmap of grad", "jvp", "dual", "fake", "second", "batched", "traced", "compiled"]
 
 
 @gpu
@@ -1335,3 +1335,89 @@ def test_what_is_taken_for_an_ordinary_pass():
     assert T.is_stock(ln, torch.nn.LayerNorm)
     ln.forward = lambda t: t
     assert not T.is_stock(ln, torch.nn.LayerNorm)
+
+
+def _gradients_case(kind, gate, post, res, given, dtype=torch.float64):
+    g = _gen(len(kind) + 3 * res)
+    r = lambda *s: torch.randn(*s, generator=g, dtype=torch.float64).to(dtype).requires_grad_()
+    t = dict(x=r(2, 3, 5), res=r(2, 3, 5) if res else None, gate=None if gate is None else r(5) if gate == "channel" else r(2, 5))
+    for k in ("pre", "post"):
+        there = k == "pre" or post
+        t[k + "_gamma"], t[k + "_beta"] = (r(5), r(5)) if there else (None, None)
+    return t, r(2, 3, 5) if "y" in given else None, r(2, 3, 5) if "s" in given else None
+
+
+@pytest.mark.parametrize("given", ["ys", "y", "s"])
+@pytest.mark.parametrize("kind,gate,post,res", [("layer", None, None, False), ("layer", "sample", "rms", True), ("rms", "channel", "layer", True), ("rms", "sample", None, False)])
+def test_block_norm_gradients_in_torch(kind, gate, post, res, given):
+    """The form that higher derivatives take, in 64 bits: equal to autograd of the definition (fewer than 200 roundings of 2^-53 of values
+    below 100), and differentiable itself."""
+    from geodiffuser_amd import training as T
+    t, gy, gs = _gradients_case(kind, gate, post, res, given)
+    names = {"d" + k: v for k, v in t.items() if v is not None}
+
+    def norm(v, kind, gamma, beta):
+        c = v - v.mean(-1, keepdim=True) if kind == "layer" else v
+        return c / (c.square().mean(-1, keepdim=True) + EPS).sqrt() * gamma + beta
+
+    h = t["x"] if post is None else norm(t["x"], post, t["post_gamma"], t["post_beta"])
+    h = h if gate is None else h * (t["gate"] if gate == "channel" else t["gate"][:, None])
+    s = h + 0.5 * t["res"] if res else h
+    y = norm(s, kind, t["pre_gamma"], t["pre_beta"])
+    outs = [(o, g) for o, g in ((y, gy), (s, gs)) if g is not None]
+    want = torch.autograd.grad([o for o, _ in outs], list(names.values()), [g for _, g in outs], allow_unused=True)
+
+    def grads(*leaves):
+        p = dict(zip(names, leaves))
+        pre = T.Norm(kind, p["dpre_gamma"], p["dpre_beta"], EPS)
+        po = T.Norm(post, p["dpost_gamma"], p["dpost_beta"], EPS) if post else None
+        d = T._block_norm_grads_in_torch(p["dx"], p.get("dres"), leaves[len(names)] if gy is not None else None, leaves[-1] if gs is not None else None, pre, po, p.get("dgate"), 0.5)
+        return tuple(d[k] for k in names)
+    leaves = list(names.values()) + [g for g in (gy, gs) if g is not None]
+    for k, a, b in zip(names, grads(*leaves), want):
+        assert a.shape == names[k].shape and float((a - (0 if b is None else b)).abs().max()) < 200 * 2.0 ** -53 * 100, k
+    assert torch.autograd.gradcheck(lambda *a: tuple(v for v in grads(*a) if v.requires_grad), leaves)
+
+
+def test_embedding_gradients_in_torch():
+    from geodiffuser_amd import training as T
+    ids = torch.tensor([[0, 3, -1, 2], [3, 9, 2, 2 ** 40]])
+    dy = torch.randn(2, 4, 3, generator=_gen(1), dtype=torch.float64, requires_grad=True)
+    for i in (ids, ids.clamp(max=9).int()):
+        table, pos = T._embed_grads_in_torch(i, dy, 5, 6, 0.5, 2)
+        want = torch.zeros(5, 3, dtype=torch.float64)
+        want[0], want[3] = 0.5 * dy[0, 0], 0.5 * (dy[0, 1] + dy[1, 0])
+        assert torch.allclose(table, want, rtol=0, atol=1e-15) and torch.equal(pos, torch.cat([dy.sum(0), torch.zeros(2, 3, dtype=torch.float64)]))
+        assert torch.autograd.gradcheck(lambda d: T._embed_grads_in_torch(i, d, 5, 6, 0.5, 2), (dy,))
+    assert T._embed_grads_in_torch(ids[0], dy[0], 0, None, 1.0, None)[0].shape == (0, 3) and T._embed_grads_in_torch(ids[:0], dy[:0], 4, 4, 1.0, None)[1].sum() == 0
+
+
+@gpu
+def test_second_derivatives_of_the_training_operators(ops):
+    """Embedding, then a gated block norm with both norms: second derivatives against the same in 64 bits on the CPU.  f32: 2 * 400 roundings of
+    2^-24 in relative 2-norm for all of them together."""
+    from geodiffuser_amd import training as T
+    g = _gen(31)
+    ids = torch.randint(0, 20, (3, 6), generator=g)
+    init = dict(table=_randn(g, 20, 24, dev="cpu"), pos=_randn(g, 6, 24, dev="cpu"), gate=_randn(g, 3, 24, dev="cpu"), g1=_randn(g, 24, dev="cpu"), b1=_randn(g, 24, dev="cpu"),
+                g2=_randn(g, 24, dev="cpu"), w=_randn(g, 24, 24, dev="cpu"))
+    t = {k: _randn(g, *v.shape, dev="cpu") for k, v in init.items()}
+
+    def norm(v, kind, gamma, beta=0.0):
+        c = v - v.mean(-1, keepdim=True) if kind == "layer" else v
+        return c / (c.square().mean(-1, keepdim=True) + EPS).sqrt() * gamma + beta
+
+    def second(dev, dtype):
+        p = {k: v.to(dev, dtype).requires_grad_() for k, v in init.items()}
+        if dev == "cpu":
+            x = 2.0 * torch.nn.functional.embedding(ids, p["table"]) + p["pos"]
+            s = 0.5 * x + p["gate"][:, None] * norm(x @ p["w"], "rms", p["g2"])
+            y = norm(s, "layer", p["g1"], p["b1"])
+        else:
+            x = T.embed_tokens(ids.to(dev), p["table"], p["pos"], 2.0)
+            s, y = T.block_norm(x @ p["w"], x, T.Norm("layer", p["g1"], p["b1"], EPS), post=T.Norm("rms", p["g2"], None, EPS), gate=p["gate"], res_scale=0.5)
+        first = torch.autograd.grad(y.pow(3).mean() + s.square().mean(), list(p.values()), create_graph=True)
+        z = sum((a * t[k].to(dev, dtype)).sum() for a, k in zip(first, p))
+        return torch.cat([a.detach().cpu().double().flatten() for a in (*first, *torch.autograd.grad(z, list(p.values())))])
+    got, want = second(DEV, torch.float32), second("cpu", torch.float64)
+    assert float((got - want).norm()) <= 2 * 400 * U32 * float(want.norm())
