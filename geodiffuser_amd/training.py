@@ -174,11 +174,23 @@ def layer_norm_of(module: torch.nn.LayerNorm) -> Norm:
     return Norm("layer", module.weight, module.bias, module.eps)
 
 
+def _as_it_lies(grad):
+    """A dense gradient's elements in the order of memory, whatever the order of its axes (a transposed parameter's gradient is transposed too):
+    norm and scaling do not ask for more."""
+    grad = grad.detach()
+    if grad.is_contiguous() or not torch.ops.aten.is_non_overlapping_and_dense(grad):
+        return grad
+    return grad.as_strided((grad.numel(),), (1,))
+
+
 def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: float, norm_type: float = 2.0):
     """torch.nn.utils.clip_grad_norm_ on ``ops.clip_grad_norm``: scales the parameters' gradients in place so that their joint norm is at most
-    ``max_norm`` -> the norm before (0-d tensor on the device, nothing is synchronised; 0 if no parameter has a gradient)."""
+    ``max_norm`` -> the norm before (0-d tensor on the device, nothing is synchronised; 0 if no parameter has a gradient).
+
+    Gradients: f16 / bf16 / f32, mixed as they come, dense in any order of their axes, all on one GPU; ``norm_type`` 2 or inf.  A parameter
+    listed twice is refused (torch counts and scales its gradient twice)."""
     params = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
     grads = [p.grad for p in params if p.grad is not None]
     if not grads:
-        return torch.zeros(())
-    return ops.clip_grad_norm([g.detach() for g in grads], max_norm, norm_type)
+        return torch.zeros((), device=params[0].device if params else None)
+    return ops.clip_grad_norm([_as_it_lies(g) for g in grads], max_norm, norm_type)

@@ -1421,3 +1421,37 @@ def test_second_derivatives_of_the_training_operators(ops):
         return torch.cat([a.detach().cpu().double().flatten() for a in (*first, *torch.autograd.grad(z, list(p.values())))])
     got, want = second(DEV, torch.float32), second("cpu", torch.float64)
     assert float((got - want).norm()) <= 2 * 400 * U32 * float(want.norm())
+
+
+@gpu
+def test_clip_grad_norm_of_gradients_in_any_dense_order(ops):
+    """Parameters whose axes lie in another order have gradients that do too: the norm and every value as torch's function has them."""
+    from geodiffuser_amd import training as T
+    for kind in (2.0, math.inf):
+        g = _gen(4)
+        flat = _randn(g, 6000)
+        params = [torch.nn.Parameter(p) for p in (
+            _randn(g, 40, 65).t(), _randn(g, 4, 3, 5, 7, 6).to(memory_format=torch.channels_last_3d), _randn(g, 5, 6, 7).permute(2, 0, 1), _randn(g, 9, 2, 4).transpose(0, 1),
+            flat[1001:1001 + 24].view(4, 6).t(), _randn(g, 1, 7, dtype=torch.bfloat16).t(), _randn(g, 8, 6, dtype=torch.float16).t(), _randn(g, 33))]
+        sum((p.float() * p.float().sin()).sum() for p in params).backward()
+        assert sum(not p.grad.is_contiguous() for p in params) >= 6
+        ref, versions = [p.grad.clone() for p in params], [p.grad._version for p in params]
+        total = float(_norm_ref(ref, kind))
+        n = T.clip_grad_norm_(params, total / 7, kind)
+        assert abs(float(n) - total) <= 2 * U32 * total
+        for p, r, v in zip(params, ref, versions):
+            assert p.grad.stride() == r.stride() and p.grad._version > v
+            want = r.double() * (total / 7 / (total + 1e-6))
+            _close(p.grad, want, 4, want.abs())                               # the norm to f32 in the test's factor, the factor, the product
+    p = torch.nn.Parameter(torch.ones(4, 6, device=DEV))
+    p.grad = torch.ones(8, 6, device=DEV)[::2]                                # gaps: not dense
+    with pytest.raises(GeodiffError, match="contiguous"):
+        T.clip_grad_norm_(p, 1.0)
+    p.grad = torch.ones(4, 1, device=DEV).expand(4, 6)
+    with pytest.raises(GeodiffError, match="contiguous"):
+        T.clip_grad_norm_(p, 1.0)
+    p.grad = torch.ones(4, 6, device=DEV)
+    with pytest.raises(GeodiffError, match="overlaps"):
+        T.clip_grad_norm_([p, p], 1.0)
+    p.grad = None
+    assert T.clip_grad_norm_([p], 1.0).device == p.device and float(T.clip_grad_norm_([], 1.0)) == 0.0
