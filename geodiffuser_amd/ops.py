@@ -1360,12 +1360,13 @@ def _grad_norm(grads, norm_type, max_norm, out):
                     or not (dense and all(map(torch.Tensor.is_contiguous, out)) or all(o.stride() == t.stride() for o, t in zip(out, grads)))):
                 raise _lib.GeodiffError("clip_grad_norm: out needs a tensor of the same shape, strides, dtype and device for each gradient")
             dst = (ctypes.c_void_p * n)(*map(torch.Tensor.data_ptr, out))
-        torch._C._increment_version(grads if out is None else out)       # what autograd saved of them is no longer what it was
     where = grads[0].device
     nbytes = lib.gd_grad_norm_workspace_bytes()
     ws = torch.empty(nbytes, dtype=torch.uint8, device=where)
     norm = torch.empty((), dtype=torch.float32, device=where)
     _launch(lib.gd_grad_norm, "gd_grad_norm", dev, src, dst, numel, dts, n, int(norm_type != 2.0), max_norm or 0.0, ws.data_ptr(), nbytes, norm.data_ptr())
+    if dst is not None:
+        torch._C._increment_version(grads if out is None else out)       # what autograd saved of them is no longer what it was
     return norm
 
 

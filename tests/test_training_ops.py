@@ -1455,3 +1455,19 @@ def test_clip_grad_norm_of_gradients_in_any_dense_order(ops):
         T.clip_grad_norm_([p, p], 1.0)
     p.grad = None
     assert T.clip_grad_norm_([p], 1.0).device == p.device and float(T.clip_grad_norm_([], 1.0)) == 0.0
+
+
+@gpu
+def test_refused_clipping_leaves_its_tensors_as_they_were(ops):
+    """A call that the library refuses has written nothing, and autograd is not told otherwise."""
+    t, o = torch.ones(6, device=DEV), torch.ones(6, device=DEV)
+    for call in (lambda: ops.clip_grad_norm([t, t], 1.0), lambda: ops.clip_grad_norm([t, o], 1.0, out=[o, torch.empty_like(t)])):
+        v = t._version, o._version
+        with pytest.raises(GeodiffError, match="overlaps"):
+            call()
+        assert (t._version, o._version) == v and bool((t == 1).all())
+    v = t._version, o._version
+    ops.clip_grad_norm([t], 1.0, out=[o])
+    assert t._version == v[0] and o._version > v[1]
+    ops.clip_grad_norm([t], 1.0)
+    assert t._version > v[0]
