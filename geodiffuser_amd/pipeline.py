@@ -75,7 +75,7 @@ class TextEncoder(nn.Module):
         tok = self.tok                                       # anything that changes what the module does keeps its own call
         stock = (training.in_plain_torch(input_ids, w, pos) and training.is_stock(tok, nn.Embedding) and tok.padding_idx is None and tok.max_norm is None
                  and not tok.sparse and not tok.scale_grad_by_freq)
-        if stock and w.is_cuda and input_ids.device == pos.device == w.device and w.dtype in (torch.float16, torch.bfloat16, torch.float32) and w.is_contiguous():
+        if stock and input_ids.dim() == 2 and w.is_cuda and input_ids.device == pos.device == w.device and w.dtype in (torch.float16, torch.bfloat16, torch.float32) and w.is_contiguous():
             return training.embed_tokens(input_ids.contiguous(), w, pos.contiguous())
         return self.tok(input_ids) + pos[: input_ids.shape[1]]
 

@@ -1471,3 +1471,12 @@ def test_refused_clipping_leaves_its_tensors_as_they_were(ops):
     assert t._version == v[0] and o._version > v[1]
     ops.clip_grad_norm([t], 1.0)
     assert t._version > v[0]
+
+
+@gpu
+def test_text_tower_takes_a_batch_of_prompts_only(ops):
+    """Ids without a batch axis end where the unfused addition ends them, on the GPU as on the CPU."""
+    for dev in ("cpu", DEV):
+        te = _small_tower(dev)
+        with pytest.raises(IndexError):
+            te(torch.zeros(32, dtype=torch.long, device=dev))
