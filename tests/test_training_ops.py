@@ -1480,3 +1480,102 @@ def test_text_tower_takes_a_batch_of_prompts_only(ops):
         te = _small_tower(dev)
         with pytest.raises(IndexError):
             te(torch.zeros(32, dtype=torch.long, device=dev))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("C", [1, 5, 8, 24, 65, 333, 513, 1027, 2056, 4097])
+def test_results_do_not_depend_on_where_they_lie(ops, monkeypatch, dtype, C):
+    """Outputs at an address that is a multiple of the element only, and inputs there: the embeddings' bits are those of the ordinary call, the
+    norms' results as near to the 64-bit ones as any."""
+    g = _gen(C)
+    V, B, L, P = 23, 5, 4, 7
+    ids, table, pos, dy = torch.randint(0, V, (B, L), generator=g).to(DEV), _randn(g, V, C, dtype=dtype), _randn(g, P, C, dtype=dtype), _randn(g, B, L, C, dtype=dtype)
+    many, dmany = torch.randint(0, V, (1100,), generator=g).to(DEV), _randn(g, 1100, C, dtype=dtype)
+    dbatch = _randn(g, 130, L, C, dtype=dtype)
+    embed = lambda mis: [ops.embed_tokens(ids, mis(table), mis(pos), 3.0), ops.embed_tokens_bwd(ids, mis(dy), V), ops.embed_tokens_bwd(many, mis(dmany), V),
+                         ops.embed_positions_bwd(mis(dy), P), ops.embed_positions_bwd(mis(dbatch), P)]
+    x, r, pre, po, gt, gy, gs = _block_case(ops, (B, L, C), dtype, "layer", "sample", True, True, C)
+
+    def norms(mis):
+        n, p = (ops.Norm(t.kind, mis(t.gamma), mis(t.beta), t.eps) for t in (pre, po))
+        s, y, stats = ops.block_norm(mis(x), mis(r), n, p, mis(gt), 0.5)
+        return {"s": s, "y": y, **ops.block_norm_bwd(mis(x), mis(r), mis(gy), mis(gs), stats, n, p, mis(gt), 0.5)}
+    same = lambda t: t
+    want, (v, m) = embed(same), _block_ref(x, r, pre, po, gt, 0.5, gy, gs)
+    moved_inputs = embed(_misaligned), norms(_misaligned)
+    empty = torch.empty
+
+    def inside(*shape, dtype=torch.float32, device=None):
+        shape = torch.Size(shape[0] if len(shape) == 1 and not isinstance(shape[0], int) else shape)
+        front = 64 if dtype == torch.uint8 else 33                               # (workspaces keep their alignment)
+        return empty(front + shape.numel(), dtype=dtype, device=device)[front:].view(shape)
+    monkeypatch.setattr(torch, "empty", inside)
+    monkeypatch.setattr(torch, "empty_like", lambda t: inside(*t.shape, dtype=t.dtype, device=t.device))
+    moved_outputs = embed(same), norms(same)
+    monkeypatch.undo()
+    for e, n in (moved_inputs, moved_outputs):
+        assert all(torch.equal(a, b) for a, b in zip(e, want))
+        for k, t in n.items():
+            _close(t, v[k], (1 if k in ("s", "y") else 2) * K_ROW + (B * L if k[1:] in ("gate", "pre_gamma", "pre_beta", "post_gamma", "post_beta") else 0), m[k], k)
+
+
+@gpu
+@pytest.mark.parametrize("n,V", [((1 << 20) + 1, 300), (1400000, 50000), (1300000, 100001)])
+def test_embedding_gradient_of_more_positions_than_a_sort_keeps_in_registers(ops, n, V):
+    """More than 2048 positions a workgroup of the sort, two and three passes of it, half of them one token.  Whole numbers up to 8 as gradients: sums
+    of a million of them are exact in 32 bits in any order, and a position at a wrong place shows."""
+    g = torch.Generator(device=DEV).manual_seed(n)
+    ids = torch.randint(0, V, (n,), generator=g, device=DEV)
+    ids[torch.rand(n, generator=g, device=DEV) < 0.5] = V // 3
+    dy = torch.randint(-8, 9, (n, 5), generator=g, device=DEV).float()
+    ref = torch.stack([torch.bincount(ids.cpu(), weights=col.double(), minlength=V) for col in dy.cpu().t()], 1).to(DEV)
+    for i in (ids, ids.int()):
+        assert torch.equal(ops.embed_tokens_bwd(i, dy, V).double(), ref)
+    ref[V // 3] = 0
+    assert torch.equal(ops.embed_tokens_bwd(ids, dy, V, padding_idx=V // 3).double(), ref)
+
+
+@gpu
+def test_null_text_optimiser_sees_clipped_gradients(ops, monkeypatch):
+    """What Adam is handed in NullInversion(max_grad_norm=...): gradients of that norm where they were longer, the gradients themselves where
+    not.  f32 or f16 gradients: the clipped norm is off by the factor's and each element's rounding, at most (2 2^-24 + u) of it."""
+    import cases
+    from geodiffuser_amd import inversion, training as T
+    from geodiffuser_amd.diffusion import load_model
+    p, tok, sched = load_model(device="cuda:0", tiny=True, dtype=torch.float16)
+    c = cases.NULL_TEXT
+    traj = [torch.from_numpy(a).cuda().half() for a in cases.null_text_inputs()]
+    before, after = [], []
+    real, step = T.clip_grad_norm_, torch.optim.Adam.step
+
+    def clip(ps, limit):
+        grad = ps.grad.clone()
+        n = real(ps, limit)
+        before.append((float(n), float(grad.double().norm()), grad))
+        return n
+
+    def look(self, *a, **k):
+        after.append(self.param_groups[0]["params"][0].grad.clone())
+        return step(self, *a, **k)
+    monkeypatch.setattr(T, "clip_grad_norm_", clip)
+    monkeypatch.setattr(torch.optim.Adam, "step", look)
+
+    def run(limit):
+        before.clear(), after.clear()
+        ni = inversion.NullInversion(p, num_ddim_steps=c["steps"], device="cuda:0", guidance_scale=c["guidance"], max_grad_norm=limit)
+        ni.init_prompt("")
+        ni.null_optimization(traj, c["inner"], c["eps"])
+        assert after and (limit is None or len(before) == len(after))
+
+    run(None)
+    assert not before
+    first = float(after[0].double().norm())
+    run(1e9)
+    assert first > 0 and all(torch.equal(g, a) and abs(n - e) <= 2 * U32 * e for (n, e, g), a in zip(before, after))
+    limit = first / 4
+    run(limit)
+    u = 0.0 if after[0].dtype == torch.float32 else torch.finfo(after[0].dtype).eps / 2
+    assert before[0][0] > limit
+    for (n, e, g), a in zip(before, after):
+        assert abs(float(a.double().norm()) - min(e, limit)) <= (4 * U32 + u) * limit + 1e-6
