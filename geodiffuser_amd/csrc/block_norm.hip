@@ -11,9 +11,10 @@
 //   dres = alpha ds;   dgate = sum ds h;   dh = gate ds;   dx = N'(dh * gamma_post, xh_x) or dh
 //   dgamma = sum g_out xh, dbeta = sum g_out over all rows, for each of the two norms.
 //
-// Bound by HBM: the forward reads x, res and writes s, y once, the backward reads x, res, gy, gs and writes dx, dres once.  A row stays in
-// registers from its load to its last use (64 / 256 / 1024 threads a row, 8 or 16 channels a thread), so that the two-pass variance and
-// both norms cost no second read.  Everything between the loads and the one rounding of each result is binary32; y comes from the sum s
+// Bound by HBM: the forward reads x, res and writes s, y once, the backward reads x, res, gy, gs and writes dx, dres once (above 4096
+// channels it reads them a second time for the sums of a gate or a norm on x: a launch of their own).  A row stays in registers from its
+// load to its last use (64 / 256 / 512 / 1024 threads a row, 8 or 16 channels a thread), so that the two-pass variance and both norms cost
+// no second read.  Everything between the loads and the one rounding of each result is binary32; y comes from the sum s
 // BEFORE its rounding, and the backward recomputes that sum from x and res instead of reading the rounded s: the gradients are those of
 // the function that the forward computed, at the same traffic.
 //
@@ -280,8 +281,7 @@ template <typename T, int TPR, int N, int MODE, bool WRAP, int SUMS>
 __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) k_block_norm_bwd(const bn_bwd_args b) {
     using PART = bn_part<T, TPR, N, MODE>;
     constexpr int RPB = TPR < 256 ? 256 / TPR : 1;
-    // the next row's data beside this one's and the parameters over all rows, where the registers hold them: 8 waves and 16 channels a
-    // thread leave none
+    // the next row's data beside this one's and the parameters over all rows, where the registers hold them: 1024 threads a row leave none
     constexpr bool AHEAD = TPR * N < 8192;
     __shared__ float lds[TPR < 256 ? 4 * 64 * N : 64];
     int turn = 0;
@@ -479,6 +479,7 @@ static int bn_check(const gd_block_norm_t* f, int dtype, const char* who) {
     GD_REQUIRE((f->post_kind || (!f->post_gamma && !f->post_beta)) && (f->pre_kind || (!f->pre_gamma && !f->pre_beta)), GD_EINVAL, "%s: gamma or beta without its norm", who);
     GD_REQUIRE(!f->gate || (f->rows_per_gate > 0 && f->rows % f->rows_per_gate == 0 && f->gate_ld >= f->C), GD_EINVAL,
                "%s: gate rows must divide the rows and be at least C apart", who);
+    // (the backward's column sums have a row of workgroups for each; the forward refuses what could not be differentiated)
     GD_REQUIRE(!f->gate || f->rows / f->rows_per_gate <= 65535 - BN_SUMS, GD_EUNSUPPORTED, "%s: at most %d gate rows", who, 65535 - BN_SUMS);
     GD_REQUIRE(dtype == GD_F16 || dtype == GD_BF16 || dtype == GD_F32, GD_EINVAL, "%s: dtype must be f16/bf16/f32", who);
     return GD_OK;

@@ -749,7 +749,7 @@ static bool em_vec(int C, int elem) { return C * elem >= 16; }
 #define EM_ELEM(dtype) ((dtype) == GD_F32 ? 4 : 2)
 
 static int em_check(int64_t n, int64_t vocab, int C, int dtype, const char* who) {
-    GD_REQUIRE(n >= 0 && n < (1ll << 30), GD_EUNSUPPORTED, "%s: %lld positions (at most 2^30)", who, (long long)n);
+    GD_REQUIRE(n >= 0 && n < (1ll << 30), GD_EUNSUPPORTED, "%s: %lld positions (less than 2^30)", who, (long long)n);
     GD_REQUIRE(vocab > 0 && vocab < (1ll << 31) - 1, GD_EUNSUPPORTED, "%s: a table of %lld rows", who, (long long)vocab);
     GD_REQUIRE(C > 0 && C <= (1 << 20), GD_EUNSUPPORTED, "%s: C=%d", who, C);
     GD_REQUIRE(dtype == GD_F16 || dtype == GD_BF16 || dtype == GD_F32, GD_EINVAL, "%s: dtype must be f16/bf16/f32", who);

@@ -205,7 +205,7 @@ class NullInversion:
         return (image_gt, image_rec), ddim_latents[-1], uncond_embeddings, ddim_latents, ddim_noise
 
     def __init__(self, model, num_ddim_steps=50, uncond_text="", device="cuda:0", progress_bar=None, guidance_scale=3.0, max_grad_norm=None):
-        """``max_grad_norm``: null-text optimisation clips its embedding's gradient to this norm before each Adam step (None, as the
+        """``max_grad_norm``: null-text optimisation clips its embedding's gradient to this norm before each Adam step, on the GPU (None, as the
         reference: no clipping)."""
         self.guidance_scale = guidance_scale
         self.max_grad_norm = max_grad_norm

@@ -1092,8 +1092,7 @@ def conv3x3(x, w, bias=None, stride: int = 1, upsample: bool = False, res=None):
 # ---------------------------------------------------------------------------------------------------
 # Training side: token embedding, block norms, gradient clipping (embed.hip, block_norm.hip, grad_clip.hip).  f16 / bf16 / f32.  The
 # autograd forms are in training.py.  A call runs on its tensors' device (whichever device is current) and that device's current stream.
-# At a prompt's sizes a call is bound by this file, not by its kernel: hence plain integers for pointers, the raw stream handle, and one
-# buffer behind several small outputs.
+# At a prompt's sizes a call is bound by this file, not by its kernel: hence plain integers for pointers and the raw stream handle.
 # ---------------------------------------------------------------------------------------------------
 def _launch(fn, what: str, dev: int, *args) -> None:
     """fn(*args, current stream of GPU ``dev``), with that GPU current."""
@@ -1140,8 +1139,8 @@ def _token_ids(ids: torch.Tensor, ref: torch.Tensor) -> int:
 
 
 def embed_tokens(ids, table, pos=None, scale: float = 1.0):
-    """y = scale * table[ids] + pos[:L]: ids int64 / int32 [..., L], table [V, C], pos [>= L, C] or None -> [..., L, C].  One rounding.  An id
-    outside the table gives a row of NaN (nothing is read there, and the device is not synchronised to raise)."""
+    """y = scale * table[ids] + pos[:L]: ids int64 / int32 [..., L], table [V, C], pos [>= L, C] or None -> [..., L, C], of less than 2^30 ids and
+    C <= 2^20.  One rounding.  An id outside the table gives a row of NaN (nothing is read there, and the device is not synchronised to raise)."""
     lib = _lib.load()
     _need(table, "table")
     dt = _dt(table, "table")
@@ -1262,7 +1261,7 @@ def block_norm(x, res, pre: Optional[Norm], post: Optional[Norm] = None, gate=No
         s = res_scale * res + gate * post(x),   y = pre(s)            -> (s, y, stats)
 
     x, res [..., C] (res None: nothing is added; with neither gate nor post, s is then x itself), C <= 16384; gate [C], or [x.shape[0], C]
-    with a row for each sample (its rows may be strided); pre / post: ``Norm`` or None (pre None: y is None).  y is computed from the
+    with a row for each sample (at most 65531; its rows may be strided); pre / post: ``Norm`` or None (pre None: y is None).  y is computed from the
     unrounded sum; stats [rows, 4] f32 is what ``block_norm_bwd`` needs."""
     lib = _lib.load()
     dt, shape, C, rows, dev = _block_norm_x(x)

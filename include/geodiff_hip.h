@@ -541,12 +541,12 @@ int gd_copy_rows(const gd_copy_rows_t* entries, int n, int row, int64_t max_byte
  * for the gradient norm), one rounding of each result, fixed summation orders (no float atomics).
  * ---------------------------------------------------------------------------------------------- */
 
-/* y[i] = scale * table[ids[i]] + pos[i mod L] for n positions: table [vocab, C], pos [>= L, C] or NULL, y [n, C], ids int64 (ids64 = 1) or
+/* y[i] = scale * table[ids[i]] + pos[i mod L] for n < 2^30 positions of C <= 2^20 channels: table [vocab, C], pos [>= L, C] or NULL, y [n, C], ids int64 (ids64 = 1) or
  * int32.  An id outside [0, vocab) gives a row of NaN. */
 int gd_embed(const void* ids, int ids64, int64_t n, const void* table, int64_t vocab, const void* pos, int L, int C, float scale, void* y, int dtype,
              void* stream);
 /* dtable[v] = scale * sum of dy[i] over the positions with ids[i] = v, for EVERY row v of the table (zeros where there is none, and in
- * row `padding`; -1: no such row); ids outside the table add nothing. */
+ * row `padding`; -1: no such row); ids outside the table add nothing.  (Refused from about 2^30 - 2^24 positions on.) */
 size_t gd_embed_bwd_workspace_bytes(int64_t n, int64_t vocab, int C);
 int gd_embed_bwd(const void* ids, int ids64, int64_t n, const void* dy, int64_t vocab, int C, int64_t padding, float scale, void* dtable,
                  void* workspace, size_t workspace_bytes, int dtype, void* stream);
@@ -556,8 +556,8 @@ int gd_embed_pos_bwd(const void* dy, int64_t B, int L, int C, int pos_rows, void
 
 /* h = post(x);  s = res_scale * res + gate * h;  y = pre(s) for rows of C <= 16384 channels.
  *   kinds: GD_NORM_NONE, GD_NORM_LAYER (xh = (v - mean) / sqrt(var + eps)), GD_NORM_RMS (xh = v / sqrt(mean v^2 + eps)), then
- *   xh * gamma + beta; gamma, beta [C] or NULL (1, 0), NULL without the norm.  gate: one row of C for every rows_per_gate rows, gate_ld elements apart, or
- *   NULL (1).  res NULL: s = gate * h.  s may be NULL; y goes with pre_kind.  stats [rows, 4] f32 (mean, 1 / deviation of x, then of
+ *   xh * gamma + beta; gamma, beta [C] or NULL (1, 0), NULL without the norm.  gate: one row of C for every rows_per_gate rows (at most 65531 gate
+ *   rows), gate_ld elements apart, or NULL (1).  res NULL: s = gate * h.  s may be NULL; y goes with pre_kind.  stats [rows, 4] f32 (mean, 1 / deviation of x, then of
  *   s; 0, 1 for a norm that is not there; NULL: not kept) is what the backward needs.  y is computed from the unrounded s.
  *   No output may overlap an input. */
 enum { GD_NORM_NONE = 0, GD_NORM_LAYER = 1, GD_NORM_RMS = 2 };
