@@ -49,10 +49,11 @@ class _TextLayer(nn.Module):
         self.fc1, self.fc2 = nn.Linear(d, 4 * d), nn.Linear(4 * d, d)
 
     def forward(self, x, mask):
-        if training.fuses_norms(x, (self.ln1, self.ln2)):    # a pass that learns them: residual add and norms fused, with their gradients
-            x, h = training.block_norm(x, None, training.layer_norm_of(self.ln1))
-            x, h = training.block_norm(self.attn(h, h, h, attn_mask=mask, need_weights=False)[0].contiguous(), x, training.layer_norm_of(self.ln2))
-            return x + self.fc2(F.gelu(self.fc1(h)))
+        if not torch.jit.is_scripting():
+            if training.fuses_norms(x, (self.ln1, self.ln2)):        # a pass that learns them: residual add and norms fused, with their gradients
+                x, h = training.block_norm(x, None, training.layer_norm_of(self.ln1))
+                x, h = training.block_norm(self.attn(h, h, h, attn_mask=mask, need_weights=False)[0].contiguous(), x, training.layer_norm_of(self.ln2))
+                return x + self.fc2(F.gelu(self.fc1(h)))
         h = self.ln1(x)
         x = x + self.attn(h, h, h, attn_mask=mask, need_weights=False)[0]
         return x + self.fc2(F.gelu(self.fc1(self.ln2(x))))
@@ -71,12 +72,13 @@ class TextEncoder(nn.Module):
     def _embed(self, input_ids):
         """Token + position embedding: one launch on the GPU (gd_embed, the same rounding), with its gradient where table or positions learn.  An id
         outside the table gives a row of NaN there."""
-        w, pos = self.tok.weight, self.pos.to(self.tok.weight.dtype)
-        tok = self.tok                                       # anything that changes what the module does keeps its own call
-        stock = (training.in_plain_torch(input_ids, w, pos) and training.is_stock(tok, nn.Embedding) and tok.padding_idx is None and tok.max_norm is None
-                 and not tok.sparse and not tok.scale_grad_by_freq)
-        if stock and input_ids.dim() == 2 and w.is_cuda and input_ids.device == pos.device == w.device and w.dtype in (torch.float16, torch.bfloat16, torch.float32) and w.is_contiguous():
-            return training.embed_tokens(input_ids.contiguous(), w, pos.contiguous())
+        pos = self.pos.to(self.tok.weight.dtype)
+        if not torch.jit.is_scripting():
+            tok, w = self.tok, self.tok.weight               # anything that changes what the module does keeps its own call
+            stock = (training.in_plain_torch(input_ids, w, pos) and training.is_stock(tok, nn.Embedding) and tok.padding_idx is None and tok.max_norm is None
+                     and not tok.sparse and not tok.scale_grad_by_freq)
+            if stock and input_ids.dim() == 2 and w.is_cuda and input_ids.device == pos.device == w.device and w.dtype in (torch.float16, torch.bfloat16, torch.float32) and w.is_contiguous():
+                return training.embed_tokens(input_ids.contiguous(), w, pos.contiguous())
         return self.tok(input_ids) + pos[: input_ids.shape[1]]
 
     def forward(self, input_ids):

@@ -1579,3 +1579,13 @@ def test_null_text_optimiser_sees_clipped_gradients(ops, monkeypatch):
     assert before[0][0] > limit
     for (n, e, g), a in zip(before, after):
         assert abs(float(a.double().norm()) - min(e, limit)) <= (4 * U32 + u) * limit + 1e-6
+
+
+@pytest.mark.parametrize("dev", ["cpu", pytest.param(DEV, marks=gpu)])
+def test_text_tower_is_scriptable(dev):
+    """torch.jit.script compiles the tower (its plain operations) and gives its values; f32: the 60 * 16 roundings of a pass."""
+    te = _small_tower(dev).eval()
+    te.layers[0].attn = torch.nn.MultiheadAttention(32, 2, batch_first=True).to(dev).eval()
+    ids = torch.randint(0, 50, (2, 9), generator=_gen(1)).to(dev)
+    got, want = torch.jit.script(te)(ids)[0], te(ids)[0]
+    assert float((got - want).norm()) <= 60 * 16 * U32 * float(want.norm())
